@@ -1,0 +1,130 @@
+"""ctypes binding of libss_sequence.so (include/ss_sequence.h): the sequence operators' only way to their kernels.
+
+As with the neuron library there is no fallback: a missing library, a CPU tensor or an operand of another type raises SSNeuronError.
+"""
+import ctypes as C
+import os
+
+import torch  # before the CDLL, so that one HIP runtime is shared
+
+from ._lib import SSNeuronError, _check, _stream
+
+_PKG = os.path.dirname(os.path.abspath(__file__))
+LIB_PATH = os.path.join(_PKG, 'lib', 'libss_sequence.so')
+ABI_VERSION = 1
+DT_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+MAX_HEAD_DIM = 256
+MAX_NORM_WIDTH = 16384
+MAX_INT8_K = 131071
+
+_lib = None
+
+
+class LeakyDesc(C.Structure):
+    """struct ss_seq_leaky_desc (include/ss_sequence.h)."""
+    _fields_ = ([('size', C.c_uint), ('dtype', C.c_int), ('out_dtype', C.c_int)] + [(n, C.c_int) for n in ('T', 'B', 'H', 'DA', 'DC', 'reverse')] +
+                [('b_scale', C.c_float), ('o_scale', C.c_float)] + [(n, C.c_void_p) for n in ('a', 'b', 'c', 'out')] +
+                [(f'{n}_{s}', C.c_longlong) for n in 'abco' for s in 'tbh'] + [(f'{n}_group', C.c_int) for n in 'abc'] +
+                [('log_decay', C.c_void_p), ('lengths', C.c_void_p), ('s_in', C.c_void_p), ('s_out', C.c_void_p)] +
+                [(n, C.c_int) for n in ('s_in_row', 's_in_col', 's_out_row', 's_out_col')] + [('ws', C.c_void_p)])
+
+
+EXPORTS = ('ss_seq_abi_version', 'ss_seq_leaky_ws_floats', 'ss_seq_leaky', 'ss_seq_group_sum', 'ss_seq_rms_norm_fwd', 'ss_seq_rms_norm_ws_floats',
+           'ss_seq_rms_norm_bwd', 'ss_seq_rms_norm_int8', 'ss_seq_dequant_int8', 'ss_seq_int8_linear_ws_ints', 'ss_seq_int8_linear')
+
+
+def lib():
+    """Load (once) and return the library.  Raises loudly when it has not been built."""
+    global _lib
+    if _lib is not None:
+        return _lib
+    if not os.path.exists(LIB_PATH):
+        raise SSNeuronError(f'{LIB_PATH} not found: the HIP extension is not built.  Run `python -c "import __graft_entry__ as g; g.build()"` or '
+                            f'`make -C stereospike_amd/csrc` (hipcc --offload-arch=gfx950).  There is no CPU fallback.')
+    L = C.CDLL(LIB_PATH)
+    p, i32, i64, f32, desc = C.c_void_p, C.c_int, C.c_longlong, C.c_float, C.POINTER(LeakyDesc)
+    for name, res, args in (('ss_seq_abi_version', i32, []), ('ss_seq_leaky_ws_floats', i64, [desc]), ('ss_seq_leaky', i32, [desc, p]),
+                            ('ss_seq_group_sum', i32, [p, p, i64, i32, i32, i32, p]),
+                            ('ss_seq_rms_norm_fwd', i32, [p, i64, p, i64, p, p, p, p, i64, i32, f32, i32, p]),
+                            ('ss_seq_rms_norm_ws_floats', i64, [i64, i32, i32]),
+                            ('ss_seq_rms_norm_bwd', i32, [p, p, p, p, p, p, p, p, i64, i32, i32, p]),
+                            ('ss_seq_rms_norm_int8', i32, [p, i64, p, i64, p, p, p, p, i64, i32, f32, i32, p]),
+                            ('ss_seq_dequant_int8', i32, [p, p, p, i64, i32, i32, p]),
+                            ('ss_seq_int8_linear_ws_ints', i64, [i64, i32, i32]),
+                            ('ss_seq_int8_linear', i32, [p, i64, p, p, i64, p, p, p, i64, i32, i32, i32, p, p])):
+        f = getattr(L, name)
+        f.restype, f.argtypes = res, args
+    if L.ss_seq_abi_version() != ABI_VERSION:
+        raise SSNeuronError(f'libss_sequence.so ABI {L.ss_seq_abi_version()} != expected {ABI_VERSION}; rebuild')
+    _lib = L
+    return _lib
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def leaky(a, b, c, out, log_decay, b_scale, o_scale, reverse=False, lengths=None, s_in=None, s_in_t=False, s_out=None, s_out_t=False):
+    """One leaky map (struct ss_seq_leaky_desc): a, b, c, out [T, B, heads, D] views with a contiguous last axis; states [B, H, rows, columns] contiguous, or
+    transposed (`*_t`: the matrix is stored [DC, DA])."""
+    T, B, H, DC = out.shape
+    DA = a.shape[3]
+    d = LeakyDesc(size=C.sizeof(LeakyDesc), dtype=DT_CODE[a.dtype], out_dtype=DT_CODE[out.dtype], T=T, B=B, H=H, DA=DA, DC=DC, reverse=int(reverse),
+                  b_scale=b_scale, o_scale=o_scale, a=a.data_ptr(), b=b.data_ptr(), c=c.data_ptr(), out=out.data_ptr(),
+                  a_group=H // a.shape[2], b_group=H // b.shape[2], c_group=H // c.shape[2], log_decay=log_decay.data_ptr(), lengths=_p(lengths),
+                  s_in=_p(s_in), s_out=_p(s_out), s_in_row=1 if s_in_t else DC, s_in_col=DA if s_in_t else 1, s_out_row=1 if s_out_t else DC,
+                  s_out_col=DA if s_out_t else 1)
+    d.a_t, d.a_b, d.a_h = a.stride()[:3]
+    d.b_t, d.b_b, d.b_h = b.stride()[:3]
+    d.c_t, d.c_b, d.c_h = c.stride()[:3]
+    d.o_t, d.o_b, d.o_h = out.stride()[:3]
+    with torch.cuda.device(a.device):
+        n = lib().ss_seq_leaky_ws_floats(C.byref(d))
+        ws = torch.empty(n, dtype=torch.float32, device=a.device) if n else None
+        d.ws = _p(ws)
+        _check(lib().ss_seq_leaky(C.byref(d), _stream(a)), 'ss_seq_leaky')
+
+
+def group_sum(x, out, group):
+    """x fp32 [rows * group, D] contiguous -> out [rows, D]: sums of `group` consecutive rows."""
+    D = x.shape[-1]
+    with torch.cuda.device(x.device):
+        _check(lib().ss_seq_group_sum(x.data_ptr(), out.data_ptr(), out.numel() // D, group, D, DT_CODE[out.dtype], _stream(x)), 'ss_seq_group_sum')
+
+
+def rms_norm_fwd(x, residual, weight, y, total, rstd, eps):
+    """x, residual: [rows, C] with a contiguous last axis; y, total contiguous; rstd fp32 [rows] or None."""
+    with torch.cuda.device(x.device):
+        _check(lib().ss_seq_rms_norm_fwd(x.data_ptr(), x.stride(0), _p(residual), 0 if residual is None else residual.stride(0), weight.data_ptr(), y.data_ptr(),
+                                         _p(total), _p(rstd), x.shape[0], x.shape[1], eps, DT_CODE[x.dtype], _stream(x)), 'ss_seq_rms_norm_fwd')
+
+
+def rms_norm_bwd(g_y, g_sum, h, weight, rstd, g_h, g_w):
+    rows, C_ = h.shape
+    with torch.cuda.device(h.device):
+        ws = None if g_w is None else torch.empty(lib().ss_seq_rms_norm_ws_floats(rows, C_, DT_CODE[h.dtype]), dtype=torch.float32, device=h.device)
+        _check(lib().ss_seq_rms_norm_bwd(_p(g_y), _p(g_sum), h.data_ptr(), weight.data_ptr(), rstd.data_ptr(), g_h.data_ptr(), _p(g_w), _p(ws), rows, C_,
+                                         DT_CODE[h.dtype], _stream(h)), 'ss_seq_rms_norm_bwd')
+
+
+def rms_norm_int8(x, residual, weight, codes, scales, total, eps):
+    with torch.cuda.device(x.device):
+        _check(lib().ss_seq_rms_norm_int8(x.data_ptr(), x.stride(0), _p(residual), 0 if residual is None else residual.stride(0), weight.data_ptr(),
+                                          codes.data_ptr(), scales.data_ptr(), _p(total), x.shape[0], x.shape[1], eps, DT_CODE[x.dtype], _stream(x)),
+               'ss_seq_rms_norm_int8')
+
+
+def dequant_int8(codes, scales, out):
+    with torch.cuda.device(codes.device):
+        _check(lib().ss_seq_dequant_int8(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), codes.shape[0], codes.shape[1], DT_CODE[out.dtype], _stream(codes)),
+               'ss_seq_dequant_int8')
+
+
+def int8_linear(a, a_scale, w, w_scale, bias, out):
+    """a [M, K], w [N, K] int8 with contiguous last axes; out [M, N] contiguous."""
+    (M, K), N = a.shape, w.shape[0]
+    with torch.cuda.device(a.device):
+        n = lib().ss_seq_int8_linear_ws_ints(M, N, K)
+        ws = torch.empty(n, dtype=torch.int32, device=a.device) if n else None
+        _check(lib().ss_seq_int8_linear(a.data_ptr(), a.stride(0), a_scale.data_ptr(), w.data_ptr(), w.stride(0), w_scale.data_ptr(), _p(bias), out.data_ptr(),
+                                        M, N, K, DT_CODE[out.dtype], _p(ws), _stream(a)), 'ss_seq_int8_linear')

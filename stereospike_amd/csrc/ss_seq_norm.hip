@@ -1,0 +1,404 @@
+// ss_seq_norm.hip — add + root-mean-square norm: forward, gradients, and the 8-bit form.
+//
+//   h = round(x + residual);  n = h * rstd,  rstd = (mean h^2 + eps)^(-1/2);  y = n * weight
+//
+// One pass: a row's h stays in registers between the sum of squares and the output, so every element is read once and written once (HBM-bound: 4 accesses
+// per element with a residual).  TPR threads share a row: a wavefront (no barrier) up to 4 accesses of 16 bytes per lane, then 256 or 1024 threads.  Blocks
+// walk rows with a grid stride so that the weight is read once per block.
+#include "ss_seq_common.hpp"
+
+namespace {
+
+constexpr int kMaxC = 16384;
+constexpr int kBwdBlocks = 1024;        // partials of the weight's gradient: 4 blocks of 4 wavefronts for each of 256 CUs
+
+struct NormArgs {
+    const void *x, *r;
+    long long xs, rs;
+    const float* w;
+    void *y, *sum;
+    float* rstd;
+    signed char* codes;
+    float* scales;
+    long long rows;
+    int C;
+    float eps;
+};
+
+// sum / max over the TPR threads of a row; every thread gets it.  `red`: one slot per wavefront (unused for TPR = 64)
+template <int TPR, typename V, bool MAX> __device__ __forceinline__ V row_reduce(V v, V* red)
+{
+    if constexpr (MAX) v = wave_max(v); else v = wave_sum(v);
+    if constexpr (TPR > 64) {
+        constexpr int W = TPR / 64;
+        __syncthreads();                                   // the slots of the last reduction have been read
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int i = 1; i < W; ++i) v = MAX ? (V)fmax(v, red[i]) : v + red[i];
+    }
+    return v;
+}
+
+// mean of squares -> 1 / sqrt(mean + eps).  fp32 sums leave their range for |h| beyond 1e18 or below 1e-14: those rows are summed again in fp64.
+template <int TPR, int NE> __device__ __forceinline__ float rstd_of(const float (&h)[NE], int C, float eps, float* redf, double* redd, bool& broken)
+{
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) s = fmaf(h[i], h[i], s);
+    s = row_reduce<TPR, float, false>(s, redf);
+    broken = false;
+    if (s < 1e37f && s > 1e-25f) return rsqrtf(s / (float)C + eps);
+    double d = 0.;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) d += (double)h[i] * (double)h[i];
+    d = row_reduce<TPR, double, false>(d, redd);
+    broken = !(d <= 1.7976931348623157e308);              // a NaN or an infinity in the row
+    return (float)(1.0 / sqrt(d / (double)C + (double)eps));
+}
+
+template <int DT, int VEC, int TPR, int NV, bool INT8>
+__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_fwd_kernel(const NormArgs p)
+{
+    constexpr int BLOCK = TPR == 64 ? 256 : TPR, RPB = BLOCK / TPR, NE = NV * VEC;
+    __shared__ float redf[16];
+    __shared__ double redd[16];
+    typedef Pack<DT, VEC> P;
+    const int lane = threadIdx.x % TPR;
+    float w[NE];
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const int j = (v * TPR + lane) * VEC + e;
+            w[v * VEC + e] = j < p.C ? p.w[j] : 0.f;
+        }
+    for (long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR; row < p.rows; row += (long long)gridDim.x * RPB) {
+        const elem_t<DT>* x = static_cast<const elem_t<DT>*>(p.x) + row * p.xs;
+        const elem_t<DT>* r = p.r ? static_cast<const elem_t<DT>*>(p.r) + row * p.rs : nullptr;
+        float h[NE];
+        P px[NV], pr[NV];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {                     // all loads of the row first
+            const int j = (v * TPR + lane) * VEC;
+            if (j < p.C) {
+                px[v] = *reinterpret_cast<const P*>(x + j);
+                if (r) pr[v] = *reinterpret_cast<const P*>(r + j);
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int j = (v * TPR + lane) * VEC;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) h[v * VEC + e] = 0.f;
+            if (j < p.C) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    if (r) px[v].v[e] = narrow<DT>(widen<DT>(px[v].v[e]) + widen<DT>(pr[v].v[e]));     // the sum is kept, and normed, in the input's type
+                    h[v * VEC + e] = widen<DT>(px[v].v[e]);
+                }
+                if (r) *reinterpret_cast<P*>(static_cast<elem_t<DT>*>(p.sum) + row * p.C + j) = px[v];
+            }
+        }
+        bool broken;
+        const float rstd = rstd_of<TPR, NE>(h, p.C, p.eps, redf, redd, broken);
+        if constexpr (!INT8) {
+            if (p.rstd && lane == 0) p.rstd[row] = rstd;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const int j = (v * TPR + lane) * VEC;
+                if (j < p.C) {
+                    P o;
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) o.v[e] = narrow<DT>(h[v * VEC + e] * rstd * w[v * VEC + e]);
+                    *reinterpret_cast<P*>(static_cast<elem_t<DT>*>(p.y) + row * p.C + j) = o;
+                }
+            }
+        } else {
+            // codes = rint(127 u / top), u = h w: rstd cancels.  In fp32 the quotient is off by at most 127 * 4 * 2^-24 = 3e-5; values within 1e-4 of the
+            // border of two codes (2 in 10^4) are decided in fp64, where u is exact, so codes do not depend on how the sum of squares was rounded.
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < NE; ++i) top = fmaxf(top, fabsf(h[i] * w[i]));
+            top = row_reduce<TPR, float, true>(top, redf);
+            double top64 = 0.;                             // rounding keeps order: the largest u in fp64 is among those whose rounded value is the largest
+#pragma unroll
+            for (int i = 0; i < NE; ++i)
+                if (fabsf(h[i] * w[i]) == top) top64 = fmax(top64, fabs((double)h[i] * (double)w[i]));
+            top64 = row_reduce<TPR, double, true>(top64, redd);
+            broken = broken || !(top64 < 3.4e38);
+            const float c = 127.f / top;
+            const bool plain = top > 1e-30f && !broken;    // 127 / top in range
+            if (lane == 0) p.scales[row] = broken ? __uint_as_float(0x7FC00000u) : top64 == 0. ? 0.f : (float)(top64 * (double)rstd / 127.0);
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const int j = (v * TPR + lane) * VEC;
+                if (j < p.C) {
+                    struct alignas(VEC) { signed char v[VEC]; } o;
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const float hi = h[v * VEC + e], wi = w[v * VEC + e], t = hi * wi * c, q = rintf(t);
+                        int code = (int)q;
+                        if (!plain || fabsf(t - q) > 0.4999f)
+                            code = broken || top64 == 0. ? 0 : (int)rint((double)hi * (double)wi * 127.0 / top64);
+                        o.v[e] = (signed char)code;
+                    }
+                    *reinterpret_cast<decltype(o)*>(p.codes + row * p.C + j) = o;
+                }
+            }
+        }
+    }
+}
+
+struct NormBwdArgs {
+    const void *gy, *gs, *h;
+    const float *w, *rstd;
+    void* gh;
+    float* ws;                              // [gridDim.x][C] partials of the weight's gradient, or NULL
+    long long rows;
+    int C;
+};
+
+template <int DT, int VEC, int TPR, int NV>
+__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_bwd_kernel(const NormBwdArgs p)
+{
+    constexpr int BLOCK = TPR == 64 ? 256 : TPR, RPB = BLOCK / TPR, NE = NV * VEC;
+    __shared__ float redf[16];
+    __shared__ float part[TPR == 64 ? 3 * 64 * NE : 1];
+    typedef Pack<DT, VEC> P;
+    const int lane = threadIdx.x % TPR;
+    float w[NE], gw[NE];
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const int j = (v * TPR + lane) * VEC + e;
+            w[v * VEC + e] = j < p.C ? p.w[j] : 0.f;
+            gw[v * VEC + e] = 0.f;
+        }
+    for (long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR; row < p.rows; row += (long long)gridDim.x * RPB) {
+        P pg[NV], ph[NV], ps[NV];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int j = (v * TPR + lane) * VEC;
+            if (j < p.C) {
+                ph[v] = *reinterpret_cast<const P*>(static_cast<const elem_t<DT>*>(p.h) + row * p.C + j);
+                if (p.gy) pg[v] = *reinterpret_cast<const P*>(static_cast<const elem_t<DT>*>(p.gy) + row * p.C + j);
+                if (p.gs) ps[v] = *reinterpret_cast<const P*>(static_cast<const elem_t<DT>*>(p.gs) + row * p.C + j);
+            }
+        }
+        const float rstd = p.rstd[row];
+        float n[NE], g[NE], dot = 0.f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const bool in = (v * TPR + lane) * VEC < p.C;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const int i = v * VEC + e;
+                n[i] = in ? widen<DT>(ph[v].v[e]) * rstd : 0.f;
+                g[i] = in && p.gy ? widen<DT>(pg[v].v[e]) : 0.f;
+                gw[i] = fmaf(g[i], n[i], gw[i]);
+                g[i] *= w[i];
+                dot = fmaf(g[i], n[i], dot);
+            }
+        }
+        dot = row_reduce<TPR, float, false>(dot, redf) / (float)p.C;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int j = (v * TPR + lane) * VEC;
+            if (j < p.C) {
+                P o;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const int i = v * VEC + e;
+                    float d = rstd * (g[i] - n[i] * dot);
+                    if (p.gs) d += widen<DT>(ps[v].v[e]);
+                    o.v[e] = narrow<DT>(d);
+                }
+                *reinterpret_cast<P*>(static_cast<elem_t<DT>*>(p.gh) + row * p.C + j) = o;
+            }
+        }
+    }
+    if (!p.ws) return;
+    if constexpr (TPR == 64) {                             // the block's four rows share their columns: one partial per block
+        const int wv = threadIdx.x >> 6;
+        if (wv)
+#pragma unroll
+            for (int i = 0; i < NE; ++i) part[((wv - 1) * NE + i) * 64 + lane] = gw[i];
+        __syncthreads();
+        if (wv) return;
+#pragma unroll
+        for (int i = 0; i < NE; ++i) gw[i] += part[i * 64 + lane] + part[(NE + i) * 64 + lane] + part[(2 * NE + i) * 64 + lane];
+    }
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const int j = (v * TPR + lane) * VEC + e;
+            if (j < p.C) p.ws[(long long)blockIdx.x * p.C + j] = gw[v * VEC + e];
+        }
+}
+
+// g_w[j] = sum of the blocks' partials, in their order: 32 columns x 32 slices per block
+__global__ __launch_bounds__(1024) void rms_gw_kernel(const float* __restrict__ ws, float* __restrict__ gw, int P, int C)
+{
+    __shared__ float red[32][33];
+    const int cx = threadIdx.x & 31, sl = threadIdx.x >> 5, j = blockIdx.x * 32 + cx;
+    float s = 0.f;
+    if (j < C)
+        for (int i = sl; i < P; i += 32) s += ws[(long long)i * C + j];
+    red[sl][cx] = s;
+    __syncthreads();
+    if (sl == 0 && j < C) {
+        for (int i = 1; i < 32; ++i) s += red[i][cx];
+        gw[j] = s;
+    }
+}
+
+template <int DT, int VEC> __global__ __launch_bounds__(256) void dequant_kernel(const signed char* __restrict__ q, const float* __restrict__ sc,
+                                                                                 elem_t<DT>* __restrict__ out, long long rows, int C)
+{
+    const int cv = (C + VEC - 1) / VEC;                    // C % VEC == 0 where VEC > 1
+    for (long long row = (long long)blockIdx.y * 4 + (threadIdx.x >> 6); row < rows; row += (long long)gridDim.y * 4) {
+        const float s = sc[row];
+        for (int v = blockIdx.x * 64 + (threadIdx.x & 63); v < cv; v += gridDim.x * 64) {
+            struct alignas(VEC) Q { signed char v[VEC]; };
+            const Q a = *reinterpret_cast<const Q*>(q + row * C + (long long)v * VEC);
+            Pack<DT, VEC> o;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) o.v[e] = narrow<DT>((float)a.v[e] * s);
+            *reinterpret_cast<Pack<DT, VEC>*>(out + row * C + (long long)v * VEC) = o;
+        }
+    }
+}
+
+// Threads of a row and accesses per thread.  Many rows: a wavefront per row as long as its 4 accesses reach.  Few rows (under 1024, the card is not filled and
+// a call is one row's latency): the most threads that have something to do.
+template <typename F> int with_shape(int C, long long rows, int vec, F&& f)
+{
+    const int acc = (C + vec - 1) / vec;
+    const bool few = rows < 1024;
+    const int lim64 = few ? 128 : 256;
+    if (vec > 1) {
+        if (acc <= 64) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
+        if (acc <= lim64 && acc <= 128) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+        if (acc <= lim64) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
+        if (acc <= 512) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
+        if (acc <= 1024 && !few) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 4>());
+        if (acc <= 1024) return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 1>());
+        if (acc <= 2048) return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
+        return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
+    }
+    if (acc <= 64) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
+    if (acc <= 256) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
+    if (acc <= 1024 && !few) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 16>());
+    if (acc <= 1024) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 4>());
+    if (acc <= 4096) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 16>());
+    return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 16>());
+}
+
+template <int DT, bool INT8> int fwd_dt(const NormArgs& p, hipStream_t s)
+{
+    constexpr int V = DT == SS_SEQ_F32 ? 4 : 8;
+    const void* out = INT8 ? (const void*)p.codes : p.y;
+    const bool vec = p.C % V == 0 && p.xs % V == 0 && aligned(p.x, 16) && (!p.r || (p.rs % V == 0 && aligned(p.r, 16) && aligned(p.sum, 16))) && aligned(out, INT8 ? V : 16);
+    auto go = [&](auto VC) {
+        return with_shape(p.C, p.rows, VC.value, [&](auto TPR, auto NV) {
+            constexpr int block = TPR.value == 64 ? 256 : TPR.value, rpb = block / TPR.value;
+            const long long want = (p.rows + rpb - 1) / rpb, cap = 256 * (2048 / block);          // 32 wavefronts for each of 256 CUs
+            rms_fwd_kernel<DT, VC.value, TPR.value, NV.value, INT8><<<(unsigned)(want < cap ? want : cap), block, 0, s>>>(p);
+            return launched();
+        });
+    };
+    return vec ? go(std::integral_constant<int, V>()) : go(std::integral_constant<int, 1>());
+}
+
+template <int DT> int bwd_dt(const NormBwdArgs& p, float* gw, hipStream_t s)
+{
+    constexpr int V = DT == SS_SEQ_F32 ? 4 : 8;
+    const bool vec = p.C % V == 0 && aligned(p.gy, 16) && aligned(p.gs, 16) && aligned(p.h, 16) && aligned(p.gh, 16);
+    auto go = [&](auto VC) {
+        return with_shape(p.C, p.rows, VC.value, [&](auto TPR, auto NV) {
+            constexpr int block = TPR.value == 64 ? 256 : TPR.value, rpb = block / TPR.value;
+            const long long want = (p.rows + rpb - 1) / rpb;
+            const unsigned grid = (unsigned)(want < kBwdBlocks ? want : kBwdBlocks);
+            rms_bwd_kernel<DT, VC.value, TPR.value, NV.value><<<grid, block, 0, s>>>(p);
+            if (int rc = launched()) return rc;
+            if (gw) {
+                rms_gw_kernel<<<(p.C + 31) / 32, 1024, 0, s>>>(p.ws, gw, (int)grid, p.C);
+                return launched();
+            }
+            return SS_SEQ_OK;
+        });
+    };
+    return vec ? go(std::integral_constant<int, V>()) : go(std::integral_constant<int, 1>());
+}
+
+bool sizes_ok(long long rows, int C, int dtype) { return rows >= 0 && C > 0 && C <= kMaxC && (dtype == SS_SEQ_F32 || dtype == SS_SEQ_F16 || dtype == SS_SEQ_BF16); }
+
+}  // namespace
+
+extern "C" {
+
+int ss_seq_abi_version(void) { return SS_SEQ_ABI_VERSION; }
+
+int ss_seq_rms_norm_fwd(const void* x, long long x_stride, const void* residual, long long r_stride, const float* weight, void* y, void* sum, float* rstd,
+                        long long rows, int C, float eps, int dtype, void* stream)
+{
+    if (!sizes_ok(rows, C, dtype) || !(eps >= 0.f)) return SS_SEQ_EINVAL;
+    if (rows == 0) return SS_SEQ_OK;
+    if (!x || !weight || !y || (residual && !sum)) return SS_SEQ_EINVAL;
+    const NormArgs p{x, residual, x_stride, r_stride, weight, y, sum, rstd, nullptr, nullptr, rows, C, eps};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return dtype == SS_SEQ_F32 ? fwd_dt<SS_SEQ_F32, false>(p, s) : dtype == SS_SEQ_F16 ? fwd_dt<SS_SEQ_F16, false>(p, s) : fwd_dt<SS_SEQ_BF16, false>(p, s);
+}
+
+int ss_seq_rms_norm_int8(const void* x, long long x_stride, const void* residual, long long r_stride, const float* weight, signed char* codes, float* scales,
+                         void* sum, long long rows, int C, float eps, int dtype, void* stream)
+{
+    if (!sizes_ok(rows, C, dtype) || !(eps >= 0.f)) return SS_SEQ_EINVAL;
+    if (rows == 0) return SS_SEQ_OK;
+    if (!x || !weight || !codes || !scales || (residual && !sum)) return SS_SEQ_EINVAL;
+    const NormArgs p{x, residual, x_stride, r_stride, weight, nullptr, sum, nullptr, codes, scales, rows, C, eps};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return dtype == SS_SEQ_F32 ? fwd_dt<SS_SEQ_F32, true>(p, s) : dtype == SS_SEQ_F16 ? fwd_dt<SS_SEQ_F16, true>(p, s) : fwd_dt<SS_SEQ_BF16, true>(p, s);
+}
+
+long long ss_seq_rms_norm_ws_floats(long long rows, int C, int dtype)
+{
+    if (!sizes_ok(rows, C, dtype)) return 0;
+    return (rows < kBwdBlocks ? rows : kBwdBlocks) * (long long)C;
+}
+
+int ss_seq_rms_norm_bwd(const void* g_y, const void* g_sum, const void* h, const float* weight, const float* rstd, void* g_h, float* g_w, float* ws,
+                        long long rows, int C, int dtype, void* stream)
+{
+    if (!sizes_ok(rows, C, dtype) || rows == 0 || !h || !weight || !rstd || !g_h || (g_w && !ws)) return SS_SEQ_EINVAL;
+    const NormBwdArgs p{g_y, g_sum, h, weight, rstd, g_h, g_w ? ws : nullptr, rows, C};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return dtype == SS_SEQ_F32 ? bwd_dt<SS_SEQ_F32>(p, g_w, s) : dtype == SS_SEQ_F16 ? bwd_dt<SS_SEQ_F16>(p, g_w, s) : bwd_dt<SS_SEQ_BF16>(p, g_w, s);
+}
+
+int ss_seq_dequant_int8(const signed char* codes, const float* scales, void* out, long long rows, int C, int dtype, void* stream)
+{
+    if (rows < 0 || C <= 0 || (dtype != SS_SEQ_F32 && dtype != SS_SEQ_F16 && dtype != SS_SEQ_BF16)) return SS_SEQ_EINVAL;
+    if (rows == 0) return SS_SEQ_OK;
+    if (!codes || !scales || !out) return SS_SEQ_EINVAL;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const bool vec = C % 8 == 0 && aligned(codes, 8) && aligned(out, 32);
+    const int cv = vec ? C / 8 : C;
+    const int gx = (cv + 255) / 256;                       // four accesses per lane
+    const dim3 grid((unsigned)gx, (unsigned)(rows < 65536ll * 4 ? (rows + 3) / 4 : 65535));
+    auto go = [&](auto DTC) {
+        constexpr int DT = DTC.value;
+        elem_t<DT>* o = static_cast<elem_t<DT>*>(out);
+        if (vec) dequant_kernel<DT, 8><<<grid, 256, 0, s>>>(codes, scales, o, rows, C);
+        else dequant_kernel<DT, 1><<<grid, 256, 0, s>>>(codes, scales, o, rows, C);
+        return launched();
+    };
+    return dtype == SS_SEQ_F32 ? go(std::integral_constant<int, SS_SEQ_F32>()) : dtype == SS_SEQ_F16 ? go(std::integral_constant<int, SS_SEQ_F16>())
+                                                                                                     : go(std::integral_constant<int, SS_SEQ_BF16>());
+}
+
+}  // extern "C"

@@ -1,0 +1,562 @@
+"""MI355X suite of the sequence operators against plain 64-bit implementations.
+
+Tolerances count roundings.  u = 2^-24 is half a step of fp32, HALF[dtype] half a step of the output's type.  A computed sum of products may be off by
+(roundings a term passes through) * u * (the sum of the terms' magnitudes), so every comparison has the same sum with absolute values beside it."""
+import math
+
+import pytest
+import torch
+
+from stereospike_amd import sequence
+from stereospike_amd.clock_driven import functional, layer
+
+pytestmark = pytest.mark.gpu
+U = 2. ** -24
+HALF = {torch.float32: 2. ** -24, torch.bfloat16: 2. ** -8, torch.float16: 2. ** -11}
+# below its smallest normal number 2^-14 fp16 has steps of 2^-24: half of one, whatever the value (the other types' steps there are under 1e-38)
+TINY = {torch.float32: 1e-30, torch.bfloat16: 1e-30, torch.float16: 2. ** -25 * 1.01}
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+DEV = 'cuda'
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def normal(g, *shape, dtype=torch.float32, std=1.):
+    return (torch.randn(shape, generator=g) * std).to(dtype)
+
+
+def within(got, want, room, what):
+    got, want, room = got.detach().cpu().double(), want.detach().cpu().double(), room.detach().cpu().double()
+    assert got.shape == want.shape, what
+    assert torch.isfinite(got).all(), f'{what}: not finite'
+    off = (got - want).abs() - room
+    assert (off <= 0).all(), f'{what}: {(off > 0).sum().item()} of {off.numel()} out of tolerance, worst by {off.max().item():.3g} (values up to {want.abs().max().item():.3g})'
+
+
+# ----------------------------------------------------------------------------------------------------------------------------------------------------------
+# leaky attention
+# ----------------------------------------------------------------------------------------------------------------------------------------------------------
+def leaky_ref(q, k, v, log_decay, scale, state=None, lengths=None):
+    """The recurrence in fp64 on the CPU, differentiable: the definition."""
+    T, B, H, Dk = q.shape
+    r = H // k.shape[2]
+    q, k, v = q.double().cpu(), k.double().cpu().repeat_interleave(r, 2), v.double().cpu().repeat_interleave(r, 2)
+    lam = log_decay.double().cpu().exp()[:, None, None]
+    S = torch.zeros(B, H, Dk, v.shape[3], dtype=torch.float64) if state is None else state.double().cpu()
+    out = []
+    for t in range(T):
+        new = lam * S + k[t, :, :, :, None] * v[t, :, :, None, :]
+        o = scale * torch.einsum('bhi,bhij->bhj', q[t], new)
+        if lengths is not None:
+            live = (t < lengths.cpu())[:, None, None]
+            new, o = torch.where(live[..., None], new, S), torch.where(live, o, torch.zeros_like(o))
+        S = new
+        out.append(o)
+    return torch.stack(out), S
+
+
+def leaky_case(T, B, H, Hk, Dk, Dv, dtype, state, ragged, seed=0):
+    g = gen(seed)
+    q, k, v = normal(g, T, B, H, Dk, dtype=dtype), normal(g, T, B, Hk, Dk, dtype=dtype), normal(g, T, B, Hk, Dv, dtype=dtype)
+    decay = torch.tensor([0., -1e-3, -0.05, -0.7, -20., -math.inf])[torch.arange(H) * 5 % 6]
+    s = normal(g, B, H, Dk, Dv) if state else None
+    n = torch.tensor([T, 0, 1, T - 1, T // 2 + 1, T + 5, -1])[torch.arange(B) % 7].to(torch.int32) if ragged else None
+    return q, k, v, decay, s, n
+
+
+def leaky_check(T, B, H, Hk, Dk, Dv, dtype, state, ragged, grads, seed=0):
+    q, k, v, decay, s, n = leaky_case(T, B, H, Hk, Dk, Dv, dtype, state, ragged, seed)
+    scale = Dk ** -0.5
+    leaf = [t.clone().to(DEV).requires_grad_(grads) if t is not None else None for t in (q, k, v, s)]
+    poison = [t.detach().clone() if t is not None else None for t in leaf[:3]]
+    if ragged:                                             # what lies behind the last valid step is not looked at
+        for t in poison:
+            t[torch.arange(T, device=DEV)[:, None] >= n.to(DEV).clamp(0, T)[None, :]] = math.nan
+    use = [t.requires_grad_(grads) for t in poison] + [leaf[3]]
+    o, last = sequence.leaky_attention(use[0], use[1], use[2], decay.to(DEV), state=use[3], lengths=None if n is None else n.to(DEV), return_state=True)
+    # every term passes through at most 2 roundings per step it leaks, the products, and the sum over Dk and the steps of a tile
+    steps = 2 * T + Dk + Dv + 80
+    sharp = HALF[dtype] if dtype != torch.float32 else U   # one rounding of the token-by-token weights, or of the state, to the operands' type
+    ref = [t.double().requires_grad_(grads) if t is not None else None for t in (q, k, v, s)]
+    want, want_last = leaky_ref(*ref[:3], decay, scale, ref[3], n)
+    mag = [t.detach().abs().double().requires_grad_(grads) if t is not None else None for t in (q, k, v, s)]
+    size, size_last = leaky_ref(*mag[:3], decay, scale, mag[3], n)
+    within(o, want, size * (steps * U + sharp) + want.abs() * HALF[dtype] * 1.02 + TINY[dtype], 'o')
+    within(last, want_last, size_last * (steps * U) + 1e-30, 'state')
+    assert o.dtype == dtype and last.dtype == torch.float32
+    if not grads:
+        return
+    g = gen(seed + 1)
+    go, gl = normal(g, *o.shape, dtype=dtype), normal(g, *last.shape)
+    used = go.to(DEV)
+    if ragged:
+        used = used.clone()
+        used[torch.arange(T, device=DEV)[:, None] >= n.to(DEV).clamp(0, T)[None, :]] = math.nan
+    wrt = [i for i in range(4) if use[i] is not None]
+    got = torch.autograd.grad([o, last], [use[i] for i in wrt], [used, gl.to(DEV)])
+    exp = torch.autograd.grad([want, want_last], [ref[i] for i in wrt], [go.double(), gl.double()])
+    mags = torch.autograd.grad([size, size_last], [mag[i] for i in wrt], [go.double().abs(), gl.double().abs()])
+    for i, a, b, m in zip(wrt, got, exp, mags):
+        name = 'qkvs'[i]
+        low = name != 's'
+        within(a, b, m * (steps * U + (sharp if low else 0)) + (b.abs() * HALF[dtype] * 1.02 if low else 0) + TINY[dtype], 'gradient of ' + name)
+        assert a.dtype == use[i].dtype
+
+
+SHAPES = [(1, 1, 1, 1, 1, 1), (2, 1, 2, 1, 16, 16), (5, 3, 2, 2, 7, 9), (16, 2, 2, 2, 64, 64), (63, 2, 2, 2, 8, 24), (64, 1, 1, 1, 128, 128), (65, 7, 3, 1, 33, 17),
+          (130, 2, 4, 2, 64, 64), (257, 1, 2, 2, 128, 128), (200, 2, 2, 1, 20, 256), (129, 1, 1, 1, 256, 80), (1100, 1, 2, 2, 48, 72)]
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('shape', SHAPES)
+def test_leaky_attention(shape, dtype):
+    leaky_check(*shape, dtype, state=False, ragged=False, grads=True)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('shape', [(3, 7, 2, 1, 8, 8), (70, 7, 2, 2, 24, 40), (200, 7, 4, 2, 64, 128)])
+def test_leaky_attention_state_and_lengths(shape, dtype):
+    leaky_check(*shape, dtype, state=True, ragged=True, grads=True)
+    leaky_check(*shape, dtype, state=True, ragged=False, grads=True, seed=3)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_leaky_attention_long(dtype):
+    leaky_check(5000, 1, 2, 2, 16, 24, dtype, state=True, ragged=False, grads=False)
+
+
+def test_leaky_gradient_against_differences():
+    """The map is linear in each operand: a central difference of the definition along a direction is its derivative, up to the definition's fp64."""
+    q, k, v, decay, s, n = leaky_case(70, 3, 2, 1, 12, 10, torch.float32, True, True, seed=5)
+    use = [t.to(DEV).requires_grad_() for t in (q, k, v, s)]
+    o, last = sequence.leaky_attention(*use[:3], decay.to(DEV), state=use[3], lengths=n.to(DEV), return_state=True)
+    g = gen(9)
+    wo, wl = normal(g, *o.shape), normal(g, *last.shape)
+    got = torch.autograd.grad([o, last], use, [wo.to(DEV), wl.to(DEV)])
+    base = [t.double() for t in (q, k, v, s)]
+
+    def loss(x):
+        a, b = leaky_ref(*x[:3], decay, 12 ** -0.5, x[3], n)
+        return (a * wo).sum() + (b * wl).sum()
+
+    for i, grad in enumerate(got):
+        d = normal(g, *base[i].shape).double()
+        up, down = [list(base) for _ in range(2)]
+        up[i], down[i] = base[i] + 0.5 * d, base[i] - 0.5 * d
+        slope, along = loss(up) - loss(down), (grad.cpu().double() * d)
+        # fp32 roundings of the gradient (300 of them at most), against the size of the terms
+        assert abs(along.sum() - slope) <= 300 * U * 40 * along.abs().sum(), 'qkvs'[i]
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_leaky_attention_strides(dtype):
+    """Batch-major tensors, slices of one projection, rows off any alignment, expanded heads: what the contiguous copies give, within the
+    roundings of the two kernel forms."""
+    g, decay = gen(2), torch.tensor([-0.1, -0.01]).to(DEV)
+    T, B, H, D = 75, 2, 2, 32
+    x = normal(g, B, T, 3, H, D + 1, dtype=dtype).to(DEV)
+    q, k, v = (x[:, :, i, :, 1:].transpose(0, 1) for i in range(3))
+    want = sequence.leaky_attention(q.contiguous(), k.contiguous(), v.contiguous(), decay, return_state=True)
+    got = sequence.leaky_attention(q, k, v, decay, return_state=True)
+    size = leaky_ref(q.abs(), k.abs(), v.abs(), decay, D ** -0.5)
+    for a, b, m in zip(got, want, size):
+        within(a, b, m * (600 * U + 2 * HALF[dtype]) + 2 * TINY[dtype], 'strided')
+    one = k[:, :, :1].expand(T, B, H, D)
+    a, b = sequence.leaky_attention(q, one, v, decay), sequence.leaky_attention(q, one.contiguous(), v, decay)
+    within(a, b, leaky_ref(q.abs(), one.abs(), v.abs(), decay, D ** -0.5)[0] * (600 * U + 2 * HALF[dtype]) + 2 * TINY[dtype], 'expanded')
+    vt = normal(g, T, B, D, H, dtype=dtype).to(DEV).transpose(2, 3)              # a last axis that is not contiguous
+    assert torch.equal(sequence.leaky_attention(q, k, vt, decay), sequence.leaky_attention(q, k, vt.contiguous(), decay))
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('shape', [(1, 1, 1, 1, 1), (3, 4, 2, 64, 64), (2, 6, 3, 33, 17), (5, 2, 2, 128, 128), (2, 1, 1, 256, 200), (300, 2, 1, 16, 32)])
+def test_step(shape, dtype):
+    """Several single steps: the state is updated in place, each against the definition from the state that was there."""
+    B, H, Hk, Dk, Dv = shape
+    q, k, v, decay, s, _ = leaky_case(3, B, H, Hk, Dk, Dv, dtype, True, False, seed=7)
+    state = s.to(DEV)
+    for t in range(3):
+        before = state.clone()
+        o = sequence.leaky_attention_step(q[t].to(DEV), k[t].to(DEV), v[t].to(DEV), decay.to(DEV), state)
+        want, last = leaky_ref(q[t:t + 1], k[t:t + 1], v[t:t + 1], decay, Dk ** -0.5, before)
+        size, size_last = leaky_ref(q[t:t + 1].abs(), k[t:t + 1].abs(), v[t:t + 1].abs(), decay, Dk ** -0.5, before.abs())
+        within(o, want[0], size[0] * (Dk + 8) * U + want[0].abs() * HALF[dtype] * 1.02 + TINY[dtype], 'o')
+        within(state, last, size_last * 8 * U + 1e-30, 'state')
+
+
+def test_step_continues_a_sequence():
+    q, k, v, decay, s, _ = (t.to(DEV) if t is not None else None for t in leaky_case(90, 2, 3, 1, 40, 24, torch.float32, True, False, seed=8))
+    want, want_last = sequence.leaky_attention(q, k, v, decay, state=s, return_state=True)
+    _, state = sequence.leaky_attention(q[:87], k[:87], v[:87], decay, state=s, return_state=True)
+    for t in range(87, 90):
+        o = sequence.leaky_attention_step(q[t], k[t], v[t], decay, state)
+    size, size_last = leaky_ref(q.abs(), k.abs(), v.abs(), decay, 40 ** -0.5, s.abs())
+    within(o, want[-1], size[-1] * 2 * 400 * U, 'o')
+    within(state, want_last, size_last * 2 * 400 * U, 'state')
+
+
+def test_step_notices_autograd():
+    q, k, v, decay, s, _ = (t.to(DEV) if t is not None else None for t in leaky_case(1, 1, 1, 1, 8, 8, torch.float32, True, False))
+    q.requires_grad_()
+    o = sequence.leaky_attention(q, k, v, decay, state=s)
+    sequence.leaky_attention_step(q.detach()[0], k[0], v[0], decay, s)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        o.sum().backward()
+
+
+# ----------------------------------------------------------------------------------------------------------------------------------------------------------
+# add + root-mean-square norm
+# ----------------------------------------------------------------------------------------------------------------------------------------------------------
+WIDTHS = [1, 7, 8, 63, 64, 100, 512, 513, 1000, 1024, 2048, 4096, 5000, 8192, 16383, 16384]
+# a sum of squares: at most 64 values in a row and 26 levels of threads; half of that in its root, and a few roundings after it
+NORM_ROOM = 55 * U
+
+
+def norm_case(rows, C, dtype, residual, seed=0):
+    g = gen(seed)
+    x, w = normal(g, rows, C, dtype=dtype), 1 + normal(g, C, std=0.2)
+    return x, w, normal(g, rows, C, dtype=dtype, std=2.) if residual else None
+
+
+def norm_ref(x, w, r, eps):
+    h = x if r is None else (x.float() + r.float()).to(x.dtype)
+    d = h.double()
+    return h, d, (d.square().mean(-1, keepdim=True) + eps).rsqrt()
+
+
+@pytest.mark.parametrize('residual', [True, False])
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('C', WIDTHS)
+def test_norm_and_gradients(C, dtype, residual):
+    for rows in (1, 5, 1030 if C <= 2048 else 6):
+        x, w, r = norm_case(rows, C, dtype, residual, seed=C)
+        use = [t.to(DEV).requires_grad_() if t is not None else None for t in (x, r, w)]
+        y, h = sequence.add_rms_norm(use[0], use[2], use[1], eps=1e-5)
+        hr, d, rstd = norm_ref(x, w, r, 1e-5)
+        assert torch.equal(h.detach().cpu(), hr) and y.dtype == dtype
+        n = d * rstd
+        within(y, n * w.double(), (n * w.double()).abs() * (NORM_ROOM + HALF[dtype] * 1.01) + TINY[dtype], f'y {rows}')
+        g = gen(rows)
+        gy, gh = normal(g, rows, C, dtype=dtype), normal(g, rows, C, dtype=dtype)
+        outs, gs = ([y, h], [gy.to(DEV), gh.to(DEV)]) if residual else ([y], [gy.to(DEV)])
+        got = torch.autograd.grad(outs, [t for t in use if t is not None], gs)
+        gw = gy.double() * w.double()
+        dot, dot_size = (gw * n).mean(-1, keepdim=True), (gw * n).abs().mean(-1, keepdim=True)
+        want = rstd * (gw - n * dot) + (gh.double() if residual else 0)
+        size = rstd * (gw.abs() + n.abs() * dot_size) + (gh.double().abs() if residual else 0)
+        for a in got[:-1]:
+            within(a, want, size * 3 * NORM_ROOM + want.abs() * HALF[dtype] * 1.01 + TINY[dtype], f'gradient of h {rows}')
+        # rows of a block one after the other, the blocks in 32 slices
+        within(got[-1], (gy.double() * n).sum(0), (gy.double() * n).abs().sum(0) * (rows + 70 + 60) * U + 1e-30, f'gradient of the weight {rows}')
+
+
+def test_norm_gradient_against_differences():
+    x, w, r = (t.double() for t in norm_case(4, 40, torch.float32, True, seed=1))
+    use = [t.float().to(DEV).requires_grad_() for t in (x, r, w)]
+    y, h = sequence.add_rms_norm(use[0], use[2], use[1])
+    g = gen(4)
+    wy, wh = normal(g, 4, 40).double(), normal(g, 4, 40).double()
+    got = torch.autograd.grad([y, h], use, [wy.float().to(DEV), wh.float().to(DEV)])
+
+    def loss(x, r, w):
+        d = x + r
+        return ((d * (d.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * w) * wy).sum() + (d * wh).sum()
+
+    base, step = [x, r, w], 1e-5
+    for i, grad in enumerate(got):
+        d = normal(g, *base[i].shape).double()
+        up, down = list(base), list(base)
+        up[i], down[i] = base[i] + step * d, base[i] - step * d
+        along = grad.cpu().double() * d
+        # fp32 roundings, the rounding of x + r (2^-24 of it), and the difference's own error: step^2 times a third derivative of order one per value
+        assert abs(along.sum() - (loss(*up) - loss(*down)) / (2 * step)) <= (4 * NORM_ROOM + 1e-9) * 10 * along.abs().sum()
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_norm_strided_rows_and_alignment(dtype):
+    g = gen(3)
+    big, w = normal(g, 9, 3, 130, dtype=dtype).to(DEV), (1 + normal(g, 128, std=0.1)).to(DEV)
+    for cut in (slice(0, 128), slice(1, 129), slice(2, 130)):
+        x, r = big[:, 0, cut], big[:, 2, cut]
+        a, b = sequence.add_rms_norm(x, w, r), sequence.add_rms_norm(x.contiguous(), w, r.contiguous())
+        assert torch.equal(a[1], b[1])
+        within(a[0], b[0], b[0].double().abs() * (2 * NORM_ROOM + 2.02 * HALF[dtype]) + 2 * TINY[dtype], 'strided')
+        c, d = sequence.add_rms_norm_int8(x, w, r), sequence.add_rms_norm_int8(x.contiguous(), w, r.contiguous())
+        assert torch.equal(c[0], d[0]) and torch.equal(c[2], d[2])
+    assert sequence.add_rms_norm(big[:, :, :128].reshape(3, 9, 128), w)[0].shape == (3, 9, 128)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_norm_range(dtype):
+    """Values whose squares leave fp32's range on either side."""
+    g = gen(6)
+    for size in (1e25, 1e-25):
+        x = (normal(g, 3, 200) * size).to(dtype)
+        w = 1 + normal(g, 200, std=0.1)
+        y, _ = sequence.add_rms_norm(x.to(DEV), w.to(DEV), eps=0.)
+        _, d, rstd = norm_ref(x, w, None, 0.)
+        want = d * rstd * w.double()
+        within(y, want, want.abs() * (NORM_ROOM + HALF[dtype] * 1.01), f'y at {size}')
+        codes, scales, _ = sequence.add_rms_norm_int8(x.to(DEV), w.to(DEV), eps=0.)
+        u = d * w.double()
+        assert torch.equal(codes.cpu().double(), torch.round(u * 127. / u.abs().amax(-1, keepdim=True)))
+    zero = torch.zeros(2, 64, dtype=dtype, device=DEV)
+    assert not sequence.add_rms_norm(zero, torch.ones(64, device=DEV))[0].any()
+
+
+@pytest.mark.parametrize('residual', [True, False])
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('C', WIDTHS)
+def test_norm_int8(C, dtype, residual):
+    for rows in (1, 5, 1030 if C <= 2048 else 6):
+        x, w, r = norm_case(rows, C, dtype, residual, seed=C + 1)
+        codes, scales, h = sequence.add_rms_norm_int8(x.to(DEV), w.to(DEV), None if r is None else r.to(DEV))
+        hr, d, rstd = norm_ref(x, w, r, 1e-6)
+        assert torch.equal(h.cpu(), hr)
+        u = d * w.double()
+        top = u.abs().amax(-1, keepdim=True)
+        assert codes.dtype == torch.int8 and torch.equal(codes.cpu().double(), torch.round(u * 127. / top.clamp_min(1e-300)))         # (a row of zeros has codes 0)
+        want = (top * rstd / 127.)[:, 0]
+        within(scales, want, want * NORM_ROOM, 'scales')
+        back = sequence.dequantize_int8(codes, scales, dtype)
+        values = codes.cpu().double() * scales.cpu().double()[:, None]
+        within(back, values, values.abs() * (HALF[dtype] + U) * 1.01 + TINY[dtype], 'values')
+
+
+def test_norm_int8_ties_zeros_and_what_is_not_finite():
+    x = torch.zeros(6, 64)
+    x[0, 0], x[0, 1:8] = 127., torch.tensor([0.5, 1.5, 2.5, -0.5, -1.5, -2.5, 126.5])         # a code's step is 1: ties, to even
+    x[1] = x[0] * 2. ** 40
+    x[2, 0], x[2, 1:8] = -127., x[0, 1:8]
+    x[4, 3], x[5, 3] = math.nan, -math.inf
+    x[4, 5] = x[5, 5] = 1.
+    for dtype in DTYPES:
+        if dtype == torch.float16:
+            x[1] = x[0] * 2. ** 8
+        codes, scales, _ = sequence.add_rms_norm_int8(x.to(dtype).to(DEV), torch.ones(64, device=DEV))
+        xd = x.to(dtype).double()
+        want = torch.round(xd[:3] * 127 / xd[:3].abs().amax(-1, keepdim=True))
+        assert torch.equal(codes[:3].cpu().double(), want)
+        assert not codes[3:].any() and scales[3] == 0 and scales[4:].isnan().all() and scales[:3].isfinite().all()
+
+
+# ----------------------------------------------------------------------------------------------------------------------------------------------------------
+# 8-bit integer product
+# ----------------------------------------------------------------------------------------------------------------------------------------------------------
+def product_case(M, N, K, bias, seed=0, full=False):
+    g = gen(seed)
+    lo, hi = (-128, 128)
+    a, w = (torch.randint(lo, hi, s, generator=g, dtype=torch.int32).to(torch.int8) for s in ((M, K), (N, K)))
+    return a, torch.rand(M, generator=g) + 0.01, w, torch.rand(N, generator=g) + 0.01, normal(g, N, std=1000.) if bias else None
+
+
+def product_check(M, N, K, bias, out, seed=0):
+    a, sa, w, sw, b = product_case(M, N, K, bias, seed)
+    got = sequence.int8_linear(a.to(DEV), sa.to(DEV), w.to(DEV), sw.to(DEV), None if b is None else b.to(DEV), out)
+    acc = a.double() @ w.double().t()
+    y = acc * sa.double()[:, None] * sw.double()
+    want = y if b is None else y + b.double()
+    # what rounds beyond fp16's largest number, 65504 (from 65520 on), is an infinity there
+    over = want.abs() > 65520 * (1 + 8 * U) if out == torch.float16 else torch.zeros_like(want, dtype=torch.bool)
+    assert torch.equal(got.cpu().double()[over], want[over].sign() * math.inf)
+    got, y, want = got.cpu().masked_fill(over, 0), y.masked_fill(over, 0), want.masked_fill(over, 0)
+    # the integer to fp32, two scales, the bias; then the output's rounding
+    within(got, want, y.abs() * 3.1 * U + want.abs() * (HALF[out] * 1.01 + U) + TINY[out], f'{M} x {N} x {K}')
+    assert got.dtype == out
+
+
+@pytest.mark.parametrize('K', [1, 15, 16, 17, 48, 64, 100, 128, 144, 1000, 4096])
+@pytest.mark.parametrize('M', [1, 2, 5, 16, 17, 33, 64, 65, 130, 300])
+def test_int8_linear(M, K):
+    for N in (1, 8, 17, 64, 100, 257):
+        product_check(M, N, K, bias=(M + N) % 2 == 0, out=DTYPES[(M + N + K) % 3], seed=M + N + K)
+
+
+@pytest.mark.parametrize('shape', [(1, 8192, 512), (4, 2048, 4608), (700, 512, 4608), (513, 1025, 2064), (2100, 600, 320), (1100, 1300, 77), (66000, 8, 32)])
+def test_int8_linear_larger(shape):
+    a, sa, w, sw, b = product_case(*shape, True, seed=1)
+    got = sequence.int8_linear(a.to(DEV), sa.to(DEV), w.to(DEV), sw.to(DEV), b.to(DEV))
+    y = (a.to(DEV).double() @ w.to(DEV).double().t()) * sa.to(DEV).double()[:, None] * sw.to(DEV).double()
+    want = y + b.to(DEV).double()
+    within(got, want, y.abs() * 3.1 * U + want.abs() * 2 * U + 1e-30, str(shape))
+
+
+def test_int8_linear_extreme_sums_and_strides():
+    K = 131071
+    a, w = torch.full((3, K), -128, dtype=torch.int8, device=DEV), torch.full((2, K), -128, dtype=torch.int8, device=DEV)
+    w[1] = 127
+    got = sequence.int8_linear(a, torch.ones(3, device=DEV), w, torch.ones(2, device=DEV))
+    want = torch.tensor([128. * 128 * K, -128. * 127 * K], dtype=torch.float64)
+    within(got, want.expand(3, 2), want.abs().expand(3, 2) * 4 * U, 'extreme')
+    g = gen(5)
+    x = torch.randint(-128, 128, (40, 2, 300), generator=g, dtype=torch.int32).to(torch.int8).to(DEV)
+    w = torch.randint(-128, 128, (33, 300), generator=g, dtype=torch.int32).to(torch.int8).to(DEV)
+    s, sw = torch.rand(40, generator=g).to(DEV), torch.rand(33, generator=g).to(DEV)
+    for cut in (slice(0, 256), slice(1, 257), slice(3, 290)):
+        assert torch.equal(sequence.int8_linear(x[:, 1, cut], s, w[:, cut], sw), sequence.int8_linear(x[:, 1, cut].contiguous(), s, w[:, cut].contiguous(), sw))
+    out = sequence.int8_linear(x[:, :, :256], torch.stack((s, s), 1), w[:, :256], sw)                     # leading axes are kept
+    assert out.shape == (40, 2, 33) and torch.equal(out[:, 1], sequence.int8_linear(x[:, 1, :256], s, w[:, :256], sw))
+
+
+# ----------------------------------------------------------------------------------------------------------------------------------------------------------
+# together, streams, graphs
+# ----------------------------------------------------------------------------------------------------------------------------------------------------------
+class Block(torch.nn.Module):
+    """A pre-norm sequence layer for serving: norm in 8 bits -> projections -> leaky attention -> projection; the sum is handed on."""
+
+    def __init__(self, width, heads, dk, dv):
+        super().__init__()
+        self.norm, self.att = layer.AddRMSNorm(width), layer.LeakyAttention(heads)
+        self.q, self.k = (layer.Int8Linear(torch.nn.Linear(width, heads * dk, bias=False), torch.bfloat16) for _ in range(2))
+        self.v = layer.Int8Linear(torch.nn.Linear(width, heads * dv, bias=False), torch.bfloat16)
+        self.norm_o, self.o = layer.AddRMSNorm(heads * dv), layer.Int8Linear(torch.nn.Linear(heads * dv, width), torch.bfloat16)
+        self.heads, self.dk, self.dv = heads, dk, dv
+
+    def forward_sequence(self, x, residual):
+        c, s, h = self.norm.forward_int8(x, residual)
+        q, k, v = self.q(c, s).unflatten(-1, (self.heads, self.dk)), self.k(c, s).unflatten(-1, (self.heads, self.dk)), self.v(c, s).unflatten(-1, (self.heads, self.dv))
+        o = self.att.forward_sequence(q, k, v) if x.dim() == 3 else self.att(q, k, v)
+        c, s, _ = self.norm_o.forward_int8(o.flatten(-2))
+        return self.o(c, s), h
+
+
+def test_block_sequence_equals_steps_and_the_definition():
+    torch.manual_seed(0)
+    T, B, W, H, D = 70, 2, 96, 3, 32
+    block = Block(W, H, D, D).to(DEV)
+    g = gen(1)
+    x, r = normal(g, T, B, W, dtype=torch.bfloat16).to(DEV), normal(g, T, B, W, dtype=torch.bfloat16).to(DEV)
+    with torch.no_grad():
+        y, h = block.forward_sequence(x, r)
+        last = block.att.s.clone()
+        functional.reset_net(block)
+        steps = torch.stack([block.forward_sequence(x[t], r[t])[0] for t in range(T)])
+    # the norms, products and codes before the attention are the same numbers; the attention's outputs differ by the tile form's roundings (2 * 2^-8 of the
+    # terms), which may move a code of the second norm by one: 1 / 127 of a row's largest value, against sums of 96 of them
+    assert (y.float() - steps.float()).square().mean().sqrt() <= 0.02 * y.float().square().mean().sqrt()
+    assert torch.allclose(last, block.att.s, rtol=1e-4, atol=1e-3)
+    # the definition in fp64, with the same codes
+    with torch.no_grad():
+        c, s, _ = block.norm.forward_int8(x, r)
+        n = c.cpu().double() * s.cpu().double()[..., None]
+        lin = lambda l, z: z @ (l.weight.cpu().double() * l.weight_scale.cpu().double()[:, None]).t() + (0 if l.bias is None else l.bias.cpu().double())   # noqa: E731
+        q, k, v = (lin(l, n).unflatten(-1, (H, D)) for l in (block.q, block.k, block.v))
+        o = leaky_ref(q, k, v, block.att.log_decay, D ** -0.5)[0].flatten(-2)
+        o = o / (o.square().mean(-1, keepdim=True) + 1e-6).sqrt()
+        want = lin(block.o, o)
+    # bf16 roundings of q, k, v, o and y (five halves of 2^-8) and the second norm's codes (uniform within half of 1/127 of the row's largest, about three
+    # times its rms): 5 * 2^-9 + 3 / 127 / sqrt(12) of the rms
+    assert (y.cpu().double() - want).square().mean().sqrt() <= 0.03 * want.square().mean().sqrt()
+
+
+def test_training_block_gradients():
+    """Norm -> projections -> leaky attention -> projection in fp32, its gradients against the definition's in fp64."""
+    torch.manual_seed(1)
+    T, B, W, H, D = 66, 2, 24, 2, 16
+    g = gen(2)
+    x, r = normal(g, T, B, W), normal(g, T, B, W)
+    wq, wk, wv, wo = (normal(g, H * D, W, std=0.2) for _ in range(3)), None, None, normal(g, W, H * D, std=0.2)
+    wq, wk, wv = tuple(wq)
+    nw = 1 + normal(g, W, std=0.1)
+    decay = torch.tensor([-0.02, -0.3])
+
+    def run(x, r, nw, wq, wk, wv, wo, norm, att):
+        n, h = norm(x, nw, r)
+        q, k, v = ((n @ w.t()).unflatten(-1, (H, D)) for w in (wq, wk, wv))
+        return att(q, k, v).flatten(-2) @ wo.t() + h
+
+    leaves = (x, r, nw, wq, wk, wv, wo)
+    ours = [t.to(DEV).requires_grad_() for t in leaves]
+    y = run(*ours, sequence.add_rms_norm, lambda q, k, v: sequence.leaky_attention(q, k, v, decay.to(DEV)))
+    ref = [t.double().requires_grad_() for t in leaves]
+    norm64 = lambda x, w, r: ((x + r) * ((x + r).square().mean(-1, keepdim=True) + 1e-6).rsqrt() * w, x + r)     # noqa: E731
+    want = run(*ref, norm64, lambda q, k, v: leaky_ref(q, k, v, decay, D ** -0.5)[0])
+    gy = normal(g, T, B, W)
+    got, exp = torch.autograd.grad(y, ours, gy.to(DEV)), torch.autograd.grad(want, ref, gy.double())
+    # chains of some 500 fp32 roundings, largely independent: 500 * u of the gradient's own norm is their worst case with a tenfold cancellation to spare
+    for a, b in zip((y, *got), (want, *exp)):
+        assert (a.cpu().double() - b).norm() <= 5000 * U * b.norm()
+
+
+def test_other_stream_and_repeat():
+    """On a side stream, and twice on the same inputs: the same bits."""
+    q, k, v, decay, s, _ = (t.to(DEV) if t is not None else None for t in leaky_case(300, 2, 4, 2, 64, 64, torch.bfloat16, True, False))
+    use = [t.requires_grad_() for t in (q, k, v)]
+    g = normal(gen(1), 300, 2, 4, 64, dtype=torch.bfloat16).to(DEV)
+
+    def once():
+        o = sequence.leaky_attention(*use, decay, state=s)
+        return (o, *torch.autograd.grad(o, use, g))
+
+    want = once()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = once()
+    side.synchronize()
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+
+
+def test_captured_calls_replay():
+    """A serving step (norm, product, attention step) and a prompt in two graphs, replayed in turn with eager work between: every replay is the eager result."""
+    torch.manual_seed(2)
+    block = Block(64, 2, 32, 32).to(DEV)
+    g = gen(3)
+    xs, rs = normal(g, 4, 3, 64, dtype=torch.bfloat16).to(DEV), normal(g, 4, 3, 64, dtype=torch.bfloat16).to(DEV)
+    ps, pr = normal(g, 100, 3, 64, dtype=torch.bfloat16).to(DEV), normal(g, 100, 3, 64, dtype=torch.bfloat16).to(DEV)
+    x, r, px, pres = xs[0].clone(), rs[0].clone(), ps.clone(), pr.clone()
+    state = torch.zeros(3, 2, 32, 32, device=DEV)
+
+    def step():
+        block.att.s = state
+        return block.forward_sequence(x, r)[0]
+
+    def prompt():
+        block.att.s = None
+        y = block.forward_sequence(px, pres)[0]
+        return y, block.att.s
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.no_grad():
+        step(), prompt()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    gs, gp = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.no_grad():
+        with torch.cuda.graph(gs):
+            ys = step()
+        with torch.cuda.graph(gp):
+            yp, sp = prompt()
+        state.zero_()
+        eager_state = torch.zeros_like(state)
+        for t in range(4):
+            x.copy_(xs[t]), r.copy_(rs[t]), px.copy_(ps.roll(t, 0)), pres.copy_(pr.roll(t, 0))
+            gp.replay()
+            gs.replay()
+            torch.cuda.synchronize()
+            block.att.s = eager_state
+            want = block.forward_sequence(xs[t], rs[t])[0]
+            assert torch.equal(ys, want) and torch.equal(state, eager_state)
+            wp, ws = prompt()
+            assert torch.equal(yp, wp) and torch.equal(sp, ws)
+
+
+def test_layer_protocol_on_the_device():
+    att = layer.LeakyAttention(2, tau=[2., 50.]).to(DEV)
+    q, k, v, _, _, _ = (t.to(DEV) if t is not None else None for t in leaky_case(6, 2, 2, 2, 16, 16, torch.float32, False, False))
+    want = sequence.leaky_attention(q, k, v, att.log_decay)
+    size = leaky_ref(q.abs(), k.abs(), v.abs(), att.log_decay, 0.25)[0]
+    first = att.forward_sequence(q[:3], k[:3], v[:3])
+    rest = torch.stack([att(q[t], k[t], v[t]) for t in range(3, 6)])
+    within(torch.cat((first, rest)), want, size * 200 * U, 'steps after a sequence')
+    functional.reset_net(att)
+    x = q.clone().requires_grad_()
+    out = torch.stack([att(x[t], k[t], v[t]) for t in range(6)])                 # single steps under autograd: back through time
+    assert torch.allclose(torch.autograd.grad(out.sum(), x)[0], torch.autograd.grad(sequence.leaky_attention(x, k, v, att.log_decay).sum(), x)[0], rtol=1e-4, atol=1e-4)
+    functional.detach_net(att)
+    with pytest.raises(sequence.SSNeuronError, match='reset_net'):
+        att(q[0, :1], k[0, :1], v[0, :1])

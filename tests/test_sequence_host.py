@@ -1,0 +1,176 @@
+"""CPU suite of the sequence operators: the library's exports and refusals, the Python checks, the layers' state protocol, weight quantisation."""
+import ctypes
+import math
+import os
+import re
+
+import pytest
+import torch
+
+from stereospike_amd import _seqlib, sequence
+from stereospike_amd._lib import SSNeuronError
+from stereospike_amd.clock_driven import functional, layer
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def test_header_binding_and_library_agree():
+    src = re.sub(r'/\*.*?\*/', '', open(os.path.join(ROOT, 'include', 'ss_sequence.h')).read(), flags=re.S)
+    declared = sorted(set(re.findall(r'\b(?:int|long long)\s+(ss_seq_[a-z0-9_]+)\s*\(', src)))
+    assert declared == sorted(_seqlib.EXPORTS)
+    L = _seqlib.lib()
+    for name in declared:
+        assert hasattr(L, name), name
+    assert L.ss_seq_abi_version() == _seqlib.ABI_VERSION
+    assert b'gfx950' in open(_seqlib.LIB_PATH, 'rb').read()
+
+
+def test_product_fails_loudly_on_cpu_tensors():
+    q = torch.zeros(2, 1, 1, 8)
+    with pytest.raises(SSNeuronError, match='no CPU fallback'):
+        sequence.leaky_attention(q, q, q, torch.zeros(1))
+    with pytest.raises(SSNeuronError, match='no CPU fallback'):
+        sequence.leaky_attention_step(q[0], q[0], q[0], torch.zeros(1), torch.zeros(1, 1, 8, 8))
+    with pytest.raises(SSNeuronError, match='no CPU fallback'):
+        sequence.add_rms_norm(q, torch.ones(8))
+    with pytest.raises(SSNeuronError, match='no CPU fallback'):
+        sequence.add_rms_norm_int8(q, torch.ones(8))
+    with pytest.raises(SSNeuronError, match='no CPU fallback'):
+        sequence.dequantize_int8(q.to(torch.int8), torch.ones(2, 1, 1))
+    with pytest.raises(SSNeuronError, match='no CPU fallback'):
+        sequence.int8_linear(q.to(torch.int8), torch.ones(2, 1, 1), torch.zeros(3, 8, dtype=torch.int8), torch.ones(3))
+
+
+def test_library_missing(monkeypatch):
+    monkeypatch.setattr(_seqlib, '_lib', None)
+    monkeypatch.setattr(_seqlib, 'LIB_PATH', '/nonexistent/libss_sequence.so')
+    with pytest.raises(SSNeuronError, match='not built'):
+        _seqlib.lib()
+
+
+def _desc(**kw):
+    d = _seqlib.LeakyDesc(size=ctypes.sizeof(_seqlib.LeakyDesc), T=1, B=1, H=1, DA=8, DC=8, a_group=1, b_group=1, c_group=1, a=256, b=256, c=256, out=256,
+                          log_decay=256, b_scale=1., o_scale=1.)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize('bad', [dict(size=8), dict(T=0), dict(B=0), dict(H=0), dict(DA=0), dict(DA=257), dict(DC=0), dict(DC=257), dict(dtype=3), dict(dtype=1, out_dtype=2),
+                                 dict(a_group=0), dict(b_group=2), dict(c_group=2), dict(a=0), dict(b=0), dict(c=0), dict(out=0), dict(log_decay=0), dict(B=70000)])
+def test_leaky_entry_refuses(bad):
+    """Refused on the host, before any HIP call (the pointers are never read)."""
+    assert _seqlib.lib().ss_seq_leaky(ctypes.byref(_desc(**bad)), None) == -22
+
+
+def test_other_entries_refuse():
+    L = _seqlib.lib()
+    assert L.ss_seq_leaky(None, None) == -22
+    assert L.ss_seq_group_sum(None, None, 1, 1, 1, 0, None) == -22
+    ok = (256, 8, None, 0, 256, 256, None, None, 4, 8, 1e-6, 0, None)
+    for at, value in ((0, None), (4, None), (5, None), (8, -1), (9, 0), (9, 16385), (10, -1.), (10, math.nan), (11, 3), (2, 256)):       # (residual without a sum)
+        bad = list(ok)
+        bad[at] = value
+        assert L.ss_seq_rms_norm_fwd(*bad) == -22, (at, value)
+    assert L.ss_seq_rms_norm_fwd(None, 0, None, 0, None, None, None, None, 0, 8, 1e-6, 0, None) == 0          # no rows: nothing to do
+    assert L.ss_seq_rms_norm_int8(256, 8, None, 0, 256, None, 256, None, 4, 8, 1e-6, 0, None) == -22
+    assert L.ss_seq_rms_norm_bwd(None, None, None, None, None, None, None, None, 4, 8, 0, None) == -22
+    assert L.ss_seq_rms_norm_bwd(None, None, 256, 256, 256, 256, 256, None, 4, 8, 0, None) == -22             # a weight gradient without its workspace
+    assert L.ss_seq_dequant_int8(None, None, None, 4, 8, 0, None) == -22
+    for M, N, K, dt in ((-1, 8, 8, 0), (1, 0, 8, 0), (1, 8, 0, 0), (1, 8, 131072, 0), (1, 8, 8, 5)):
+        assert L.ss_seq_int8_linear(256, K, 256, 256, K, 256, None, 256, M, N, K, dt, None, None) == -22
+    assert L.ss_seq_int8_linear(None, 8, 256, 256, 8, 256, None, 256, 1, 8, 8, 0, None, None) == -22
+
+
+@pytest.fixture
+def anywhere(monkeypatch):
+    """The checks behind the device check, on CPU tensors; no kernel may be reached."""
+    monkeypatch.setattr(sequence, '_require_hip', lambda t, name: None)
+    monkeypatch.setattr(_seqlib, 'lib', lambda: pytest.fail('a kernel was reached'))
+
+
+def _qkv(T=3, B=2, H=4, Hk=2, Dk=8, Dv=6, dtype=torch.float32):
+    return torch.zeros(T, B, H, Dk, dtype=dtype), torch.zeros(T, B, Hk, Dk, dtype=dtype), torch.zeros(T, B, Hk, Dv, dtype=dtype)
+
+
+def test_attention_refusals(anywhere):
+    q, k, v = _qkv()
+    g, i32 = torch.zeros(4), torch.int32
+    for args, kw, what in (((q.double(), k, v, g), {}, 'q: expected float32'), ((q[0], k, v, g), {}, '4 axes'), ((q, k.half(), v, g), {}, 'k: expected'),
+                           ((q, k[:2], v, g), {}, 'k: expected shape'), ((q, k, v[:, :1], g), {}, 'v: expected shape'), ((q[:, :, :3], k, v, g[:3]), {}, 'cannot share'),
+                           ((q, k, v, g[:2]), {}, 'log_decay'), ((q, k, v, g.double()), {}, 'log_decay'),
+                           ((q, k, v, torch.zeros(4, requires_grad=True)), {}, 'no gradient'),
+                           ((q, k, v, g), dict(state=torch.zeros(2, 4, 6, 8)), 'state: expected shape'),
+                           ((q, k, v, g), dict(state=torch.zeros(2, 4, 8, 6, dtype=torch.float16)), 'state: expected torch.float32'),
+                           ((q, k, v, g), dict(lengths=torch.zeros(2)), 'lengths: expected torch.int32'), ((q, k, v, g), dict(lengths=torch.zeros(3, dtype=i32)), 'lengths')):
+        with pytest.raises(SSNeuronError, match=what):
+            sequence.leaky_attention(*args, **kw)
+    with pytest.raises(SSNeuronError, match='head sizes'):
+        sequence.leaky_attention(*_qkv(Dk=257), g)
+    with pytest.raises(SSNeuronError, match='at most 65535'):
+        sequence.leaky_attention(*_qkv(T=1, B=16384, Dk=1, Dv=1), g)
+    s = torch.zeros(2, 4, 8, 6)
+    with pytest.raises(SSNeuronError, match='state: tensor must be contiguous'):
+        sequence.leaky_attention_step(q[0], k[0], v[0], g, torch.zeros(2, 4, 6, 8).transpose(2, 3))
+    with pytest.raises(SSNeuronError, match='3 axes'):
+        sequence.leaky_attention_step(q, k, v, g, s)
+    # no step, no stream: no launch
+    o, last = sequence.leaky_attention(q[:0], k[:0], v[:0], g, state=s + 2, return_state=True)
+    assert o.shape == (0, 2, 4, 6) and torch.equal(last, s + 2)
+    assert sequence.leaky_attention(q[:, :0], k[:, :0], v[:, :0], g).shape == (3, 0, 4, 6)
+    assert sequence.leaky_attention_step(q[0, :0], k[0, :0], v[0, :0], g, s[:0]).shape == (0, 4, 6)
+
+
+def test_norm_and_product_refusals(anywhere):
+    x, w = torch.zeros(3, 8), torch.ones(8)
+    for args, kw, what in (((x.double(), w), {}, 'x: expected'), ((x, w[:4]), {}, 'weight'), ((x, w.half()), {}, 'weight'), ((x, w), dict(residual=x.half()), 'residual'),
+                           ((x, w), dict(residual=x[:2]), 'residual'), ((x, w), dict(eps=-1.), 'eps'), ((torch.zeros(1, 16385), torch.ones(16385)), {}, 'rows of')):
+        with pytest.raises(SSNeuronError, match=what):
+            sequence.add_rms_norm(*args, **kw)
+        with pytest.raises(SSNeuronError, match=what):
+            sequence.add_rms_norm_int8(*args, **kw)
+    assert sequence.add_rms_norm(x[:0], w)[0].shape == (0, 8)
+    assert [t.shape for t in sequence.add_rms_norm_int8(x[:0], w, x[:0])] == [(0, 8), (0,), (0, 8)]
+    a, sa, b, sb = torch.zeros(3, 8, dtype=torch.int8), torch.ones(3), torch.zeros(5, 8, dtype=torch.int8), torch.ones(5)
+    for args, kw, what in (((a.float(), sa, b, sb), {}, 'codes'), ((a[:, :4], sa, b, sb), {}, 'codes'), ((a, sa[:2], b, sb), {}, 'scales'), ((a, sa, b.float(), sb), {}, 'weight'),
+                           ((a, sa, b, sb[:4]), {}, 'weight_scale'), ((a, sa, b, sb), dict(bias=torch.ones(4)), 'bias'), ((a, sa, b, sb), dict(out_dtype=torch.int32), 'out_dtype'),
+                           ((a, sa, b[0], sb), {}, 'weight'), ((a, sa.requires_grad_(), b, sb), {}, 'no gradient')):
+        with pytest.raises(SSNeuronError, match=what):
+            sequence.int8_linear(*args, **kw)
+    with pytest.raises(SSNeuronError, match='K <= 131071'):
+        sequence.int8_linear(torch.zeros(1, 131072, dtype=torch.int8), torch.ones(1), torch.zeros(1, 131072, dtype=torch.int8), torch.ones(1))
+    with pytest.raises(SSNeuronError, match='scales'):
+        sequence.dequantize_int8(a, torch.ones(2))
+    with pytest.raises(SSNeuronError, match='dtype'):
+        sequence.dequantize_int8(a, torch.ones(3), torch.float64)
+
+
+def test_quantize_channels():
+    torch.manual_seed(0)
+    w = torch.randn(5, 40)
+    w[3] = 0
+    codes, scale = sequence.quantize_channels(w)
+    assert codes.dtype == torch.int8 and codes.abs().max() == 127 and scale[3] == 0 and not codes[3].any()
+    # half a code's step, and the scale's own rounding (2^-24) over 127 codes
+    assert ((codes * scale[:, None]).double() - w.double()).abs().le(scale[:, None].double() * (0.5 + 127 * 2. ** -23)).all()
+    with pytest.raises(SSNeuronError, match='weight'):
+        sequence.quantize_channels(torch.zeros(3, dtype=torch.float32))
+
+
+def test_layers_keep_the_state_protocol():
+    att = layer.LeakyAttention(4)
+    tau = 1. / -torch.expm1(att.log_decay.double())
+    assert torch.allclose(tau, 2. * 512. ** (torch.arange(4).double() / 3), rtol=1e-4)        # tau = 1 / (1 - lambda): 1024 times the rounding of log lambda
+    att.s = torch.ones(1, 4, 2, 2, requires_grad=True) * 2
+    functional.detach_net(att)
+    assert not att.s.requires_grad
+    functional.reset_net(att)
+    assert att.s is None
+    assert layer.LeakyAttention(2, tau=[1., math.inf]).log_decay.tolist() == [-math.inf, 0.]
+    with pytest.raises(AssertionError):
+        layer.LeakyAttention(2, tau=[0.5, 2.])
+    lin = torch.nn.Linear(6, 3)
+    q = layer.Int8Linear(lin)
+    assert set(q.state_dict()) == {'weight', 'weight_scale', 'bias'} and q.weight.dtype == torch.int8
+    assert layer.Int8Linear(torch.nn.Linear(6, 3, bias=False)).bias is None
+    assert list(layer.AddRMSNorm(7).state_dict()) == ['weight']
