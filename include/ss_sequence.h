@@ -41,8 +41,8 @@ int ss_seq_abi_version(void);
  *   gradient of v  a, b, c = k, q, g     b_scale scale, o_scale 1, reverse, s_in = gradient of the last state; s_out = gradient of the first state
  *
  * a [T][B][H / a_group][DA], b [T][B][H / b_group][DA], c [T][B][H / c_group][DC], out [T][B][H][DC] with the strides given; head h reads operand head
- * h / group.  s_in / s_out: [B][H] matrices DA x DC, element (i, j) at i * s_*_row + j * s_*_col, matrices DA * DC apart.  s_in may alias s_out when the
- * strides are the same.
+ * h / group.  s_in / s_out: [B][H] matrices DA x DC, element (i, j) at i * s_*_row + j * s_*_col, matrices DA * DC apart.  s_in may be s_out itself
+ * when T = 1 and their strides are the same.
  */
 struct ss_seq_leaky_desc {
     unsigned size;                       /* sizeof(struct ss_seq_leaky_desc) */

@@ -1,0 +1,598 @@
+// ss_seq_attention.hpp — leaky attention: a matrix-valued leaky integrator per head, read by a query.
+//
+//   S_i = lambda S_{i-1} + b_scale b_i c_i^T,   out_i = o_scale a_i^T S_i,   lambda = exp(log_decay) of the head
+//
+// The forward pass and the three token gradients are this one map with other operands, forwards or backwards in time (ss_sequence.h).  One unit per element
+// type instantiates it (ss_seq_attention_{f32,f16,bf16}.hip).
+#pragma once
+#include "ss_seq_common.hpp"
+
+// (in ss_seq_attention.hip: checks and dispatch by element type)
+struct LeakyArgs {
+    int T, B, H, DA, DC, reverse;
+    float b_scale, o_scale;
+    const void *a, *b, *c;
+    void* out;
+    long long a_t, a_b, a_h, b_t, b_b, b_h, c_t, c_b, c_h, o_t, o_b, o_h;
+    int a_group, b_group, c_group;
+    const float* log_decay;
+    const int* lengths;
+    const float* s_in;
+    float* s_out;
+    int s_in_row, s_in_col, s_out_row, s_out_col;
+    int out_f32;
+};
+
+long long ss_seq_leaky_ws_f32(const LeakyArgs&);
+long long ss_seq_leaky_ws_f16(const LeakyArgs&);
+long long ss_seq_leaky_ws_bf16(const LeakyArgs&);
+int ss_seq_leaky_f32(const LeakyArgs&, float* ws, hipStream_t);
+int ss_seq_leaky_f16(const LeakyArgs&, float* ws, hipStream_t);
+int ss_seq_leaky_bf16(const LeakyArgs&, float* ws, hipStream_t);
+
+namespace {
+
+
+// The recurrence itself, one step after the other with the state in registers: HBM-bound on reading and writing the state when T is small (the single-step
+// call).  A workgroup owns 64 columns of one head's state: thread (g, x) holds rows g + 16 r of columns 4 x .. 4 x + 3.
+template <int DT, int ODT, int R, bool V4> __global__ __launch_bounds__(256) void leaky_steps_kernel(const LeakyArgs p)
+{
+    __shared__ float sa[256], sb[256], red[4][64];
+    const int tid = threadIdx.x, x = tid & 15, g = tid >> 4;
+    const int bh = blockIdx.y, b = bh / p.H, h = bh % p.H, j0 = blockIdx.x * 64 + 4 * x;
+    int n = p.T;
+    if (p.lengths) { n = p.lengths[b]; n = n < 0 ? 0 : n > p.T ? p.T : n; }
+    // lambda S as S + S * expm1(g) while lambda is over a half: a rounded lambda near 1 would drift over many steps (2^-25 of it each)
+    const float g_h = fmaxf(p.log_decay[h], -1e30f), lam = expf(g_h), leak = g_h > -0.69f ? expm1f(g_h) : lam, kept = g_h > -0.69f ? 1.f : 0.f;
+    const elem_t<DT>* pa = static_cast<const elem_t<DT>*>(p.a) + b * p.a_b + (h / p.a_group) * p.a_h;
+    const elem_t<DT>* pb = static_cast<const elem_t<DT>*>(p.b) + b * p.b_b + (h / p.b_group) * p.b_h;
+    const elem_t<DT>* pc = static_cast<const elem_t<DT>*>(p.c) + b * p.c_b + (h / p.c_group) * p.c_h;
+    elem_t<ODT>* po = static_cast<elem_t<ODT>*>(p.out) + b * p.o_b + h * p.o_h;
+    const float* s_in = p.s_in ? p.s_in + (long long)bh * p.DA * p.DC : nullptr;
+    float* s_out = p.s_out ? p.s_out + (long long)bh * p.DA * p.DC : nullptr;
+    f32x4 S[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        S[r] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        const int i = g + 16 * r;
+        if (s_in && i < p.DA) {
+            if constexpr (V4) { if (j0 < p.DC) S[r] = *reinterpret_cast<const f32x4*>(s_in + i * p.s_in_row + j0); }
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e) if (j0 + e < p.DC) S[r][e] = s_in[i * p.s_in_row + (j0 + e) * p.s_in_col];
+        }
+    }
+    for (int i = 0; i < n; ++i) {
+        const long long t = p.reverse ? n - 1 - i : i;
+        __syncthreads();
+        if (tid < p.DA) { sa[tid] = widen<DT>(pa[t * p.a_t + tid]) * p.o_scale; sb[tid] = widen<DT>(pb[t * p.b_t + tid]) * p.b_scale; }
+        __syncthreads();
+        f32x4 c = {0.f, 0.f, 0.f, 0.f}, o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) if (j0 + e < p.DC) c[e] = widen<DT>(pc[t * p.c_t + j0 + e]);
+        const bool leaks = i > 0 || !p.reverse;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int row = g + 16 * r;
+            if (row < p.DA) {
+                const float bi = sb[row], ai = sa[row];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float s = S[r][e];
+                    if (leaks) s = fmaf(s, leak, s * kept);
+                    s = fmaf(bi, c[e], s);
+                    o[e] = fmaf(ai, s, o[e]);
+                    S[r][e] = s;
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            o[e] += __shfl_xor(o[e], 16);
+            o[e] += __shfl_xor(o[e], 32);
+        }
+        if ((tid & 48) == 0) *reinterpret_cast<f32x4*>(&red[tid >> 6][4 * x]) = o;
+        __syncthreads();
+        if (tid < 64 && blockIdx.x * 64 + tid < p.DC)
+            po[t * p.o_t + blockIdx.x * 64 + tid] = narrow<ODT>(red[0][tid] + red[1][tid] + red[2][tid] + red[3][tid]);
+    }
+    if (tid < 64 && blockIdx.x * 64 + tid < p.DC)
+        for (int t = n; t < p.T; ++t) po[t * p.o_t + blockIdx.x * 64 + tid] = 0;
+    if (s_out) {
+        const float last = p.reverse && n > 0 ? lam : 1.f;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int i = g + 16 * r;
+            if (i < p.DA) {
+                if constexpr (V4) { if (j0 < p.DC) *reinterpret_cast<f32x4*>(s_out + i * p.s_out_row + j0) = S[r] * last; }
+                else
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) if (j0 + e < p.DC) s_out[i * p.s_out_row + (j0 + e) * p.s_out_col] = S[r][e] * last;
+            }
+        }
+    }
+}
+
+template <int DT, int ODT> int steps(const LeakyArgs& p, hipStream_t s)
+{
+    const bool v4 = p.DC % 4 == 0 && (!p.s_in || (p.s_in_col == 1 && p.s_in_row % 4 == 0 && aligned(p.s_in, 16))) &&
+                    (!p.s_out || (p.s_out_col == 1 && p.s_out_row % 4 == 0 && aligned(p.s_out, 16)));
+    const dim3 grid((unsigned)((p.DC + 63) / 64), (unsigned)(p.B * p.H));
+    auto go = [&](auto R) {
+        if (v4) leaky_steps_kernel<DT, ODT, R.value, true><<<grid, 256, 0, s>>>(p);
+        else leaky_steps_kernel<DT, ODT, R.value, false><<<grid, 256, 0, s>>>(p);
+        return launched();
+    };
+    if (p.DA <= 64) return go(std::integral_constant<int, 4>());
+    if (p.DA <= 128) return go(std::integral_constant<int, 8>());
+    return go(std::integral_constant<int, 16>());
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------------------------------
+// The tile form.  A chunk of CH steps is four products, with W the state as the NEXT step would see it (already leaked once):
+//
+//   P_ij  = a_i . b_j * lambda^(i-j)  (j <= i)             (1)
+//   out_i = sum_j P_ij c_j                                 (2)
+//         + lambda^i a_i W                                 (3)
+//   W    <- lambda^CH W + sum_j lambda^(CH-j) b_j c_j^T    (4)
+//
+// A workgroup owns 64 NT columns of one head's state for one SEGMENT of the steps; wavefront w owns 16 NT of them, with all DA rows of W in its registers.
+// Products are taken so that accumulators ARE the next product's operand: a 16 x 16 accumulator gives lane l rows 4 (l / 16) .. + 3 of column l % 16; two
+// of them, one above the other, are the 8 contraction values of a 16x16x32 operand in the order {4g .. 4g+3, 16+4g .. 16+4g+3} (four 16x16x4 operands in
+// fp32).  a and b are staged in LDS in that order, so W never leaves the registers; P is shared between the wavefronts through LDS in operand order.
+// Out comes out transposed: a lane stores four consecutive columns of one step.
+//
+// Rounding (bf16): P and W are rounded to bf16 as operands of (2) and (3), each term once; (4) splits lambda^(CH-j) c_j into three bf16 terms (24 bits), so the
+// state keeps fp32 accuracy.  fp32 and fp16 run on the fp32 matrix instructions: P and W may leave fp16's range, and the state has to keep fp32's accuracy.
+// ---------------------------------------------------------------------------------------------------------------------------------------------------------
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef s16x4 __attribute__((address_space(3))) * lds_s16x4;
+
+struct LeakyPlan {
+    int nseg, seg;                           // segments and their steps (a multiple of the chunk)
+    int ncb;                                 // column blocks
+    int fold;                                // the output pass joins the segments' states itself (no scan launch)
+};
+
+__device__ __forceinline__ unsigned pack_hi16(float lo, float hi) { return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u); }
+__device__ __forceinline__ float top16(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFF0000u); }
+__device__ __forceinline__ bf16x8 mk8(unsigned a, unsigned b, unsigned c, unsigned d)
+{
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(bf16x8, (u32x4){a, b, c, d});
+}
+__device__ __forceinline__ unsigned round_pk(float lo, float hi)
+{
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, (bf16x2){(__bf16)lo, (__bf16)hi});
+}
+
+template <int DT, int DA, int NT, bool STATE>
+__global__ __launch_bounds__(256, DA <= 128 ? 2 : 1) void leaky_chunk_kernel(const LeakyArgs p, const LeakyPlan plan, const int vec, const int vec_out, float* __restrict__ ws)
+{
+    constexpr bool BF = DT == SS_SEQ_BF16;
+    constexpr int CH = BF ? 64 : 32, DCB = 64 * NT, IT = CH / 16, KA = DA / 16;
+    typedef typename std::conditional<BF, unsigned short, float>::type LT;
+    constexpr int SA = DA + (BF ? 8 : 4), SC = DCB + (BF ? 8 : 4);       // LDS rows 16 bytes longer than a power of two
+    constexpr int GA = CH * DA / 8 / 256, GC = CH * DCB / 8 / 256;       // 8-element granules per thread
+    __shared__ __attribute__((aligned(16))) LT sa[STATE ? 8 : CH * SA];
+    __shared__ __attribute__((aligned(16))) LT sb[CH * SA];
+    __shared__ __attribute__((aligned(16))) LT sc[CH * SC];
+    __shared__ __attribute__((aligned(16))) LT sp[STATE ? 8 : (BF ? IT * (IT / 2) * 64 * 8 : IT * IT * 64 * 4)];
+    __shared__ __attribute__((aligned(16))) float rw[CH];                // lambda^(e - j) b_scale of the chunk's steps
+    typedef Pack<DT, 8> G;
+
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g = lane >> 4;
+    const int cb = blockIdx.x % plan.ncb, rest = blockIdx.x / plan.ncb;
+    const int nst = STATE ? plan.nseg - 1 : plan.nseg, seg = rest % nst, bh = rest / nst, b = bh / p.H, h = bh - b * p.H;
+    int n = p.T;
+    if (p.lengths) { n = p.lengths[b]; n = n < 0 ? 0 : n > p.T ? p.T : n; }
+    const int start = seg * plan.seg, stop = n < start + plan.seg ? n : start + plan.seg;      // this segment's valid steps
+    if (STATE && n <= start + plan.seg) return;                          // no later segment reads this one's state
+    const float gl = fmaxf(p.log_decay[h], -1e30f) * 1.44269504088896341f;                     // log2 lambda
+    const int c0 = cb * DCB, col0 = c0 + wv * 16 * NT;
+    const elem_t<DT>* pa = static_cast<const elem_t<DT>*>(p.a) + b * p.a_b + (h / p.a_group) * p.a_h;
+    const elem_t<DT>* pb = static_cast<const elem_t<DT>*>(p.b) + b * p.b_b + (h / p.b_group) * p.b_h;
+    const elem_t<DT>* pc = static_cast<const elem_t<DT>*>(p.c) + b * p.c_b + (h / p.c_group) * p.c_h + c0;
+    const int dc = p.DC - c0 < DCB ? p.DC - c0 : DCB;
+
+    // ---- the state that enters the segment
+    f32x4 W[KA][NT];
+    {
+        const long long per = (long long)DA * DCB;
+        const float* mine = ws + ((long long)bh * plan.ncb + cb) * (plan.nseg - 1) * per + (wv * KA * NT) * 256 + lane * 4;
+        if (seg == 0) {
+            const float* s_in = p.s_in ? p.s_in + (long long)bh * p.DA * p.DC : nullptr;
+            const float first = p.reverse || n == 0 ? 1.f : exp2f(gl);
+#pragma unroll
+            for (int kt = 0; kt < KA; ++kt)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int i = 16 * kt + 4 * g + r, j = col0 + 16 * nt + l16;
+                        W[kt][nt][r] = s_in && i < p.DA && j < p.DC ? s_in[i * p.s_in_row + j * p.s_in_col] * first : 0.f;
+                    }
+        } else if constexpr (STATE) {
+#pragma unroll
+            for (int kt = 0; kt < KA; ++kt)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) W[kt][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        } else if (start < n) {
+            const int from = plan.fold ? 0 : seg - 1;
+            const float leak = exp2f(gl * (float)plan.seg);
+#pragma unroll
+            for (int kt = 0; kt < KA; ++kt)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) W[kt][nt] = *reinterpret_cast<const f32x4*>(mine + from * per + (kt * NT + nt) * 256);
+            for (int s = from + 1; s < seg; ++s)
+#pragma unroll
+                for (int kt = 0; kt < KA; ++kt)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) W[kt][nt] = W[kt][nt] * leak + *reinterpret_cast<const f32x4*>(mine + s * per + (kt * NT + nt) * 256);
+        }
+    }
+
+    // ---- staging: global -> registers (one chunk ahead) -> LDS
+    G ra[STATE ? 1 : GA], rb[GA], rc[GC];
+    auto fetch = [&](const elem_t<DT>* base, long long st, int i, int q, int d, G& o) {
+        const bool in = i < stop && 8 * q < d;
+        if (vec) {
+            if (in) o = *reinterpret_cast<const G*>(base + (long long)(p.reverse ? n - 1 - i : i) * st + 8 * q);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o.v[e] = 0;
+        } else {
+            const elem_t<DT>* src = base + (long long)(p.reverse ? n - 1 - i : i) * st + 8 * q;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { o.v[e] = 0; if (in && 8 * q + e < d) o.v[e] = src[e]; }
+        }
+    };
+    auto load = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < GA; ++u) {
+            const int id = tid + 256 * u, row = id / (DA / 8), q = id % (DA / 8);
+            if constexpr (!STATE) fetch(pa, p.a_t, i0 + row, q, p.DA, ra[u]);
+            fetch(pb, p.b_t, i0 + row, q, p.DA, rb[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < GC; ++u) {
+            const int id = tid + 256 * u, row = id / (DCB / 8), q = id % (DCB / 8);
+            fetch(pc, p.c_t, i0 + row, q, dc, rc[u]);
+        }
+    };
+    auto put = [&](LT* dst, const G& v, int row, int q) {                // rows of a, b: operand order within blocks of 32 (bf16)
+        if constexpr (BF) {
+            LT* at = dst + row * SA + (q >> 2) * 32 + ((q & 3) >> 1) * 4 + (q & 1) * 16;
+            *reinterpret_cast<u16x4*>(at) = (u16x4){v.v[0], v.v[1], v.v[2], v.v[3]};
+            *reinterpret_cast<u16x4*>(at + 8) = (u16x4){v.v[4], v.v[5], v.v[6], v.v[7]};
+        } else {
+            LT* at = dst + row * SA + 8 * q;
+            *reinterpret_cast<f32x4*>(at) = (f32x4){widen<DT>(v.v[0]), widen<DT>(v.v[1]), widen<DT>(v.v[2]), widen<DT>(v.v[3])};
+            *reinterpret_cast<f32x4*>(at + 4) = (f32x4){widen<DT>(v.v[4]), widen<DT>(v.v[5]), widen<DT>(v.v[6]), widen<DT>(v.v[7])};
+        }
+    };
+    auto stage = [&]() {
+#pragma unroll
+        for (int u = 0; u < GA; ++u) {
+            const int id = tid + 256 * u, row = id / (DA / 8), q = id % (DA / 8);
+            if constexpr (!STATE) put(sa, ra[u], row, q);
+            put(sb, rb[u], row, q);
+        }
+#pragma unroll
+        for (int u = 0; u < GC; ++u) {
+            const int id = tid + 256 * u, row = id / (DCB / 8), q = id % (DCB / 8);
+            if constexpr (BF) *reinterpret_cast<G*>(sc + row * SC + 8 * q) = rc[u];
+            else {
+                *reinterpret_cast<f32x4*>(sc + row * SC + 8 * q) = (f32x4){widen<DT>(rc[u].v[0]), widen<DT>(rc[u].v[1]), widen<DT>(rc[u].v[2]), widen<DT>(rc[u].v[3])};
+                *reinterpret_cast<f32x4*>(sc + row * SC + 8 * q + 4) = (f32x4){widen<DT>(rc[u].v[4]), widen<DT>(rc[u].v[5]), widen<DT>(rc[u].v[6]), widen<DT>(rc[u].v[7])};
+            }
+        }
+    };
+    auto store = [&](int i, int it_nt_col, const f32x4& v) {             // four columns of step i
+        if (i >= p.T) return;
+        const bool live = i < n;
+        const long long t = live && p.reverse ? n - 1 - i : i;
+        const long long at = b * p.o_b + h * p.o_h + t * p.o_t + it_nt_col;
+        const f32x4 o = live ? v : (f32x4){0.f, 0.f, 0.f, 0.f};
+        if (p.out_f32) {
+            float* q = static_cast<float*>(p.out) + at;
+            if (vec_out && it_nt_col < p.DC) *reinterpret_cast<f32x4*>(q) = o;
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e) if (it_nt_col + e < p.DC) q[e] = o[e];
+        } else {
+            elem_t<DT>* q = static_cast<elem_t<DT>*>(p.out) + at;
+            if (vec_out && it_nt_col < p.DC) {
+                Pack<DT, 4> w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w.v[e] = narrow<DT>(o[e]);
+                *reinterpret_cast<Pack<DT, 4>*>(q) = w;
+            } else
+#pragma unroll
+                for (int e = 0; e < 4; ++e) if (it_nt_col + e < p.DC) q[e] = narrow<DT>(o[e]);
+        }
+    };
+
+    if constexpr (!STATE && BF) {                                        // the halves of P's operands that lie above the diagonal stay zero
+        for (int i = tid; i < IT * (IT / 2) * 64; i += 256) *reinterpret_cast<f32x4*>(sp + i * 8) = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+    float row_scale[IT];                                                 // lambda^i o_scale of this lane's steps
+    if constexpr (!STATE)
+#pragma unroll
+        for (int it = 0; it < IT; ++it) row_scale[it] = exp2f(gl * (float)(16 * it + l16)) * p.o_scale;
+    if (tid < CH) rw[tid] = exp2f(gl * (float)(CH - tid)) * p.b_scale;
+
+    load(start);
+    int i0 = start;
+    for (; i0 < stop; i0 += CH) {
+        const int cnt = stop - i0 < CH ? stop - i0 : CH;
+        // the last chunk of the stream leaves the state as it is after its last step (forward) or leaked once more (reverse)
+        const bool final = i0 + cnt == n;
+        const int e = final && !p.reverse ? cnt - 1 : cnt;
+        __syncthreads();                                                 // the last chunk has been read
+        stage();
+        if (e != CH && tid < CH) rw[tid] = exp2f(gl * (float)(e > tid ? e - tid : 0)) * p.b_scale;
+        __syncthreads();
+        if (i0 + CH < stop) load(i0 + CH);
+
+        f32x4 acc[STATE ? 1 : IT][NT];
+        if constexpr (!STATE) {
+            // (1) the tiles on and below the diagonal, dealt to the wavefronts
+#pragma unroll
+            for (int z = 0; z < (IT * (IT + 1) / 2 + 3) / 4; ++z) {
+                const int idx = wv + 4 * z;
+                if (idx < IT * (IT + 1) / 2) {
+                    const int it = idx < 1 ? 0 : idx < 3 ? 1 : idx < 6 ? 2 : 3, jt = idx - it * (it + 1) / 2;
+                    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+                    const LT* qa = sa + (16 * it + l16) * SA;
+                    const LT* qb = sb + (16 * jt + l16) * SA;
+                    if constexpr (BF) {
+#pragma unroll
+                        for (int k = 0; k < DA / 32; ++k)
+                            s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(qb + 32 * k + 8 * g), *reinterpret_cast<const bf16x8*>(qa + 32 * k + 8 * g), s, 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < KA; ++k) {
+                            const f32x4 fb = *reinterpret_cast<const f32x4*>(qb + 16 * k + 4 * g), fa = *reinterpret_cast<const f32x4*>(qa + 16 * k + 4 * g);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) s = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[r], fa[r], s, 0, 0, 0);
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int d = 16 * (it - jt) + l16 - 4 * g - r;  // i - j
+                        s[r] = d < 0 ? 0.f : s[r] * (exp2f(gl * (float)d) * p.b_scale * p.o_scale);
+                    }
+                    if constexpr (BF) {
+                        typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+                        *reinterpret_cast<u32x2*>(sp + ((it * (IT / 2) + (jt >> 1)) * 64 + lane) * 8 + (jt & 1) * 4) = (u32x2){round_pk(s[0], s[1]), round_pk(s[2], s[3])};
+                    } else *reinterpret_cast<f32x4*>(sp + ((it * IT + jt) * 64 + lane) * 4) = s;
+                }
+            }
+            // (3)
+#pragma unroll
+            for (int it = 0; it < IT; ++it)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) acc[it][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            if constexpr (BF) {
+#pragma unroll
+                for (int k = 0; k < KA / 2; ++k) {
+                    bf16x8 fw[NT];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const f32x4 x = W[2 * k][nt], y = W[2 * k + 1][nt];
+                        fw[nt] = mk8(round_pk(x[0], x[1]), round_pk(x[2], x[3]), round_pk(y[0], y[1]), round_pk(y[2], y[3]));
+                    }
+#pragma unroll
+                    for (int it = 0; it < IT; ++it) {
+                        const bf16x8 fa = *reinterpret_cast<const bf16x8*>(sa + (16 * it + l16) * SA + 32 * k + 8 * g);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) acc[it][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[nt], fa, acc[it][nt], 0, 0, 0);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < KA; ++k)
+#pragma unroll
+                    for (int it = 0; it < IT; ++it) {
+                        const f32x4 fa = *reinterpret_cast<const f32x4*>(sa + (16 * it + l16) * SA + 16 * k + 4 * g);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) acc[it][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(W[k][nt][r], fa[r], acc[it][nt], 0, 0, 0);
+                    }
+            }
+#pragma unroll
+            for (int it = 0; it < IT; ++it)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) acc[it][nt] *= row_scale[it];
+            __syncthreads();                                             // P is there
+        }
+        // (2) and (4) share the wavefront's columns of c
+        const float keep = exp2f(gl * (float)e);
+#pragma unroll
+        for (int kt = 0; kt < KA; ++kt)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) W[kt][nt] *= keep;
+        if constexpr (BF) {
+#pragma unroll
+            for (int kk = 0; kk < CH / 32; ++kk) {
+                bf16x8 t0[NT], t1[NT], t2[NT];
+                const f32x4 w0 = *reinterpret_cast<const f32x4*>(rw + 32 * kk + 4 * g), w1 = *reinterpret_cast<const f32x4*>(rw + 32 * kk + 16 + 4 * g);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const LT* q = sc + (32 * kk + 4 * g + (l16 >> 2)) * SC + wv * 16 * NT + 16 * nt + 4 * (l16 & 3);
+                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)q), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(q + 16 * SC));
+                    const s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                    if constexpr (!STATE) {
+                        const bf16x8 fc = __builtin_bit_cast(bf16x8, both);
+#pragma unroll
+                        for (int it = 2 * kk; it < IT; ++it)
+                            acc[it][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fc, *reinterpret_cast<const bf16x8*>(sp + ((it * (IT / 2) + kk) * 64 + lane) * 8), acc[it][nt], 0, 0, 0);
+                    }
+                    float x[8], y[8], z[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float v = __uint_as_float((unsigned)(unsigned short)both[i] << 16) * (i < 4 ? w0[i & 3] : w1[i & 3]);
+                        x[i] = top16(v);
+                        y[i] = v - x[i];
+                        z[i] = y[i] - top16(y[i]);
+                    }
+                    t0[nt] = mk8(pack_hi16(x[0], x[1]), pack_hi16(x[2], x[3]), pack_hi16(x[4], x[5]), pack_hi16(x[6], x[7]));
+                    t1[nt] = mk8(pack_hi16(y[0], y[1]), pack_hi16(y[2], y[3]), pack_hi16(y[4], y[5]), pack_hi16(y[6], y[7]));
+                    t2[nt] = mk8(pack_hi16(z[0], z[1]), pack_hi16(z[2], z[3]), pack_hi16(z[4], z[5]), pack_hi16(z[6], z[7]));
+                }
+#pragma unroll
+                for (int kt = 0; kt < KA; ++kt) {
+                    const LT* q = sb + (32 * kk + 4 * g + (l16 >> 2)) * SA + 32 * (kt >> 1) + 8 * (l16 & 3) + 4 * (kt & 1);
+                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)q), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(q + 16 * SA));
+                    const bf16x8 fb = __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        W[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, t2[nt], W[kt][nt], 0, 0, 0);
+                        W[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, t1[nt], W[kt][nt], 0, 0, 0);
+                        W[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, t0[nt], W[kt][nt], 0, 0, 0);
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int jt = 0; jt < IT; ++jt) {
+                const f32x4 w = *reinterpret_cast<const f32x4*>(rw + 16 * jt + 4 * g);
+                float fc[4][NT];
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) fc[r][nt] = sc[(16 * jt + 4 * g + r) * SC + wv * 16 * NT + 16 * nt + l16];
+                if constexpr (!STATE)
+#pragma unroll
+                    for (int it = jt; it < IT; ++it) {
+                        const f32x4 fp = *reinterpret_cast<const f32x4*>(sp + ((it * IT + jt) * 64 + lane) * 4);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) acc[it][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(fc[r][nt], fp[r], acc[it][nt], 0, 0, 0);
+                    }
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) fc[r][nt] *= w[r];
+#pragma unroll
+                for (int kt = 0; kt < KA; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float fb = sb[(16 * jt + 4 * g + r) * SA + 16 * kt + l16];
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) W[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb, fc[r][nt], W[kt][nt], 0, 0, 0);
+                    }
+            }
+        }
+        if constexpr (!STATE)
+#pragma unroll
+            for (int it = 0; it < IT; ++it)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) store(i0 + 16 * it + l16, col0 + 16 * nt + 4 * g, acc[it][nt]);
+    }
+
+    if constexpr (STATE) {
+        const long long per = (long long)DA * DCB;
+        float* mine = ws + (((long long)bh * plan.ncb + cb) * (plan.nseg - 1) + seg) * per + (wv * KA * NT) * 256 + lane * 4;
+#pragma unroll
+        for (int kt = 0; kt < KA; ++kt)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) *reinterpret_cast<f32x4*>(mine + (kt * NT + nt) * 256) = W[kt][nt];
+    } else {
+        // steps of the segment behind the stream's last: zeros (the loop above has written its own chunks to their end)
+        const int end = start + plan.seg < p.T ? start + plan.seg : p.T;
+        for (; i0 < end; i0 += CH)
+#pragma unroll
+            for (int it = 0; it < IT; ++it)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) store(i0 + 16 * it + l16, col0 + 16 * nt + 4 * g, (f32x4){0.f, 0.f, 0.f, 0.f});
+        if (p.s_out && ((start < n && n <= start + plan.seg) || (n == 0 && seg == 0))) {
+            float* s_out = p.s_out + (long long)bh * p.DA * p.DC;
+#pragma unroll
+            for (int kt = 0; kt < KA; ++kt)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int i = 16 * kt + 4 * g + r, j = col0 + 16 * nt + l16;
+                        if (i < p.DA && j < p.DC) s_out[i * p.s_out_row + j * p.s_out_col] = W[kt][nt][r];
+                    }
+        }
+    }
+}
+
+// ws[s] (what segment s adds to the state) -> the state that enters segment s + 1
+__global__ __launch_bounds__(256) void leaky_scan_kernel(float* __restrict__ ws, const float* __restrict__ log_decay, int H, int ncb, int per, int nstate, int seg)
+{
+    const int bh = blockIdx.y / ncb;
+    const float leak = exp2f(fmaxf(log_decay[bh % H], -1e30f) * 1.44269504088896341f * (float)seg);
+    float* at = ws + (long long)blockIdx.y * nstate * per + (blockIdx.x * 256 + threadIdx.x) * 4;
+    f32x4 s = *reinterpret_cast<const f32x4*>(at);
+    for (int k = 1; k < nstate; ++k) {
+        at += per;
+        s = s * leak + *reinterpret_cast<const f32x4*>(at);
+        *reinterpret_cast<f32x4*>(at) = s;
+    }
+}
+
+constexpr int kStepsMax = 8;                 // calls of fewer steps walk the recurrence
+
+template <int DT> struct LeakyShape {
+    static constexpr int CH = DT == SS_SEQ_BF16 ? 64 : 32;
+    static LeakyPlan plan(const LeakyArgs& p)
+    {
+        LeakyPlan r;
+        r.ncb = p.DC <= 128 ? 1 : 2;
+        const int chunks = (p.T + CH - 1) / CH;
+        const long long base = (long long)p.B * p.H * r.ncb;
+        // segments: enough workgroups for two on each of 256 CUs, but not under 256 steps, where a segment's state costs as much traffic as its steps
+        long long nseg = (512 + base - 1) / base;
+        const int most = (p.T + 255) / 256;
+        if (nseg > most) nseg = most;
+        if (nseg < 1) nseg = 1;
+        const int per = (int)((chunks + nseg - 1) / nseg);
+        r.seg = per * CH;
+        r.nseg = (chunks + per - 1) / per;
+        r.fold = r.nseg <= 5;
+        return r;
+    }
+    static int da(const LeakyArgs& p) { return p.DA <= 64 ? 64 : p.DA <= 128 ? 128 : 256; }
+    static int dcb(const LeakyArgs& p) { return p.DC <= 64 ? 64 : 128; }
+    static long long ws_floats(const LeakyArgs& p)
+    {
+        if (p.T < kStepsMax) return 0;
+        const LeakyPlan r = plan(p);
+        return (long long)p.B * p.H * r.ncb * (r.nseg - 1) * da(p) * dcb(p);
+    }
+    static int run(const LeakyArgs& p, float* ws, hipStream_t s)
+    {
+        if (p.T < kStepsMax) return p.out_f32 ? steps<DT, SS_SEQ_F32>(p, s) : steps<DT, DT>(p, s);
+        const LeakyPlan r = plan(p);
+        if (r.nseg > 1 && (!ws || !aligned(ws, 16))) return SS_SEQ_EINVAL;
+        auto ok = [&](const void* q, long long t, long long b, long long h) { return aligned(q, 16) && t % 8 == 0 && b % 8 == 0 && h % 8 == 0; };
+        const int vec = p.DA % 8 == 0 && p.DC % 8 == 0 && ok(p.a, p.a_t, p.a_b, p.a_h) && ok(p.b, p.b_t, p.b_b, p.b_h) && ok(p.c, p.c_t, p.c_b, p.c_h);
+        const int vec_out = p.DC % 4 == 0 && p.o_t % 4 == 0 && p.o_b % 4 == 0 && p.o_h % 4 == 0 && aligned(p.out, 16);
+        auto go = [&](auto DAC, auto NTC) {
+            constexpr int DA = DAC.value, NT = NTC.value;
+            const unsigned heads = (unsigned)(p.B * p.H * r.ncb);
+            if (r.nseg > 1) {
+                leaky_chunk_kernel<DT, DA, NT, true><<<heads * (r.nseg - 1), 256, 0, s>>>(p, r, vec, vec_out, ws);
+                if (int rc = launched()) return rc;
+                if (!r.fold) {
+                    leaky_scan_kernel<<<dim3(DA * NT * 64 / 1024, heads), 256, 0, s>>>(ws, p.log_decay, p.H, r.ncb, DA * NT * 64, r.nseg - 1, r.seg);
+                    if (int rc = launched()) return rc;
+                }
+            }
+            leaky_chunk_kernel<DT, DA, NT, false><<<heads * r.nseg, 256, 0, s>>>(p, r, vec, vec_out, ws);
+            return launched();
+        };
+        auto by_dc = [&](auto DAC) { return p.DC <= 64 ? go(DAC, std::integral_constant<int, 1>()) : go(DAC, std::integral_constant<int, 2>()); };
+        return p.DA <= 64 ? by_dc(std::integral_constant<int, 64>()) : p.DA <= 128 ? by_dc(std::integral_constant<int, 128>()) : by_dc(std::integral_constant<int, 256>());
+    }
+};
+
+}  // namespace

@@ -1,0 +1,5 @@
+// ss_seq_attention_f32.hip — leaky attention on fp32 operands (ss_seq_attention.hpp).
+#include "ss_seq_attention.hpp"
+
+long long ss_seq_leaky_ws_f32(const LeakyArgs& p) { return LeakyShape<SS_SEQ_F32>::ws_floats(p); }
+int ss_seq_leaky_f32(const LeakyArgs& p, float* ws, hipStream_t s) { return LeakyShape<SS_SEQ_F32>::run(p, ws, s); }
