@@ -136,7 +136,8 @@ template <int DT, int ODT> int steps(const LeakyArgs& p, hipStream_t s)
 //         + lambda^i a_i W                                 (3)
 //   W    <- lambda^CH W + sum_j lambda^(CH-j) b_j c_j^T    (4)
 //
-// A workgroup owns 64 NT columns of one head's state for one SEGMENT of the steps; wavefront w owns 16 NT of them, with all DA rows of W in its registers.
+// A workgroup of WV (4 or 8) wavefronts owns 16 WV columns of one head's state for one SEGMENT of the steps; a wavefront owns 16 of them, with all DA rows
+// of W in its registers.
 // Products are taken so that accumulators ARE the next product's operand: a 16 x 16 accumulator gives lane l rows 4 (l / 16) .. + 3 of column l % 16; two
 // of them, one above the other, are the 8 contraction values of a 16x16x32 operand in the order {4g .. 4g+3, 16+4g .. 16+4g+3} (four 16x16x4 operands in
 // fp32).  a and b are staged in LDS in that order, so W never leaves the registers; P is shared between the wavefronts through LDS in operand order.
@@ -167,14 +168,14 @@ __device__ __forceinline__ unsigned round_pk(float lo, float hi)
     return __builtin_bit_cast(unsigned, (bf16x2){(__bf16)lo, (__bf16)hi});
 }
 
-template <int DT, int DA, int NT, bool STATE>
-__global__ __launch_bounds__(256, DA <= 128 ? 2 : 1) void leaky_chunk_kernel(const LeakyArgs p, const LeakyPlan plan, const int vec, const int vec_out, float* __restrict__ ws)
+template <int DT, int DA, int WV, bool STATE>
+__global__ __launch_bounds__(64 * WV, STATE ? (DA <= 128 ? 4 : 2) : DT == SS_SEQ_BF16 ? (DA == 64 && WV == 4 ? 3 : 2) : (DA <= 128 ? 4 : 2)) void leaky_chunk_kernel(const LeakyArgs p, const LeakyPlan plan, const int vec, const int vec_out, float* __restrict__ ws)
 {
     constexpr bool BF = DT == SS_SEQ_BF16;
-    constexpr int CH = BF ? 64 : 32, DCB = 64 * NT, IT = CH / 16, KA = DA / 16;
+    constexpr int CH = BF ? 64 : 32, NTH = 64 * WV, DCB = 16 * WV, IT = CH / 16, KA = DA / 16;
     typedef typename std::conditional<BF, unsigned short, float>::type LT;
     constexpr int SA = DA + (BF ? 8 : 4), SC = DCB + (BF ? 8 : 4);       // LDS rows 16 bytes longer than a power of two
-    constexpr int GA = CH * DA / 8 / 256, GC = CH * DCB / 8 / 256;       // 8-element granules per thread
+    constexpr int NA = CH * DA / 8, NC = CH * DCB / 8, GA = (NA + NTH - 1) / NTH, GC = NC / NTH;       // 8-element granules, and those of a thread
     __shared__ __attribute__((aligned(16))) LT sa[STATE ? 8 : CH * SA];
     __shared__ __attribute__((aligned(16))) LT sb[CH * SA];
     __shared__ __attribute__((aligned(16))) LT sc[CH * SC];
@@ -190,46 +191,41 @@ __global__ __launch_bounds__(256, DA <= 128 ? 2 : 1) void leaky_chunk_kernel(con
     const int start = seg * plan.seg, stop = n < start + plan.seg ? n : start + plan.seg;      // this segment's valid steps
     if (STATE && n <= start + plan.seg) return;                          // no later segment reads this one's state
     const float gl = fmaxf(p.log_decay[h], -1e30f) * 1.44269504088896341f;                     // log2 lambda
-    const int c0 = cb * DCB, col0 = c0 + wv * 16 * NT;
+    const int c0 = cb * DCB, col0 = c0 + wv * 16;
     const elem_t<DT>* pa = static_cast<const elem_t<DT>*>(p.a) + b * p.a_b + (h / p.a_group) * p.a_h;
     const elem_t<DT>* pb = static_cast<const elem_t<DT>*>(p.b) + b * p.b_b + (h / p.b_group) * p.b_h;
     const elem_t<DT>* pc = static_cast<const elem_t<DT>*>(p.c) + b * p.c_b + (h / p.c_group) * p.c_h + c0;
     const int dc = p.DC - c0 < DCB ? p.DC - c0 : DCB;
 
     // ---- the state that enters the segment
-    f32x4 W[KA][NT];
+    f32x4 W[KA];
     {
         const long long per = (long long)DA * DCB;
-        const float* mine = ws + ((long long)bh * plan.ncb + cb) * (plan.nseg - 1) * per + (wv * KA * NT) * 256 + lane * 4;
+        const float* mine = ws + ((long long)bh * plan.ncb + cb) * (plan.nseg - 1) * per + wv * KA * 256 + lane * 4;
         if (seg == 0) {
             const float* s_in = p.s_in ? p.s_in + (long long)bh * p.DA * p.DC : nullptr;
             const float first = p.reverse || n == 0 ? 1.f : exp2f(gl);
 #pragma unroll
             for (int kt = 0; kt < KA; ++kt)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const int i = 16 * kt + 4 * g + r, j = col0 + 16 * nt + l16;
-                        W[kt][nt][r] = s_in && i < p.DA && j < p.DC ? s_in[i * p.s_in_row + j * p.s_in_col] * first : 0.f;
+                        const int i = 16 * kt + 4 * g + r, j = col0 + l16;
+                        W[kt][r] = s_in && i < p.DA && j < p.DC ? s_in[i * p.s_in_row + j * p.s_in_col] * first : 0.f;
                     }
         } else if constexpr (STATE) {
 #pragma unroll
             for (int kt = 0; kt < KA; ++kt)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) W[kt][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+W[kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
         } else if (start < n) {
             const int from = plan.fold ? 0 : seg - 1;
             const float leak = exp2f(gl * (float)plan.seg);
 #pragma unroll
             for (int kt = 0; kt < KA; ++kt)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) W[kt][nt] = *reinterpret_cast<const f32x4*>(mine + from * per + (kt * NT + nt) * 256);
+W[kt] = *reinterpret_cast<const f32x4*>(mine + from * per + kt * 256);
             for (int s = from + 1; s < seg; ++s)
 #pragma unroll
                 for (int kt = 0; kt < KA; ++kt)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) W[kt][nt] = W[kt][nt] * leak + *reinterpret_cast<const f32x4*>(mine + s * per + (kt * NT + nt) * 256);
+W[kt] = W[kt] * leak + *reinterpret_cast<const f32x4*>(mine + s * per + kt * 256);
         }
     }
 
@@ -251,13 +247,14 @@ __global__ __launch_bounds__(256, DA <= 128 ? 2 : 1) void leaky_chunk_kernel(con
     auto load = [&](int i0) {
 #pragma unroll
         for (int u = 0; u < GA; ++u) {
-            const int id = tid + 256 * u, row = id / (DA / 8), q = id % (DA / 8);
+            const int id = tid + NTH * u, row = id / (DA / 8), q = id % (DA / 8);
+            if (NA % NTH && id >= NA) break;
             if constexpr (!STATE) fetch(pa, p.a_t, i0 + row, q, p.DA, ra[u]);
             fetch(pb, p.b_t, i0 + row, q, p.DA, rb[u]);
         }
 #pragma unroll
         for (int u = 0; u < GC; ++u) {
-            const int id = tid + 256 * u, row = id / (DCB / 8), q = id % (DCB / 8);
+            const int id = tid + NTH * u, row = id / (DCB / 8), q = id % (DCB / 8);
             fetch(pc, p.c_t, i0 + row, q, dc, rc[u]);
         }
     };
@@ -275,13 +272,14 @@ __global__ __launch_bounds__(256, DA <= 128 ? 2 : 1) void leaky_chunk_kernel(con
     auto stage = [&]() {
 #pragma unroll
         for (int u = 0; u < GA; ++u) {
-            const int id = tid + 256 * u, row = id / (DA / 8), q = id % (DA / 8);
+            const int id = tid + NTH * u, row = id / (DA / 8), q = id % (DA / 8);
+            if (NA % NTH && id >= NA) break;
             if constexpr (!STATE) put(sa, ra[u], row, q);
             put(sb, rb[u], row, q);
         }
 #pragma unroll
         for (int u = 0; u < GC; ++u) {
-            const int id = tid + 256 * u, row = id / (DCB / 8), q = id % (DCB / 8);
+            const int id = tid + NTH * u, row = id / (DCB / 8), q = id % (DCB / 8);
             if constexpr (BF) *reinterpret_cast<G*>(sc + row * SC + 8 * q) = rc[u];
             else {
                 *reinterpret_cast<f32x4*>(sc + row * SC + 8 * q) = (f32x4){widen<DT>(rc[u].v[0]), widen<DT>(rc[u].v[1]), widen<DT>(rc[u].v[2]), widen<DT>(rc[u].v[3])};
@@ -315,7 +313,7 @@ __global__ __launch_bounds__(256, DA <= 128 ? 2 : 1) void leaky_chunk_kernel(con
     };
 
     if constexpr (!STATE && BF) {                                        // the halves of P's operands that lie above the diagonal stay zero
-        for (int i = tid; i < IT * (IT / 2) * 64; i += 256) *reinterpret_cast<f32x4*>(sp + i * 8) = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int i = tid; i < IT * (IT / 2) * 64; i += NTH) *reinterpret_cast<f32x4*>(sp + i * 8) = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
     float row_scale[IT];                                                 // lambda^i o_scale of this lane's steps
     if constexpr (!STATE)
@@ -336,12 +334,12 @@ __global__ __launch_bounds__(256, DA <= 128 ? 2 : 1) void leaky_chunk_kernel(con
         __syncthreads();
         if (i0 + CH < stop) load(i0 + CH);
 
-        f32x4 acc[STATE ? 1 : IT][NT];
+        f32x4 acc[STATE ? 1 : IT];
         if constexpr (!STATE) {
             // (1) the tiles on and below the diagonal, dealt to the wavefronts
 #pragma unroll
-            for (int z = 0; z < (IT * (IT + 1) / 2 + 3) / 4; ++z) {
-                const int idx = wv + 4 * z;
+            for (int z = 0; z < (IT * (IT + 1) / 2 + WV - 1) / WV; ++z) {
+                const int idx = wv + WV * z;
                 if (idx < IT * (IT + 1) / 2) {
                     const int it = idx < 1 ? 0 : idx < 3 ? 1 : idx < 6 ? 2 : 3, jt = idx - it * (it + 1) / 2;
                     f32x4 s = {0.f, 0.f, 0.f, 0.f};
@@ -373,22 +371,19 @@ __global__ __launch_bounds__(256, DA <= 128 ? 2 : 1) void leaky_chunk_kernel(con
             // (3)
 #pragma unroll
             for (int it = 0; it < IT; ++it)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) acc[it][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+acc[it] = (f32x4){0.f, 0.f, 0.f, 0.f};
             if constexpr (BF) {
 #pragma unroll
                 for (int k = 0; k < KA / 2; ++k) {
-                    bf16x8 fw[NT];
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const f32x4 x = W[2 * k][nt], y = W[2 * k + 1][nt];
-                        fw[nt] = mk8(round_pk(x[0], x[1]), round_pk(x[2], x[3]), round_pk(y[0], y[1]), round_pk(y[2], y[3]));
+                    bf16x8 fw;
+{
+                        const f32x4 x = W[2 * k], y = W[2 * k + 1];
+                        fw = mk8(round_pk(x[0], x[1]), round_pk(x[2], x[3]), round_pk(y[0], y[1]), round_pk(y[2], y[3]));
                     }
 #pragma unroll
                     for (int it = 0; it < IT; ++it) {
                         const bf16x8 fa = *reinterpret_cast<const bf16x8*>(sa + (16 * it + l16) * SA + 32 * k + 8 * g);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) acc[it][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[nt], fa, acc[it][nt], 0, 0, 0);
+acc[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw, fa, acc[it], 0, 0, 0);
                     }
                 }
             } else {
@@ -399,37 +394,33 @@ __global__ __launch_bounds__(256, DA <= 128 ? 2 : 1) void leaky_chunk_kernel(con
                         const f32x4 fa = *reinterpret_cast<const f32x4*>(sa + (16 * it + l16) * SA + 16 * k + 4 * g);
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) acc[it][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(W[k][nt][r], fa[r], acc[it][nt], 0, 0, 0);
+acc[it] = __builtin_amdgcn_mfma_f32_16x16x4f32(W[k][r], fa[r], acc[it], 0, 0, 0);
                     }
             }
 #pragma unroll
             for (int it = 0; it < IT; ++it)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) acc[it][nt] *= row_scale[it];
+acc[it] *= row_scale[it];
             __syncthreads();                                             // P is there
         }
         // (2) and (4) share the wavefront's columns of c
         const float keep = exp2f(gl * (float)e);
 #pragma unroll
         for (int kt = 0; kt < KA; ++kt)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) W[kt][nt] *= keep;
+W[kt] *= keep;
         if constexpr (BF) {
 #pragma unroll
             for (int kk = 0; kk < CH / 32; ++kk) {
-                bf16x8 t0[NT], t1[NT], t2[NT];
+                bf16x8 t0, t1, t2;
                 const f32x4 w0 = *reinterpret_cast<const f32x4*>(rw + 32 * kk + 4 * g), w1 = *reinterpret_cast<const f32x4*>(rw + 32 * kk + 16 + 4 * g);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const LT* q = sc + (32 * kk + 4 * g + (l16 >> 2)) * SC + wv * 16 * NT + 16 * nt + 4 * (l16 & 3);
+{
+                    const LT* q = sc + (32 * kk + 4 * g + (l16 >> 2)) * SC + wv * 16 + 4 * (l16 & 3);
                     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)q), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(q + 16 * SC));
                     const s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
                     if constexpr (!STATE) {
                         const bf16x8 fc = __builtin_bit_cast(bf16x8, both);
 #pragma unroll
                         for (int it = 2 * kk; it < IT; ++it)
-                            acc[it][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fc, *reinterpret_cast<const bf16x8*>(sp + ((it * (IT / 2) + kk) * 64 + lane) * 8), acc[it][nt], 0, 0, 0);
+                            acc[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fc, *reinterpret_cast<const bf16x8*>(sp + ((it * (IT / 2) + kk) * 64 + lane) * 8), acc[it], 0, 0, 0);
                     }
                     float x[8], y[8], z[8];
 #pragma unroll
@@ -439,20 +430,19 @@ __global__ __launch_bounds__(256, DA <= 128 ? 2 : 1) void leaky_chunk_kernel(con
                         y[i] = v - x[i];
                         z[i] = y[i] - top16(y[i]);
                     }
-                    t0[nt] = mk8(pack_hi16(x[0], x[1]), pack_hi16(x[2], x[3]), pack_hi16(x[4], x[5]), pack_hi16(x[6], x[7]));
-                    t1[nt] = mk8(pack_hi16(y[0], y[1]), pack_hi16(y[2], y[3]), pack_hi16(y[4], y[5]), pack_hi16(y[6], y[7]));
-                    t2[nt] = mk8(pack_hi16(z[0], z[1]), pack_hi16(z[2], z[3]), pack_hi16(z[4], z[5]), pack_hi16(z[6], z[7]));
+                    t0 = mk8(pack_hi16(x[0], x[1]), pack_hi16(x[2], x[3]), pack_hi16(x[4], x[5]), pack_hi16(x[6], x[7]));
+                    t1 = mk8(pack_hi16(y[0], y[1]), pack_hi16(y[2], y[3]), pack_hi16(y[4], y[5]), pack_hi16(y[6], y[7]));
+                    t2 = mk8(pack_hi16(z[0], z[1]), pack_hi16(z[2], z[3]), pack_hi16(z[4], z[5]), pack_hi16(z[6], z[7]));
                 }
 #pragma unroll
                 for (int kt = 0; kt < KA; ++kt) {
                     const LT* q = sb + (32 * kk + 4 * g + (l16 >> 2)) * SA + 32 * (kt >> 1) + 8 * (l16 & 3) + 4 * (kt & 1);
                     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)q), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(q + 16 * SA));
                     const bf16x8 fb = __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        W[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, t2[nt], W[kt][nt], 0, 0, 0);
-                        W[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, t1[nt], W[kt][nt], 0, 0, 0);
-                        W[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, t0[nt], W[kt][nt], 0, 0, 0);
+{
+                        W[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, t2, W[kt], 0, 0, 0);
+                        W[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, t1, W[kt], 0, 0, 0);
+                        W[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, t0, W[kt], 0, 0, 0);
                     }
                 }
             }
@@ -460,44 +450,323 @@ __global__ __launch_bounds__(256, DA <= 128 ? 2 : 1) void leaky_chunk_kernel(con
 #pragma unroll
             for (int jt = 0; jt < IT; ++jt) {
                 const f32x4 w = *reinterpret_cast<const f32x4*>(rw + 16 * jt + 4 * g);
-                float fc[4][NT];
+                float fc[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) fc[r][nt] = sc[(16 * jt + 4 * g + r) * SC + wv * 16 * NT + 16 * nt + l16];
+fc[r] = sc[(16 * jt + 4 * g + r) * SC + wv * 16 + l16];
                 if constexpr (!STATE)
 #pragma unroll
                     for (int it = jt; it < IT; ++it) {
                         const f32x4 fp = *reinterpret_cast<const f32x4*>(sp + ((it * IT + jt) * 64 + lane) * 4);
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) acc[it][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(fc[r][nt], fp[r], acc[it][nt], 0, 0, 0);
+acc[it] = __builtin_amdgcn_mfma_f32_16x16x4f32(fc[r], fp[r], acc[it], 0, 0, 0);
                     }
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) fc[r][nt] *= w[r];
+fc[r] *= w[r];
 #pragma unroll
                 for (int kt = 0; kt < KA; ++kt)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const float fb = sb[(16 * jt + 4 * g + r) * SA + 16 * kt + l16];
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) W[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb, fc[r][nt], W[kt][nt], 0, 0, 0);
+W[kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb, fc[r], W[kt], 0, 0, 0);
                     }
             }
         }
         if constexpr (!STATE)
 #pragma unroll
             for (int it = 0; it < IT; ++it)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) store(i0 + 16 * it + l16, col0 + 16 * nt + 4 * g, acc[it][nt]);
+store(i0 + 16 * it + l16, col0 + 4 * g, acc[it]);
     }
 
     if constexpr (STATE) {
         const long long per = (long long)DA * DCB;
-        float* mine = ws + (((long long)bh * plan.ncb + cb) * (plan.nseg - 1) + seg) * per + (wv * KA * NT) * 256 + lane * 4;
+        float* mine = ws + (((long long)bh * plan.ncb + cb) * (plan.nseg - 1) + seg) * per + wv * KA * 256 + lane * 4;
+#pragma unroll
+        for (int kt = 0; kt < KA; ++kt)
+*reinterpret_cast<f32x4*>(mine + kt * 256) = W[kt];
+    } else {
+        // steps of the segment behind the stream's last: zeros (the loop above has written its own chunks to their end)
+        const int end = start + plan.seg < p.T ? start + plan.seg : p.T;
+        for (; i0 < end; i0 += CH)
+#pragma unroll
+            for (int it = 0; it < IT; ++it)
+store(i0 + 16 * it + l16, col0 + 4 * g, (f32x4){0.f, 0.f, 0.f, 0.f});
+        if (p.s_out && ((start < n && n <= start + plan.seg) || (n == 0 && seg == 0))) {
+            float* s_out = p.s_out + (long long)bh * p.DA * p.DC;
+#pragma unroll
+            for (int kt = 0; kt < KA; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int i = 16 * kt + 4 * g + r, j = col0 + l16;
+                        if (i < p.DA && j < p.DC) s_out[i * p.s_out_row + j * p.s_out_col] = W[kt][r];
+                    }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------------------------------
+// The tile form on 16-bit operands: chunks of 32 steps, a workgroup of four wavefronts owns 64 NT columns, a wavefront 16 NT of them (W: DA x 16 NT in its
+// registers).  a, b, c of the next chunk are on their way to registers while this one is computed, then go to the other of two LDS buffers: one barrier for
+// the buffers and one for P per chunk, two workgroups on a CU.
+// Rows are unpadded; the 16-byte granule q of row r lies in slot q ^ f(r), f chosen so that the three ways they are read (a granule of 16 rows, half granules
+// of 16 rows, and the transposing 4 x 16 read) meet no bank twice.
+// ---------------------------------------------------------------------------------------------------------------------------------------------------------
+template <int SPR> __device__ __forceinline__ int swz(int row) { return SPR >= 16 ? ((row & 7) << 1) | ((row >> 3) & 1) : (((row >> 1) & 3) << 1) | ((row >> 3) & 1); }
+// this wavefront's LDS operations are done, then the barrier: unlike __syncthreads() it does not wait for loads on their way to LDS or for stores
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+template <int DT, int DA, int NT, bool STATE, bool VEC>
+__global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel(const LeakyArgs p, const LeakyPlan plan, float* __restrict__ ws)
+{
+    constexpr int CH = 32, DCB = 64 * NT, KA = DA / 16, SA = DA / 8, SC = DCB / 8;          // SA, SC: granules of a row
+    constexpr int BA = CH * DA, BC = CH * DCB, BUF = (STATE ? 1 : 2) * BA + BC;              // elements of a buffer: [a] b c
+    __shared__ __attribute__((aligned(1024))) unsigned short lds[2 * BUF];
+    __shared__ __attribute__((aligned(16))) unsigned short sp[STATE ? 8 : 2 * 64 * 8];       // P in operand order, by tile of 16 steps
+    __shared__ __attribute__((aligned(16))) float rw[CH];                                    // lambda^(e - j) b_scale of the chunk's steps
+
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g = lane >> 4;
+    const int cb = blockIdx.x % plan.ncb, rest = blockIdx.x / plan.ncb;
+    const int nst = STATE ? plan.nseg - 1 : plan.nseg, seg = rest % nst, bh = rest / nst, b = bh / p.H, h = bh - b * p.H;
+    int n = p.T;
+    if (p.lengths) { n = p.lengths[b]; n = n < 0 ? 0 : n > p.T ? p.T : n; }
+    const int start = seg * plan.seg, stop = n < start + plan.seg ? n : start + plan.seg;    // this segment's valid steps
+    if (STATE && n <= start + plan.seg) return;                          // no later segment reads this one's state
+    const float gl = fmaxf(p.log_decay[h], -1e30f) * 1.44269504088896341f;                   // log2 lambda
+    const int c0 = cb * DCB, col0 = c0 + wv * 16 * NT;
+    const unsigned short* pa = static_cast<const unsigned short*>(p.a) + b * p.a_b + (h / p.a_group) * p.a_h;
+    const unsigned short* pb = static_cast<const unsigned short*>(p.b) + b * p.b_b + (h / p.b_group) * p.b_h;
+    const unsigned short* pc = static_cast<const unsigned short*>(p.c) + b * p.c_b + (h / p.c_group) * p.c_h + c0;
+    const int dc = p.DC - c0 < DCB ? p.DC - c0 : DCB;
+
+    // ---- the state that enters the segment
+    f32x4 W[KA][NT];
+    {
+        const long long per = (long long)DA * DCB;
+        const float* mine = ws + ((long long)bh * plan.ncb + cb) * (plan.nseg - 1) * per + wv * KA * NT * 256 + lane * 4;
+#pragma unroll
+        for (int kt = 0; kt < KA; ++kt)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) W[kt][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        if (seg == 0) {
+            if (p.s_in) {
+                const float* s_in = p.s_in + (long long)bh * p.DA * p.DC;
+                const float first = p.reverse || n == 0 ? 1.f : exp2f(gl);
+#pragma unroll
+                for (int kt = 0; kt < KA; ++kt)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int i = 16 * kt + 4 * g + r, j = col0 + 16 * nt + l16;
+                            const bool in = i < p.DA && j < p.DC;
+                            const float v = s_in[in ? i * p.s_in_row + j * p.s_in_col : 0];
+                            W[kt][nt][r] = in ? v * first : 0.f;
+                        }
+            }
+        } else if (!STATE && start < n) {
+            const float leak = exp2f(gl * (float)plan.seg);
+            for (int s = plan.fold ? 0 : seg - 1; s < seg; ++s)
+#pragma unroll
+                for (int kt = 0; kt < KA; ++kt)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) W[kt][nt] = W[kt][nt] * leak + *reinterpret_cast<const f32x4*>(mine + s * per + (kt * NT + nt) * 256);
+        }
+    }
+
+    // ---- staging: 16-byte granules of [CH][D] rows, global -> registers -> LDS
+    constexpr int GA = CH * SA / 256, GC = CH * SC / 256;
+    u16x8 ra[STATE ? 1 : GA], rb[GA], rc[GC];
+    auto fetch = [&](u16x8* dst, const unsigned short* base, long long st, int i0, int d, auto SPRC) {
+        constexpr int SPR = SPRC.value;
+#pragma unroll
+        for (int u = 0; u < CH * SPR / 256; ++u) {
+            const int x = tid + 256 * u, row = x / SPR, q = x % SPR, i = i0 + row;
+            const unsigned short* src = base + (long long)(p.reverse ? n - 1 - i : i) * st + 8 * q;
+            if (VEC && i0 + CH <= stop && d == 8 * SPR) dst[u] = *reinterpret_cast<const u16x8*>(src);       // nothing to leave out: no branch per granule
+            else {
+                dst[u] = (u16x8){0, 0, 0, 0, 0, 0, 0, 0};
+                if (i < stop && 8 * q < d) {
+                    if constexpr (VEC) dst[u] = *reinterpret_cast<const u16x8*>(src);
+                    else                                                 // rows that are not whole aligned granules
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) if (8 * q + e < d) dst[u][e] = src[e];
+                }
+            }
+        }
+    };
+    auto put = [&](unsigned short* dst, const u16x8* v, auto SPRC) {
+        constexpr int SPR = SPRC.value;
+#pragma unroll
+        for (int u = 0; u < CH * SPR / 256; ++u) {
+            const int x = tid + 256 * u, row = x / SPR, q = x % SPR;
+            *reinterpret_cast<u16x8*>(dst + (row * SPR + (q ^ swz<SPR>(row))) * 8) = v[u];
+        }
+    };
+    auto load = [&](int i0) {
+        if constexpr (!STATE) fetch(ra, pa, p.a_t, i0, p.DA, std::integral_constant<int, SA>());
+        fetch(rb, pb, p.b_t, i0, p.DA, std::integral_constant<int, SA>());
+        fetch(rc, pc, p.c_t, i0, dc, std::integral_constant<int, SC>());
+    };
+    auto stage = [&](int buf) {
+        unsigned short* at = lds + buf * BUF;
+        if constexpr (!STATE) { put(at, ra, std::integral_constant<int, SA>()); at += BA; }
+        put(at, rb, std::integral_constant<int, SA>());
+        put(at + BA, rc, std::integral_constant<int, SC>());
+    };
+    auto store = [&](int i, int col, const f32x4& v) {                   // four columns of step i
+        if (i >= p.T) return;
+        const bool live = i < n;
+        const long long t = live && p.reverse ? n - 1 - i : i;
+        const long long at = b * p.o_b + h * p.o_h + t * p.o_t + col;
+        const f32x4 o = live ? v : (f32x4){0.f, 0.f, 0.f, 0.f};
+        if (p.out_f32) {
+            float* q = static_cast<float*>(p.out) + at;
+            if constexpr (VEC) { if (col < p.DC) *reinterpret_cast<f32x4*>(q) = o; }
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e) if (col + e < p.DC) q[e] = o[e];
+        } else {
+            unsigned short* q = static_cast<unsigned short*>(p.out) + at;
+            if constexpr (VEC) {
+                if (col < p.DC) *reinterpret_cast<u16x4*>(q) = (u16x4){narrow<DT>(o[0]), narrow<DT>(o[1]), narrow<DT>(o[2]), narrow<DT>(o[3])};
+            } else
+#pragma unroll
+                for (int e = 0; e < 4; ++e) if (col + e < p.DC) q[e] = narrow<DT>(o[e]);
+        }
+    };
+
+    if constexpr (!STATE) { if (tid < 128) *reinterpret_cast<f32x4*>(sp + tid * 8) = (f32x4){0.f, 0.f, 0.f, 0.f}; }      // the half of P above the diagonal stays zero
+    if (tid < CH) rw[tid] = exp2f(gl * (float)(CH - tid)) * p.b_scale;
+    float row_scale[2];                                                  // lambda^i o_scale of this lane's steps
+#pragma unroll
+    for (int it = 0; it < 2; ++it) row_scale[it] = exp2f(gl * (float)(16 * it + l16)) * p.o_scale;
+    // byte offsets of this lane's operands in a buffer; 32 (64) bytes of the row further on is an XOR of the slot
+    const int fa = swz<SA>(l16), o1 = l16 * DA * 2 + ((g ^ fa) << 4), o3 = l16 * DA * 2 + (((g >> 1) ^ fa) << 4) + ((g & 1) << 3);
+    const int tr = 4 * g + (l16 >> 2), y = (l16 & 3) >> 1;
+    const int o4 = tr * DA * 2 + ((y ^ swz<SA>(tr)) << 4) + ((l16 & 1) << 3), oc = tr * DCB * 2 + (((2 * NT * wv + y) ^ swz<SC>(tr)) << 4) + ((l16 & 1) << 3);
+
+    int i0 = start, buf = 0;
+    if (start < stop) {
+        load(start);
+        stage(0);
+    }
+    for (; i0 < stop; i0 += CH, buf ^= 1) {
+        const int cnt = stop - i0 < CH ? stop - i0 : CH;
+        // the last chunk of the stream leaves the state as it is after its last step (forward) or leaked once more (reverse)
+        const int e = i0 + cnt == n && !p.reverse ? cnt - 1 : cnt;
+        lds_barrier();                                                   // this chunk is there, and the other buffer has been read
+        if (i0 + CH < stop) load(i0 + CH);
+        const char* la = reinterpret_cast<const char*>(lds + buf * BUF);
+        const char* lb = la + (STATE ? 0 : BA * 2);
+        const char* lc = lb + BA * 2;
+        if (e != CH && tid < CH) rw[tid] = exp2f(gl * (float)(e > tid ? e - tid : 0)) * p.b_scale;
+        f32x4 acc[2][NT];
+        if constexpr (!STATE) {
+            // (1) wavefronts 0 .. 2: the tiles (0, 0), (1, 0), (1, 1)
+            if (wv < 3) {
+                const int it = (wv + 1) >> 1, jt = wv >> 1;
+                f32x4 s = {0.f, 0.f, 0.f, 0.f}, s2 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < DA / 32; ++k) {
+                    const bf16x8 xa = *reinterpret_cast<const bf16x8*>(la + it * 16 * DA * 2 + (o1 ^ (64 * k)));
+                    const bf16x8 xb = *reinterpret_cast<const bf16x8*>(lb + jt * 16 * DA * 2 + (o1 ^ (64 * k)));
+                    if (k & 1) s2 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb, xa, s2, 0, 0, 0);
+                    else s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb, xa, s, 0, 0, 0);
+                }
+                s += s2;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int d = 16 * (it - jt) + l16 - 4 * g - r;      // i - j
+                    s[r] = d < 0 ? 0.f : s[r] * (exp2f(gl * (float)d) * p.b_scale * p.o_scale);
+                }
+                typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+                *reinterpret_cast<u32x2*>(sp + (it * 64 + lane) * 8 + jt * 4) = (u32x2){round_pk(s[0], s[1]), round_pk(s[2], s[3])};
+            }
+            // (3)
+#pragma unroll
+            for (int it = 0; it < 2; ++it)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) acc[it][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < KA / 2; ++k) {
+                bf16x8 xa[2];
+#pragma unroll
+                for (int it = 0; it < 2; ++it) {
+                    const char* q = la + it * 16 * DA * 2 + (o3 ^ (64 * k));
+                    const char* q2 = la + it * 16 * DA * 2 + (o3 ^ (64 * k + 32));
+                    xa[it] = __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(*reinterpret_cast<const s16x4*>(q), *reinterpret_cast<const s16x4*>(q2), 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const f32x4 x = W[2 * k][nt], z = W[2 * k + 1][nt];
+                    const bf16x8 fw = mk8(round_pk(x[0], x[1]), round_pk(x[2], x[3]), round_pk(z[0], z[1]), round_pk(z[2], z[3]));
+#pragma unroll
+                    for (int it = 0; it < 2; ++it) acc[it][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw, xa[it], acc[it][nt], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int it = 0; it < 2; ++it)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) acc[it][nt] *= row_scale[it];
+            lds_barrier();                                               // P is there
+        }
+        // (2) and (4) share the wavefront's columns of c
+        bf16x8 t0[NT], t1[NT], t2[NT];
+        {
+            const f32x4 w0 = *reinterpret_cast<const f32x4*>(rw + 4 * g), w1 = *reinterpret_cast<const f32x4*>(rw + 16 + 4 * g);
+            bf16x8 fp[2];
+            if constexpr (!STATE) {
+#pragma unroll
+                for (int it = 0; it < 2; ++it) fp[it] = *reinterpret_cast<const bf16x8*>(sp + (it * 64 + lane) * 8);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const char* q = lc + (oc ^ (32 * nt));
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)q), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(q + 16 * DCB * 2));
+                const s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                if constexpr (!STATE) {
+#pragma unroll
+                    for (int it = 0; it < 2; ++it) acc[it][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, both), fp[it], acc[it][nt], 0, 0, 0);
+                }
+                float x[8], z[8], u[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float v = __uint_as_float((unsigned)(unsigned short)both[i] << 16) * (i < 4 ? w0[i & 3] : w1[i & 3]);
+                    x[i] = top16(v);
+                    z[i] = v - x[i];
+                    u[i] = z[i] - top16(z[i]);
+                }
+                t0[nt] = mk8(pack_hi16(x[0], x[1]), pack_hi16(x[2], x[3]), pack_hi16(x[4], x[5]), pack_hi16(x[6], x[7]));
+                t1[nt] = mk8(pack_hi16(z[0], z[1]), pack_hi16(z[2], z[3]), pack_hi16(z[4], z[5]), pack_hi16(z[6], z[7]));
+                t2[nt] = mk8(pack_hi16(u[0], u[1]), pack_hi16(u[2], u[3]), pack_hi16(u[4], u[5]), pack_hi16(u[6], u[7]));
+            }
+        }
+        if constexpr (!STATE)
+#pragma unroll
+            for (int it = 0; it < 2; ++it)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) store(i0 + 16 * it + l16, col0 + 16 * nt + 4 * g, acc[it][nt]);
+        const float keep = exp2f(gl * (float)e);
+#pragma unroll
+        for (int kt = 0; kt < KA; ++kt) {
+            const char* q = lb + (o4 ^ (32 * kt));
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)q), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(q + 16 * DA * 2));
+            const bf16x8 fb = __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) W[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, t2[nt], W[kt][nt] * keep, 0, 0, 0);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) W[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, t1[nt], W[kt][nt], 0, 0, 0);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) W[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, t0[nt], W[kt][nt], 0, 0, 0);
+        }
+        if (i0 + CH < stop) stage(buf ^ 1);
+    }
+
+    if constexpr (STATE) {
+        const long long per = (long long)DA * DCB;
+        float* mine = ws + (((long long)bh * plan.ncb + cb) * (plan.nseg - 1) + seg) * per + wv * KA * NT * 256 + lane * 4;
 #pragma unroll
         for (int kt = 0; kt < KA; ++kt)
 #pragma unroll
@@ -507,7 +776,7 @@ __global__ __launch_bounds__(256, DA <= 128 ? 2 : 1) void leaky_chunk_kernel(con
         const int end = start + plan.seg < p.T ? start + plan.seg : p.T;
         for (; i0 < end; i0 += CH)
 #pragma unroll
-            for (int it = 0; it < IT; ++it)
+            for (int it = 0; it < 2; ++it)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) store(i0 + 16 * it + l16, col0 + 16 * nt + 4 * g, (f32x4){0.f, 0.f, 0.f, 0.f});
         if (p.s_out && ((start < n && n <= start + plan.seg) || (n == 0 && seg == 0))) {
@@ -539,10 +808,14 @@ __global__ __launch_bounds__(256) void leaky_scan_kernel(float* __restrict__ ws,
     }
 }
 
+#ifndef LEAKY_TARGET
+#define LEAKY_TARGET 768
+#endif
+constexpr int kLeakyTarget = LEAKY_TARGET;
 constexpr int kStepsMax = 8;                 // calls of fewer steps walk the recurrence
 
 template <int DT> struct LeakyShape {
-    static constexpr int CH = DT == SS_SEQ_BF16 ? 64 : 32;
+    static constexpr int CH = 32;
     static LeakyPlan plan(const LeakyArgs& p)
     {
         LeakyPlan r;
@@ -550,7 +823,7 @@ template <int DT> struct LeakyShape {
         const int chunks = (p.T + CH - 1) / CH;
         const long long base = (long long)p.B * p.H * r.ncb;
         // segments: enough workgroups for two on each of 256 CUs, but not under 256 steps, where a segment's state costs as much traffic as its steps
-        long long nseg = (512 + base - 1) / base;
+        long long nseg = (kLeakyTarget + base - 1) / base;
         const int most = (p.T + 255) / 256;
         if (nseg > most) nseg = most;
         if (nseg < 1) nseg = 1;
@@ -568,6 +841,11 @@ template <int DT> struct LeakyShape {
         const LeakyPlan r = plan(p);
         return (long long)p.B * p.H * r.ncb * (r.nseg - 1) * da(p) * dcb(p);
     }
+    template <int DA, int NT, bool STATE> static void tile(unsigned grid, const LeakyArgs& p, const LeakyPlan& r, bool vec, float* ws, hipStream_t s)
+    {
+        if (vec) leaky_tile_kernel<DT, DA, NT, STATE, true><<<grid, 256, 0, s>>>(p, r, ws);
+        else leaky_tile_kernel<DT, DA, NT, STATE, false><<<grid, 256, 0, s>>>(p, r, ws);
+    }
     static int run(const LeakyArgs& p, float* ws, hipStream_t s)
     {
         if (p.T < kStepsMax) return p.out_f32 ? steps<DT, SS_SEQ_F32>(p, s) : steps<DT, DT>(p, s);
@@ -576,21 +854,23 @@ template <int DT> struct LeakyShape {
         auto ok = [&](const void* q, long long t, long long b, long long h) { return aligned(q, 16) && t % 8 == 0 && b % 8 == 0 && h % 8 == 0; };
         const int vec = p.DA % 8 == 0 && p.DC % 8 == 0 && ok(p.a, p.a_t, p.a_b, p.a_h) && ok(p.b, p.b_t, p.b_b, p.b_h) && ok(p.c, p.c_t, p.c_b, p.c_h);
         const int vec_out = p.DC % 4 == 0 && p.o_t % 4 == 0 && p.o_b % 4 == 0 && p.o_h % 4 == 0 && aligned(p.out, 16);
-        auto go = [&](auto DAC, auto NTC) {
-            constexpr int DA = DAC.value, NT = NTC.value;
+        auto go = [&](auto DAC, auto WVC) {
+            constexpr int DA = DAC.value, WV = WVC.value;
             const unsigned heads = (unsigned)(p.B * p.H * r.ncb);
             if (r.nseg > 1) {
-                leaky_chunk_kernel<DT, DA, NT, true><<<heads * (r.nseg - 1), 256, 0, s>>>(p, r, vec, vec_out, ws);
+                if constexpr (DT == SS_SEQ_BF16) tile<DA, WV / 4, true>(heads * (r.nseg - 1), p, r, vec && vec_out, ws, s);
+                else leaky_chunk_kernel<DT, DA, WV, true><<<heads * (r.nseg - 1), 64 * WV, 0, s>>>(p, r, vec, vec_out, ws);
                 if (int rc = launched()) return rc;
                 if (!r.fold) {
-                    leaky_scan_kernel<<<dim3(DA * NT * 64 / 1024, heads), 256, 0, s>>>(ws, p.log_decay, p.H, r.ncb, DA * NT * 64, r.nseg - 1, r.seg);
+                    leaky_scan_kernel<<<dim3(DA * WV * 16 / 1024, heads), 256, 0, s>>>(ws, p.log_decay, p.H, r.ncb, DA * WV * 16, r.nseg - 1, r.seg);
                     if (int rc = launched()) return rc;
                 }
             }
-            leaky_chunk_kernel<DT, DA, NT, false><<<heads * r.nseg, 256, 0, s>>>(p, r, vec, vec_out, ws);
+            if constexpr (DT == SS_SEQ_BF16) tile<DA, WV / 4, false>(heads * r.nseg, p, r, vec && vec_out, ws, s);
+            else leaky_chunk_kernel<DT, DA, WV, false><<<heads * r.nseg, 64 * WV, 0, s>>>(p, r, vec, vec_out, ws);
             return launched();
         };
-        auto by_dc = [&](auto DAC) { return p.DC <= 64 ? go(DAC, std::integral_constant<int, 1>()) : go(DAC, std::integral_constant<int, 2>()); };
+        auto by_dc = [&](auto DAC) { return p.DC <= 64 ? go(DAC, std::integral_constant<int, 4>()) : go(DAC, std::integral_constant<int, 8>()); };
         return p.DA <= 64 ? by_dc(std::integral_constant<int, 64>()) : p.DA <= 128 ? by_dc(std::integral_constant<int, 128>()) : by_dc(std::integral_constant<int, 256>());
     }
 };
