@@ -7,7 +7,7 @@ import os
 
 import torch  # before the CDLL, so that one HIP runtime is shared
 
-from ._lib import SSNeuronError, _check, _stream
+from ._lib import SSNeuronError, _check
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, 'lib', 'libss_sequence.so')
@@ -64,67 +64,85 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+_device = getattr(torch._C, '_cuda_getDevice', None)
+
+
+def _call(name, dev, *args):
+    """One entry point on torch's current stream of `dev`, with that device current.  A context manager per launch costs as much as the launch, so it is
+    entered only for another device than the current one."""
+    f = getattr(_lib or lib(), name)
+    if _device is not None and _device() == dev.index:
+        rc = f(*args, _raw_stream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = f(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        _check(rc, name)
+
+
 def leaky(a, b, c, out, log_decay, b_scale, o_scale, reverse=False, lengths=None, s_in=None, s_in_t=False, s_out=None, s_out_t=False):
-    """One leaky map (struct ss_seq_leaky_desc): a, b, c, out [T, B, heads, D] views with a contiguous last axis; states [B, H, rows, columns] contiguous, or
-    transposed (`*_t`: the matrix is stored [DC, DA])."""
-    T, B, H, DC = out.shape
-    DA = a.shape[3]
-    d = LeakyDesc(size=C.sizeof(LeakyDesc), dtype=DT_CODE[a.dtype], out_dtype=DT_CODE[out.dtype], T=T, B=B, H=H, DA=DA, DC=DC, reverse=int(reverse),
-                  b_scale=b_scale, o_scale=o_scale, a=a.data_ptr(), b=b.data_ptr(), c=c.data_ptr(), out=out.data_ptr(),
-                  a_group=H // a.shape[2], b_group=H // b.shape[2], c_group=H // c.shape[2], log_decay=log_decay.data_ptr(), lengths=_p(lengths),
-                  s_in=_p(s_in), s_out=_p(s_out), s_in_row=1 if s_in_t else DC, s_in_col=DA if s_in_t else 1, s_out_row=1 if s_out_t else DC,
-                  s_out_col=DA if s_out_t else 1)
-    d.a_t, d.a_b, d.a_h = a.stride()[:3]
-    d.b_t, d.b_b, d.b_h = b.stride()[:3]
-    d.c_t, d.c_b, d.c_h = c.stride()[:3]
-    d.o_t, d.o_b, d.o_h = out.stride()[:3]
-    with torch.cuda.device(a.device):
-        n = lib().ss_seq_leaky_ws_floats(C.byref(d))
-        ws = torch.empty(n, dtype=torch.float32, device=a.device) if n else None
-        d.ws = _p(ws)
-        _check(lib().ss_seq_leaky(C.byref(d), _stream(a)), 'ss_seq_leaky')
+    """One leaky map (struct ss_seq_leaky_desc): a, b, c, out [T, B, heads, D] views with a contiguous last axis ([B, heads, D]: one step); states
+    [B, H, rows, columns] contiguous, or transposed (`*_t`: the matrix is stored [DC, DA])."""
+    sa, sb, sc, so = a.stride(), b.stride(), c.stride(), out.stride()
+    if len(so) == 3:
+        T, (B, H, DC) = 1, out.shape
+        sa, sb, sc, so = (0, *sa), (0, *sb), (0, *sc), (0, *so)
+    else:
+        T, B, H, DC = out.shape
+    DA = a.shape[-1]
+    dt = DT_CODE[a.dtype]
+    d = LeakyDesc(_DESC_SIZE, dt, DT_CODE[out.dtype], T, B, H, DA, DC, reverse, b_scale, o_scale, a.data_ptr(), b.data_ptr(), c.data_ptr(), out.data_ptr(),
+                  sa[0], sa[1], sa[2], sb[0], sb[1], sb[2], sc[0], sc[1], sc[2], so[0], so[1], so[2], H // a.shape[-2], H // b.shape[-2], H // c.shape[-2],
+                  log_decay.data_ptr(), _p(lengths), _p(s_in), _p(s_out), 1 if s_in_t else DC, DA if s_in_t else 1, 1 if s_out_t else DC, DA if s_out_t else 1)
+    ref = C.byref(d)
+    if T > 1:
+        n = (_lib or lib()).ss_seq_leaky_ws_floats(ref)
+        if n:
+            ws = torch.empty(n, dtype=torch.float32, device=a.device)
+            d.ws = ws.data_ptr()
+    _call('ss_seq_leaky', a.device, ref)
+
+
+_DESC_SIZE = C.sizeof(LeakyDesc)
 
 
 def group_sum(x, out, group):
     """x fp32 [rows * group, D] contiguous -> out [rows, D]: sums of `group` consecutive rows."""
     D = x.shape[-1]
-    with torch.cuda.device(x.device):
-        _check(lib().ss_seq_group_sum(x.data_ptr(), out.data_ptr(), out.numel() // D, group, D, DT_CODE[out.dtype], _stream(x)), 'ss_seq_group_sum')
+    _call('ss_seq_group_sum', x.device, x.data_ptr(), out.data_ptr(), out.numel() // D, group, D, DT_CODE[out.dtype])
 
 
 def rms_norm_fwd(x, residual, weight, y, total, rstd, eps):
     """x, residual: [rows, C] with a contiguous last axis; y, total contiguous; rstd fp32 [rows] or None."""
-    with torch.cuda.device(x.device):
-        _check(lib().ss_seq_rms_norm_fwd(x.data_ptr(), x.stride(0), _p(residual), 0 if residual is None else residual.stride(0), weight.data_ptr(), y.data_ptr(),
-                                         _p(total), _p(rstd), x.shape[0], x.shape[1], eps, DT_CODE[x.dtype], _stream(x)), 'ss_seq_rms_norm_fwd')
+    rows, C_ = x.shape
+    _call('ss_seq_rms_norm_fwd', x.device, x.data_ptr(), x.stride(0), _p(residual), 0 if residual is None else residual.stride(0), weight.data_ptr(), y.data_ptr(),
+          _p(total), _p(rstd), rows, C_, eps, DT_CODE[x.dtype])
 
 
 def rms_norm_bwd(g_y, g_sum, h, weight, rstd, g_h, g_w):
     rows, C_ = h.shape
-    with torch.cuda.device(h.device):
-        ws = None if g_w is None else torch.empty(lib().ss_seq_rms_norm_ws_floats(rows, C_, DT_CODE[h.dtype]), dtype=torch.float32, device=h.device)
-        _check(lib().ss_seq_rms_norm_bwd(_p(g_y), _p(g_sum), h.data_ptr(), weight.data_ptr(), rstd.data_ptr(), g_h.data_ptr(), _p(g_w), _p(ws), rows, C_,
-                                         DT_CODE[h.dtype], _stream(h)), 'ss_seq_rms_norm_bwd')
+    dt = DT_CODE[h.dtype]
+    ws = None if g_w is None else torch.empty((_lib or lib()).ss_seq_rms_norm_ws_floats(rows, C_, dt), dtype=torch.float32, device=h.device)
+    _call('ss_seq_rms_norm_bwd', h.device, _p(g_y), _p(g_sum), h.data_ptr(), weight.data_ptr(), rstd.data_ptr(), g_h.data_ptr(), _p(g_w), _p(ws), rows, C_, dt)
 
 
 def rms_norm_int8(x, residual, weight, codes, scales, total, eps):
-    with torch.cuda.device(x.device):
-        _check(lib().ss_seq_rms_norm_int8(x.data_ptr(), x.stride(0), _p(residual), 0 if residual is None else residual.stride(0), weight.data_ptr(),
-                                          codes.data_ptr(), scales.data_ptr(), _p(total), x.shape[0], x.shape[1], eps, DT_CODE[x.dtype], _stream(x)),
-               'ss_seq_rms_norm_int8')
+    rows, C_ = x.shape
+    _call('ss_seq_rms_norm_int8', x.device, x.data_ptr(), x.stride(0), _p(residual), 0 if residual is None else residual.stride(0), weight.data_ptr(),
+          codes.data_ptr(), scales.data_ptr(), _p(total), rows, C_, eps, DT_CODE[x.dtype])
 
 
 def dequant_int8(codes, scales, out):
-    with torch.cuda.device(codes.device):
-        _check(lib().ss_seq_dequant_int8(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), codes.shape[0], codes.shape[1], DT_CODE[out.dtype], _stream(codes)),
-               'ss_seq_dequant_int8')
+    """codes, out contiguous, rows of the last axis; a scale for each row."""
+    C_ = codes.shape[-1]
+    _call('ss_seq_dequant_int8', codes.device, codes.data_ptr(), scales.data_ptr(), out.data_ptr(), codes.numel() // C_, C_, DT_CODE[out.dtype])
 
 
 def int8_linear(a, a_scale, w, w_scale, bias, out):
     """a [M, K], w [N, K] int8 with contiguous last axes; out [M, N] contiguous."""
     (M, K), N = a.shape, w.shape[0]
-    with torch.cuda.device(a.device):
-        n = lib().ss_seq_int8_linear_ws_ints(M, N, K)
-        ws = torch.empty(n, dtype=torch.int32, device=a.device) if n else None
-        _check(lib().ss_seq_int8_linear(a.data_ptr(), a.stride(0), a_scale.data_ptr(), w.data_ptr(), w.stride(0), w_scale.data_ptr(), _p(bias), out.data_ptr(),
-                                        M, N, K, DT_CODE[out.dtype], _p(ws), _stream(a)), 'ss_seq_int8_linear')
+    n = (_lib or lib()).ss_seq_int8_linear_ws_ints(M, N, K)
+    ws = torch.empty(n, dtype=torch.int32, device=a.device) if n else None
+    _call('ss_seq_int8_linear', a.device, a.data_ptr(), a.stride(0), a_scale.data_ptr(), w.data_ptr(), w.stride(0), w_scale.data_ptr(), _p(bias), out.data_ptr(),
+          M, N, K, DT_CODE[out.dtype], _p(ws))

@@ -55,12 +55,15 @@ template <int DT, int ODT, int R, bool V4> __global__ __launch_bounds__(256) voi
     for (int r = 0; r < R; ++r) {
         S[r] = (f32x4){0.f, 0.f, 0.f, 0.f};
         const int i = g + 16 * r;
-        if (s_in && i < p.DA) {
-            if constexpr (V4) { if (j0 < p.DC) S[r] = *reinterpret_cast<const f32x4*>(s_in + i * p.s_in_row + j0); }
-            else
+        if (!s_in) continue;
+        if constexpr (V4) { if (i < p.DA && j0 < p.DC) S[r] = *reinterpret_cast<const f32x4*>(s_in + i * p.s_in_row + j0); }
+        else
 #pragma unroll
-                for (int e = 0; e < 4; ++e) if (j0 + e < p.DC) S[r][e] = s_in[i * p.s_in_row + (j0 + e) * p.s_in_col];
-        }
+            for (int e = 0; e < 4; ++e) {                  // (a select, not a branch, for each element)
+                const bool in = i < p.DA && j0 + e < p.DC;
+                const float v = s_in[in ? i * p.s_in_row + (j0 + e) * p.s_in_col : 0];
+                S[r][e] = in ? v : 0.f;
+            }
     }
     for (int i = 0; i < n; ++i) {
         const long long t = p.reverse ? n - 1 - i : i;
@@ -808,10 +811,7 @@ __global__ __launch_bounds__(256) void leaky_scan_kernel(float* __restrict__ ws,
     }
 }
 
-#ifndef LEAKY_TARGET
-#define LEAKY_TARGET 768
-#endif
-constexpr int kLeakyTarget = LEAKY_TARGET;
+constexpr int kLeakyTarget = 512;            // workgroups wanted: two on each of 256 CUs (prompt of 4096 steps, 64 heads: 256 129 us, 384 122, 512 108, 768 122, 1024 140)
 constexpr int kStepsMax = 8;                 // calls of fewer steps walk the recurrence
 
 template <int DT> struct LeakyShape {
@@ -822,7 +822,7 @@ template <int DT> struct LeakyShape {
         r.ncb = p.DC <= 128 ? 1 : 2;
         const int chunks = (p.T + CH - 1) / CH;
         const long long base = (long long)p.B * p.H * r.ncb;
-        // segments: enough workgroups for two on each of 256 CUs, but not under 256 steps, where a segment's state costs as much traffic as its steps
+        // segments: until there are enough workgroups, but not under 256 steps, where a segment's state costs as much traffic as its steps
         long long nseg = (kLeakyTarget + base - 1) / base;
         const int most = (p.T + 255) / 256;
         if (nseg > most) nseg = most;

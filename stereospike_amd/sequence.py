@@ -24,24 +24,20 @@ from ._lib import SSNeuronError, _require_hip
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
-def _same_device(ref, **tensors):
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        _require_hip(t, name)
-        if t.device != ref.device:
-            raise SSNeuronError(f'{name} is on {t.device}, expected {ref.device}')
-
-
-def _is(t, name, dtype, shape):
+def _operand(t, name, dev, dtype, shape):
+    """A tensor of this device, type and shape, or the reason why not."""
+    if isinstance(t, torch.Tensor) and t.device == dev and t.dtype is dtype and t.shape == shape:
+        return
+    _require_hip(t, name)
+    if t.device != dev:
+        raise SSNeuronError(f'{name} is on {t.device}, expected {dev}')
     if t.dtype != dtype:
         raise SSNeuronError(f'{name}: expected {dtype}, got {t.dtype}')
-    if tuple(t.shape) != tuple(shape):
-        raise SSNeuronError(f'{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}')
+    raise SSNeuronError(f'{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}')
 
 
 def _last_contiguous(t):
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 and t.numel() > 0 and t.is_contiguous() else t.contiguous()
+    return t if t.stride(-1) == 1 or t.is_contiguous() else t.contiguous()
 
 
 # ----------------------------------------------------------------------------------------------------------------------------------------------------------
@@ -49,30 +45,28 @@ def _last_contiguous(t):
 # ----------------------------------------------------------------------------------------------------------------------------------------------------------
 def _attention_operands(q, k, v, log_decay, state, lengths, lead):
     _require_hip(q, 'q')
-    if q.dtype not in _FLOATS:
-        raise SSNeuronError(f'q: expected float32, float16 or bfloat16, got {q.dtype}')
+    dt, dev = q.dtype, q.device
+    if dt not in _FLOATS:
+        raise SSNeuronError(f'q: expected float32, float16 or bfloat16, got {dt}')
     if q.dim() != lead + 2 or k.dim() != lead + 2 or v.dim() != lead + 2:
         raise SSNeuronError(f'q, k, v: expected {lead + 2} axes ([{"T, " if lead == 2 else ""}B, heads, D]), got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}')
-    _same_device(q, k=k, v=v, log_decay=log_decay, state=state, lengths=lengths)
-    head = tuple(q.shape[:lead])
-    H, Dk = q.shape[lead:]
-    Hk, Dv = v.shape[lead:]
-    _is(k, 'k', q.dtype, head + (Hk, Dk))
-    _is(v, 'v', q.dtype, head + (Hk, Dv))
+    qs, vs = q.shape, v.shape
+    B, H, Dk = qs[-3:]
+    Hk, Dv = vs[-2:]
+    head = qs[:lead]
+    _operand(k, 'k', dev, dt, (*head, Hk, Dk))
+    _operand(v, 'v', dev, dt, (*head, Hk, Dv))
     if H < 1 or Hk < 1 or H % Hk:
         raise SSNeuronError(f'{H} query heads cannot share {Hk} key / value heads')
     if not (1 <= Dk <= _seqlib.MAX_HEAD_DIM and 1 <= Dv <= _seqlib.MAX_HEAD_DIM):
         raise SSNeuronError(f'head sizes {Dk} and {Dv}: 1 .. {_seqlib.MAX_HEAD_DIM} are implemented')
-    B = q.shape[lead - 1]
     if B * H > 65535:
         raise SSNeuronError(f'B * heads = {B * H}: at most 65535 states in one call')
-    _is(log_decay, 'log_decay', torch.float32, (H,))
-    if log_decay.requires_grad and torch.is_grad_enabled():
-        raise SSNeuronError('log_decay: the decay of a head is a constant of the layer (as tau of a LIFNode); it has no gradient — pass log_decay.detach()')
+    _operand(log_decay, 'log_decay', dev, torch.float32, (H,))
     if state is not None:
-        _is(state, 'state', torch.float32, (B, H, Dk, Dv))
+        _operand(state, 'state', dev, torch.float32, (B, H, Dk, Dv))
     if lengths is not None:
-        _is(lengths, 'lengths', torch.int32, (B,))
+        _operand(lengths, 'lengths', dev, torch.int32, (B,))
     return B, H, Hk, Dk, Dv
 
 
@@ -137,6 +131,8 @@ def leaky_attention(q_seq: torch.Tensor, k_seq: torch.Tensor, v_seq: torch.Tenso
     Returns o_seq [T, B, H, Dv]; with return_state also the state after the last valid step (fp32).  States, sums and decays are fp32.  Gradients: q, k, v and
     state, from both results."""
     B, H, Hk, Dk, Dv = _attention_operands(q_seq, k_seq, v_seq, log_decay, state, lengths, 2)
+    if log_decay.requires_grad and torch.is_grad_enabled():
+        raise SSNeuronError('log_decay: the decay of a head is a constant of the layer (as tau of a LIFNode); it has no gradient — pass log_decay.detach()')
     scale = Dk ** -0.5 if scale is None else float(scale)
     T = q_seq.shape[0]
     if T == 0 or B == 0:                                   # no step: nothing to launch
@@ -147,19 +143,17 @@ def leaky_attention(q_seq: torch.Tensor, k_seq: torch.Tensor, v_seq: torch.Tenso
     return (out, last) if return_state else out
 
 
-@torch.no_grad()
 def leaky_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor,
                          scale: Optional[float] = None) -> torch.Tensor:
     """One time step of `leaky_attention`: q [B, H, Dk], k [B, Hk, Dk], v [B, Hk, Dv]; `state` (fp32 [B, H, Dk, Dv], contiguous) is updated IN PLACE.
     Returns o [B, H, Dv].  No gradients (use leaky_attention with T = 1)."""
-    _require_hip(state, 'state')
     B, H, Hk, Dk, Dv = _attention_operands(q, k, v, log_decay, state, None, 1)
     if not state.is_contiguous():
         raise SSNeuronError('state: tensor must be contiguous (it is updated in place)')
-    q, k, v = _last_contiguous(q), _last_contiguous(k), _last_contiguous(v)
     out = torch.empty((B, H, Dv), dtype=q.dtype, device=q.device)
     if B:
-        _seqlib.leaky(q[None], k[None], v[None], out[None], log_decay.contiguous(), 1.0, Dk ** -0.5 if scale is None else float(scale), s_in=state, s_out=state)
+        _seqlib.leaky(_last_contiguous(q), _last_contiguous(k), _last_contiguous(v), out, log_decay.contiguous(), 1.0, Dk ** -0.5 if scale is None else float(scale),
+                      s_in=state, s_out=state)
         if not state.is_inference():
             torch.autograd.graph.increment_version(state)  # an autograd graph that saved this state must notice
     return out
@@ -170,55 +164,54 @@ def leaky_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
 # ----------------------------------------------------------------------------------------------------------------------------------------------------------
 def _norm_operands(x, weight, residual, eps):
     _require_hip(x, 'x')
+    shape = x.shape
     if x.dtype not in _FLOATS:
         raise SSNeuronError(f'x: expected float32, float16 or bfloat16, got {x.dtype}')
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= _seqlib.MAX_NORM_WIDTH:
-        raise SSNeuronError(f'x: shape {tuple(x.shape)}; rows of 1 .. {_seqlib.MAX_NORM_WIDTH} values are implemented')
-    _same_device(x, weight=weight, residual=residual)
-    _is(weight, 'weight', torch.float32, (x.shape[-1],))
+    if len(shape) < 1 or not 1 <= shape[-1] <= _seqlib.MAX_NORM_WIDTH:
+        raise SSNeuronError(f'x: shape {tuple(shape)}; rows of 1 .. {_seqlib.MAX_NORM_WIDTH} values are implemented')
+    _operand(weight, 'weight', x.device, torch.float32, shape[-1:])
     if residual is not None:
-        _is(residual, 'residual', x.dtype, x.shape)
+        _operand(residual, 'residual', x.device, x.dtype, shape)
     if not float(eps) >= 0.:
         raise SSNeuronError(f'eps: expected a number >= 0, got {eps}')
 
 
 def _rows(t):
-    t = t.reshape(-1, t.shape[-1])
-    return t if t.shape[1] == 1 or t.stride(1) == 1 else t.contiguous()
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
 class _AddRMSNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, eps):
         ctx.set_materialize_grads(False)
-        need = any(ctx.needs_input_grad[:3])
+        need = any(ctx.needs_input_grad)
         rows = _rows(x)
         if need and residual is None:
             rows = rows.contiguous()                       # kept for the backward
         weight = weight.contiguous()
-        y = torch.empty(rows.shape, dtype=x.dtype, device=x.device)
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         total = torch.empty_like(y) if residual is not None else None
         rstd = torch.empty(rows.shape[0], dtype=torch.float32, device=x.device) if need else None
         if rows.shape[0]:
             _seqlib.rms_norm_fwd(rows, None if residual is None else _rows(residual), weight, y, total, rstd, eps)
         if need:
-            ctx.save_for_backward(rows if residual is None else total.view(rows.shape), weight, rstd)
-        ctx.shape = x.shape
-        return (y.view(x.shape), total.view(x.shape)) if residual is not None else y.view(x.shape)
+            ctx.save_for_backward(rows if residual is None else total, weight, rstd)
+            ctx.shape = x.shape
+        return (y, total) if residual is not None else y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g_y, g_sum=None):
         h, weight, rstd = ctx.saved_tensors
-        need_x, need_r, need_w = ctx.needs_input_grad[:3]
-        g_y, g_sum = (None if g is None else g.reshape(h.shape).contiguous() for g in (g_y, g_sum))
-        g_h = torch.empty_like(h)
+        need_x, need_r, need_w, _ = ctx.needs_input_grad
+        g_h = torch.empty(ctx.shape, dtype=h.dtype, device=h.device)
         g_w = torch.empty_like(weight) if need_w else None
-        if h.shape[0]:
-            _seqlib.rms_norm_bwd(g_y, g_sum, h, weight, rstd, g_h, g_w)
+        if rstd.shape[0]:
+            _seqlib.rms_norm_bwd(None if g_y is None else g_y.contiguous(), None if g_sum is None else g_sum.contiguous(), _rows(h), weight, rstd, g_h, g_w)
         elif need_w:
             g_w.zero_()
-        g_h = g_h.view(ctx.shape)
         return g_h if need_x else None, g_h if need_r else None, g_w, None
 
 
@@ -232,36 +225,34 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
     return _AddRMSNorm.apply(x, residual, weight, float(eps))
 
 
-@torch.no_grad()
 def add_rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
     """`add_rms_norm` handed on in 8 bits: returns (codes int8 [..., C], scales fp32 [...], h) with codes * scales the norm; the largest value of a row has the
     code +-127, ties go to the even code.  A row of zeros has scale 0; a row with a NaN or an infinity has codes 0 and scale NaN.  No gradients."""
     _norm_operands(x, weight, residual, eps)
+    shape, dev = x.shape, x.device
     rows = _rows(x)
-    codes = torch.empty(rows.shape, dtype=torch.int8, device=x.device)
-    scales = torch.empty(rows.shape[0], dtype=torch.float32, device=x.device)
-    total = torch.empty(rows.shape, dtype=x.dtype, device=x.device) if residual is not None else None
+    codes = torch.empty(shape, dtype=torch.int8, device=dev)
+    scales = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
+    total = torch.empty(shape, dtype=x.dtype, device=dev) if residual is not None else None
     if rows.shape[0]:
         _seqlib.rms_norm_int8(rows, None if residual is None else _rows(residual), weight.contiguous(), codes, scales, total, float(eps))
-    return codes.view(x.shape), scales.view(x.shape[:-1]), x if residual is None else total.view(x.shape)
+    return codes, scales, x if residual is None else total
 
 
-@torch.no_grad()
 def dequantize_int8(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values that 8-bit codes [..., C] with a scale per row [...] stand for."""
     _require_hip(codes, 'codes')
-    _same_device(codes, scales=scales)
-    if codes.dim() < 1 or codes.shape[-1] < 1:
-        raise SSNeuronError(f'codes: expected [..., C], got {tuple(codes.shape)}')
-    _is(codes, 'codes', torch.int8, codes.shape)
-    _is(scales, 'scales', torch.float32, codes.shape[:-1])
+    shape = codes.shape
+    if len(shape) < 1 or shape[-1] < 1:
+        raise SSNeuronError(f'codes: expected [..., C], got {tuple(shape)}')
+    _operand(codes, 'codes', codes.device, torch.int8, shape)
+    _operand(scales, 'scales', codes.device, torch.float32, shape[:-1])
     if dtype not in _FLOATS:
         raise SSNeuronError(f'dtype: expected float32, float16 or bfloat16, got {dtype}')
-    rows = codes.reshape(-1, codes.shape[-1]).contiguous()
-    out = torch.empty(rows.shape, dtype=dtype, device=codes.device)
-    if rows.shape[0]:
-        _seqlib.dequant_int8(rows, scales.reshape(-1).contiguous(), out)
-    return out.view(codes.shape)
+    out = torch.empty(shape, dtype=dtype, device=codes.device)
+    if out.numel():
+        _seqlib.dequant_int8(codes.contiguous(), scales.contiguous(), out)
+    return out
 
 
 # ----------------------------------------------------------------------------------------------------------------------------------------------------------
@@ -286,24 +277,24 @@ def int8_linear(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor,
     codes int8 [..., K] (spike counts are codes of scale 1), scales fp32 [...], weight int8 [N, K], weight_scale fp32 [N], bias fp32 [N]; K < 131072.  Scaled in
     fp32, rounded once to out_dtype (float32 / float16 / bfloat16).  No gradients."""
     _require_hip(codes, 'codes')
-    _same_device(codes, scales=scales, weight=weight, weight_scale=weight_scale, bias=bias)
-    if codes.dim() < 1 or weight.dim() != 2:
-        raise SSNeuronError(f'codes [..., K], weight [N, K]: got {tuple(codes.shape)}, {tuple(weight.shape)}')
+    shape, dev = codes.shape, codes.device
+    if len(shape) < 1 or weight.dim() != 2:
+        raise SSNeuronError(f'codes [..., K], weight [N, K]: got {tuple(shape)}, {tuple(weight.shape)}')
     N, K = weight.shape
-    _is(codes, 'codes', torch.int8, codes.shape[:-1] + (K,))
-    _is(scales, 'scales', torch.float32, codes.shape[:-1])
-    _is(weight, 'weight', torch.int8, (N, K))
-    _is(weight_scale, 'weight_scale', torch.float32, (N,))
+    lead = shape[:-1]
+    _operand(codes, 'codes', dev, torch.int8, (*lead, K))
+    _operand(scales, 'scales', dev, torch.float32, lead)
+    _operand(weight, 'weight', dev, torch.int8, (N, K))
+    _operand(weight_scale, 'weight_scale', dev, torch.float32, (N,))
     if bias is not None:
-        _is(bias, 'bias', torch.float32, (N,))
+        _operand(bias, 'bias', dev, torch.float32, (N,))
     if not 1 <= K <= _seqlib.MAX_INT8_K or N < 1:
         raise SSNeuronError(f'weight: [N, K] = [{N}, {K}]; N >= 1 and 1 <= K <= {_seqlib.MAX_INT8_K} (sums stay within 32 bits) are implemented')
     if out_dtype not in _FLOATS:
         raise SSNeuronError(f'out_dtype: expected float32, float16 or bfloat16, got {out_dtype}')
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (scales, weight_scale, bias)):
+    if (scales.requires_grad or weight_scale.requires_grad or (bias is not None and bias.requires_grad)) and torch.is_grad_enabled():
         raise SSNeuronError('int8_linear has no gradient: call it under torch.no_grad() or detach scales and bias')
-    rows = _rows(codes)
-    out = torch.empty((rows.shape[0], N), dtype=out_dtype, device=codes.device)
-    if rows.shape[0]:
-        _seqlib.int8_linear(rows, scales.reshape(-1).contiguous(), _rows(weight), weight_scale.contiguous(), None if bias is None else bias.contiguous(), out)
-    return out.view(codes.shape[:-1] + (N,))
+    out = torch.empty((*lead, N), dtype=out_dtype, device=dev)
+    if out.numel():
+        _seqlib.int8_linear(_rows(codes), scales.contiguous(), _rows(weight), weight_scale.contiguous(), None if bias is None else bias.contiguous(), out)
+    return out
