@@ -50,7 +50,7 @@ def lib():
                             ('ss_seq_rms_norm_bwd', i32, [p, p, p, p, p, p, p, p, i64, i32, i32, p]),
                             ('ss_seq_rms_norm_int8', i32, [p, i64, p, i64, p, p, p, p, i64, i32, f32, i32, p]),
                             ('ss_seq_dequant_int8', i32, [p, p, p, i64, i32, i32, p]),
-                            ('ss_seq_int8_linear_ws_ints', i64, [i64, i32, i32]),
+                            ('ss_seq_int8_linear_ws_ints', i64, [p, i64, p, i64, i64, i32, i32]),
                             ('ss_seq_int8_linear', i32, [p, i64, p, p, i64, p, p, p, i64, i32, i32, i32, p, p])):
         f = getattr(L, name)
         f.restype, f.argtypes = res, args
@@ -142,7 +142,7 @@ def dequant_int8(codes, scales, out):
 def int8_linear(a, a_scale, w, w_scale, bias, out):
     """a [M, K], w [N, K] int8 with contiguous last axes; out [M, N] contiguous."""
     (M, K), N = a.shape, w.shape[0]
-    n = (_lib or lib()).ss_seq_int8_linear_ws_ints(M, N, K)
+    pa, la, pw, lw = a.data_ptr(), a.stride(0), w.data_ptr(), w.stride(0)
+    n = (_lib or lib()).ss_seq_int8_linear_ws_ints(pa, la, pw, lw, M, N, K)
     ws = torch.empty(n, dtype=torch.int32, device=a.device) if n else None
-    _call('ss_seq_int8_linear', a.device, a.data_ptr(), a.stride(0), a_scale.data_ptr(), w.data_ptr(), w.stride(0), w_scale.data_ptr(), _p(bias), out.data_ptr(),
-          M, N, K, DT_CODE[out.dtype], _p(ws))
+    _call('ss_seq_int8_linear', a.device, pa, la, a_scale.data_ptr(), pw, lw, w_scale.data_ptr(), _p(bias), out.data_ptr(), M, N, K, DT_CODE[out.dtype], _p(ws))
