@@ -53,22 +53,17 @@ template <int DT, int ODT, int R, bool V4> __global__ __launch_bounds__(256) voi
     f32x4 S[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        S[r] = (f32x4){0.f, 0.f, 0.f, 0.f};
-        const int i = g + 16 * r;
-        if (!s_in) continue;
-        if constexpr (V4) { if (i < p.DA && j0 < p.DC) S[r] = *reinterpret_cast<const f32x4*>(s_in + i * p.s_in_row + j0); }
-        else
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {                  // (a select, not a branch, for each element)
-                const bool in = i < p.DA && j0 + e < p.DC;
-                const float v = s_in[in ? i * p.s_in_row + (j0 + e) * p.s_in_col : 0];
-                S[r][e] = in ? v : 0.f;
-            }
+        const int i = min(g + 16 * r, p.DA - 1);           // (outside: the nearest inside, never used or stored)
+        if (!s_in) S[r] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        else if constexpr (V4) S[r] = *reinterpret_cast<const f32x4*>(s_in + i * p.s_in_row + min(j0, p.DC - 4));
+        else S[r] = (f32x4){s_in[i * p.s_in_row + min(j0, p.DC - 1) * p.s_in_col], s_in[i * p.s_in_row + min(j0 + 1, p.DC - 1) * p.s_in_col],
+                            s_in[i * p.s_in_row + min(j0 + 2, p.DC - 1) * p.s_in_col], s_in[i * p.s_in_row + min(j0 + 3, p.DC - 1) * p.s_in_col]};
     }
     for (int i = 0; i < n; ++i) {
         const long long t = p.reverse ? n - 1 - i : i;
         __syncthreads();
-        if (tid < p.DA) { sa[tid] = widen<DT>(pa[t * p.a_t + tid]) * p.o_scale; sb[tid] = widen<DT>(pb[t * p.b_t + tid]) * p.b_scale; }
+        sa[tid] = tid < p.DA ? widen<DT>(pa[t * p.a_t + tid]) * p.o_scale : 0.f;
+        sb[tid] = tid < p.DA ? widen<DT>(pb[t * p.b_t + tid]) * p.b_scale : 0.f;
         __syncthreads();
         f32x4 c = {0.f, 0.f, 0.f, 0.f}, o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -76,18 +71,12 @@ template <int DT, int ODT, int R, bool V4> __global__ __launch_bounds__(256) voi
         const bool leaks = i > 0 || !p.reverse;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const int row = g + 16 * r;
-            if (row < p.DA) {
-                const float bi = sb[row], ai = sa[row];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float s = S[r][e];
-                    if (leaks) s = fmaf(s, leak, s * kept);
-                    s = fmaf(bi, c[e], s);
-                    o[e] = fmaf(ai, s, o[e]);
-                    S[r][e] = s;
-                }
-            }
+            const int row = g + 16 * r;                    // rows behind DA: sa, sb are zero there
+            f32x4 s = S[r];
+            if (leaks) s = s * leak + s * kept;
+            s += sb[row] * c;
+            o += sa[row] * s;
+            S[r] = s;
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -116,13 +105,59 @@ template <int DT, int ODT, int R, bool V4> __global__ __launch_bounds__(256) voi
     }
 }
 
+// One step, forward: the state is read, updated and written once (HBM-bound: 8 bytes for each of its values); all R rows of a thread are in flight at once.
+template <int DT, int ODT, int R> __global__ __launch_bounds__(256) void leaky_step_kernel(const LeakyArgs p)
+{
+    __shared__ float sa[256], sb[256], red[4][64];
+    const int tid = threadIdx.x, x = tid & 15, g = tid >> 4;
+    const int bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H, j0 = blockIdx.x * 64 + 4 * x;
+    const float* s_in = p.s_in + (long long)bh * p.DA * p.DC + j0;
+    float* s_out = p.s_out + (long long)bh * p.DA * p.DC + j0;
+    const bool live = j0 < p.DC;
+    f32x4 S[R];
+    // (rows and columns outside are read at the nearest inside: a branch per load would end the loads' flight together)
+    const float* from = live ? s_in : s_in - j0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) S[r] = *reinterpret_cast<const f32x4*>(from + (long long)min(g + 16 * r, p.DA - 1) * p.s_in_row);
+    const float lam = expf(fmaxf(p.log_decay[h], -1e30f));
+    if (tid < p.DA) {
+        sa[tid] = widen<DT>(static_cast<const elem_t<DT>*>(p.a)[b * p.a_b + (h / p.a_group) * p.a_h + tid]) * p.o_scale;
+        sb[tid] = widen<DT>(static_cast<const elem_t<DT>*>(p.b)[b * p.b_b + (h / p.b_group) * p.b_h + tid]) * p.b_scale;
+    }
+    f32x4 c = {0.f, 0.f, 0.f, 0.f}, o = {0.f, 0.f, 0.f, 0.f};
+    if (live)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[e] = widen<DT>(static_cast<const elem_t<DT>*>(p.c)[b * p.c_b + (h / p.c_group) * p.c_h + j0 + e]);
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int row = g + 16 * r;
+        if (live && row < p.DA) {
+            const f32x4 s = S[r] * lam + sb[row] * c;
+            o += sa[row] * s;
+            *reinterpret_cast<f32x4*>(s_out + (long long)row * p.s_out_row) = s;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        o[e] += __shfl_xor(o[e], 16);
+        o[e] += __shfl_xor(o[e], 32);
+    }
+    if ((tid & 48) == 0) *reinterpret_cast<f32x4*>(&red[tid >> 6][4 * x]) = o;
+    __syncthreads();
+    if (tid < 64 && blockIdx.x * 64 + tid < p.DC)
+        static_cast<elem_t<ODT>*>(p.out)[b * p.o_b + h * p.o_h + blockIdx.x * 64 + tid] = narrow<ODT>(red[0][tid] + red[1][tid] + red[2][tid] + red[3][tid]);
+}
+
 template <int DT, int ODT> int steps(const LeakyArgs& p, hipStream_t s)
 {
     const bool v4 = p.DC % 4 == 0 && (!p.s_in || (p.s_in_col == 1 && p.s_in_row % 4 == 0 && aligned(p.s_in, 16))) &&
                     (!p.s_out || (p.s_out_col == 1 && p.s_out_row % 4 == 0 && aligned(p.s_out, 16)));
     const dim3 grid((unsigned)((p.DC + 63) / 64), (unsigned)(p.B * p.H));
+    const bool one = p.T == 1 && !p.reverse && v4 && p.s_in && p.s_out && !p.lengths;
     auto go = [&](auto R) {
-        if (v4) leaky_steps_kernel<DT, ODT, R.value, true><<<grid, 256, 0, s>>>(p);
+        if (one) leaky_step_kernel<DT, ODT, R.value><<<grid, 256, 0, s>>>(p);
+        else if (v4) leaky_steps_kernel<DT, ODT, R.value, true><<<grid, 256, 0, s>>>(p);
         else leaky_steps_kernel<DT, ODT, R.value, false><<<grid, 256, 0, s>>>(p);
         return launched();
     };

@@ -72,7 +72,8 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_fwd_kernel(const No
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             const int j = (v * TPR + lane) * VEC + e;
-            w[v * VEC + e] = j < p.C ? p.w[j] : 0.f;
+            const float t = p.w[min(j, p.C - 1)];
+            w[v * VEC + e] = j < p.C ? t : 0.f;
         }
     for (long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR; row < p.rows; row += (long long)gridDim.x * RPB) {
         const elem_t<DT>* x = static_cast<const elem_t<DT>*>(p.x) + row * p.xs;
@@ -80,26 +81,22 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_fwd_kernel(const No
         float h[NE];
         P px[NV], pr[NV];
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {                     // all loads of the row first
-            const int j = (v * TPR + lane) * VEC;
-            if (j < p.C) {
-                px[v] = *reinterpret_cast<const P*>(x + j);
-                if (r) pr[v] = *reinterpret_cast<const P*>(r + j);
-            }
+        for (int v = 0; v < NV; ++v) {                     // all loads of the row first; behind its end: its last access, counted as zeros
+            const int j = min((v * TPR + lane) * VEC, p.C - VEC);
+            px[v] = *reinterpret_cast<const P*>(x + j);
+            if (r) pr[v] = *reinterpret_cast<const P*>(r + j);
         }
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int j = (v * TPR + lane) * VEC;
+            const bool in = j < p.C;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) h[v * VEC + e] = 0.f;
-            if (j < p.C) {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    if (r) px[v].v[e] = narrow<DT>(widen<DT>(px[v].v[e]) + widen<DT>(pr[v].v[e]));     // the sum is kept, and normed, in the input's type
-                    h[v * VEC + e] = widen<DT>(px[v].v[e]);
-                }
-                if (r) *reinterpret_cast<P*>(static_cast<elem_t<DT>*>(p.sum) + row * p.C + j) = px[v];
+            for (int e = 0; e < VEC; ++e) {
+                if (r) px[v].v[e] = narrow<DT>(widen<DT>(px[v].v[e]) + widen<DT>(pr[v].v[e]));         // the sum is kept, and normed, in the input's type
+                const float t = widen<DT>(px[v].v[e]);
+                h[v * VEC + e] = in ? t : 0.f;
             }
+            if (r && in) *reinterpret_cast<P*>(static_cast<elem_t<DT>*>(p.sum) + row * p.C + j) = px[v];
         }
         bool broken;
         const float rstd = rstd_of<TPR, NE>(h, p.C, p.eps, redf, redd, broken);
@@ -118,32 +115,37 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_fwd_kernel(const No
         } else {
             // codes = rint(127 u / top), u = h w: rstd cancels.  In fp32 the quotient is off by at most 127 * 4 * 2^-24 = 3e-5; values within 1e-4 of the
             // border of two codes (2 in 10^4) are decided in fp64, where u is exact, so codes do not depend on how the sum of squares was rounded.
-            float top = 0.f;
+            float most = 0.f;
 #pragma unroll
-            for (int i = 0; i < NE; ++i) top = fmaxf(top, fabsf(h[i] * w[i]));
-            top = row_reduce<TPR, float, true>(top, redf);
+            for (int i = 0; i < NE; ++i) most = fmaxf(most, fabsf(h[i] * w[i]));
+            const float top = row_reduce<TPR, float, true>(most, redf);
             double top64 = 0.;                             // rounding keeps order: the largest u in fp64 is among those whose rounded value is the largest
+            if (most == top)
 #pragma unroll
-            for (int i = 0; i < NE; ++i)
-                if (fabsf(h[i] * w[i]) == top) top64 = fmax(top64, fabs((double)h[i] * (double)w[i]));
+                for (int i = 0; i < NE; ++i) top64 = fmax(top64, fabs((double)h[i] * (double)w[i]));
             top64 = row_reduce<TPR, double, true>(top64, redd);
             broken = broken || !(top64 < 3.4e38);
             const float c = 127.f / top;
             const bool plain = top > 1e-30f && !broken;    // 127 / top in range
             if (lane == 0) p.scales[row] = broken ? __uint_as_float(0x7FC00000u) : top64 == 0. ? 0.f : (float)(top64 * (double)rstd / 127.0);
+            int code[NE];
+            bool close = !plain;
+#pragma unroll
+            for (int i = 0; i < NE; ++i) {
+                const float t = h[i] * w[i] * c, q = rintf(t);
+                code[i] = (int)q;
+                close = close || fabsf(t - q) > 0.4999f;
+            }
+            if (close)                                     // one branch for the thread's values, not one each
+#pragma unroll
+                for (int i = 0; i < NE; ++i) code[i] = broken || top64 == 0. ? 0 : (int)rint((double)h[i] * (double)w[i] * 127.0 / top64);
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 const int j = (v * TPR + lane) * VEC;
                 if (j < p.C) {
                     struct alignas(VEC) { signed char v[VEC]; } o;
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const float hi = h[v * VEC + e], wi = w[v * VEC + e], t = hi * wi * c, q = rintf(t);
-                        int code = (int)q;
-                        if (!plain || fabsf(t - q) > 0.4999f)
-                            code = broken || top64 == 0. ? 0 : (int)rint((double)hi * (double)wi * 127.0 / top64);
-                        o.v[e] = (signed char)code;
-                    }
+                    for (int e = 0; e < VEC; ++e) o.v[e] = (signed char)code[v * VEC + e];
                     *reinterpret_cast<decltype(o)*>(p.codes + row * p.C + j) = o;
                 }
             }
@@ -174,19 +176,18 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_bwd_kernel(const No
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             const int j = (v * TPR + lane) * VEC + e;
-            w[v * VEC + e] = j < p.C ? p.w[j] : 0.f;
+            const float t = p.w[min(j, p.C - 1)];
+            w[v * VEC + e] = j < p.C ? t : 0.f;
             gw[v * VEC + e] = 0.f;
         }
     for (long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR; row < p.rows; row += (long long)gridDim.x * RPB) {
         P pg[NV], ph[NV], ps[NV];
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int j = (v * TPR + lane) * VEC;
-            if (j < p.C) {
-                ph[v] = *reinterpret_cast<const P*>(static_cast<const elem_t<DT>*>(p.h) + row * p.C + j);
-                if (p.gy) pg[v] = *reinterpret_cast<const P*>(static_cast<const elem_t<DT>*>(p.gy) + row * p.C + j);
-                if (p.gs) ps[v] = *reinterpret_cast<const P*>(static_cast<const elem_t<DT>*>(p.gs) + row * p.C + j);
-            }
+        for (int v = 0; v < NV; ++v) {                     // behind the row's end: its last access, counted as zeros
+            const long long j = row * p.C + min((v * TPR + lane) * VEC, p.C - VEC);
+            ph[v] = *reinterpret_cast<const P*>(static_cast<const elem_t<DT>*>(p.h) + j);
+            if (p.gy) pg[v] = *reinterpret_cast<const P*>(static_cast<const elem_t<DT>*>(p.gy) + j);
+            if (p.gs) ps[v] = *reinterpret_cast<const P*>(static_cast<const elem_t<DT>*>(p.gs) + j);
         }
         const float rstd = p.rstd[row];
         float n[NE], g[NE], dot = 0.f;
@@ -240,20 +241,30 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_bwd_kernel(const No
         }
 }
 
-// g_w[j] = sum of the blocks' partials, in their order: 32 columns x 32 slices per block
+// g_w[j] = sum of the blocks' partials, in a fixed order: 16 columns x 64 slices per block, 16 partials of a slice in flight
 __global__ __launch_bounds__(1024) void rms_gw_kernel(const float* __restrict__ ws, float* __restrict__ gw, int P, int C)
 {
-    __shared__ float red[32][33];
-    const int cx = threadIdx.x & 31, sl = threadIdx.x >> 5, j = blockIdx.x * 32 + cx;
+    __shared__ float red[64][17];
+    const int cx = threadIdx.x & 15, sl = threadIdx.x >> 4, j = blockIdx.x * 16 + cx;
     float s = 0.f;
-    if (j < C)
-        for (int i = sl; i < P; i += 32) s += ws[(long long)i * C + j];
+    if (j < C) {
+        int i = sl;
+        for (; i + 15 * 64 < P; i += 16 * 64) {
+            float v[16];
+#pragma unroll
+            for (int u = 0; u < 16; ++u) v[u] = ws[(long long)(i + 64 * u) * C + j];
+#pragma unroll
+            for (int u = 0; u < 16; ++u) s += v[u];
+        }
+        for (; i < P; i += 64) s += ws[(long long)i * C + j];
+    }
     red[sl][cx] = s;
     __syncthreads();
-    if (sl == 0 && j < C) {
-        for (int i = 1; i < 32; ++i) s += red[i][cx];
-        gw[j] = s;
+    for (int k = 32; k; k >>= 1) {
+        if (sl < k) red[sl][cx] += red[sl + k][cx];
+        __syncthreads();
     }
+    if (sl == 0 && j < C) gw[j] = red[0][cx];
 }
 
 template <int DT, int VEC> __global__ __launch_bounds__(256) void dequant_kernel(const signed char* __restrict__ q, const float* __restrict__ sc,
@@ -326,7 +337,7 @@ template <int DT> int bwd_dt(const NormBwdArgs& p, float* gw, hipStream_t s)
             rms_bwd_kernel<DT, VC.value, TPR.value, NV.value><<<grid, block, 0, s>>>(p);
             if (int rc = launched()) return rc;
             if (gw) {
-                rms_gw_kernel<<<(p.C + 31) / 32, 1024, 0, s>>>(p.ws, gw, (int)grid, p.C);
+                rms_gw_kernel<<<(p.C + 15) / 16, 1024, 0, s>>>(p.ws, gw, (int)grid, p.C);
                 return launched();
             }
             return SS_SEQ_OK;
