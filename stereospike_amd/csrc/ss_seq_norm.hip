@@ -25,35 +25,32 @@ struct NormArgs {
     float eps;
 };
 
-// sum / max over the TPR threads of a row; every thread gets it.  `red`: one slot per wavefront (unused for TPR = 64)
-template <int TPR, typename V, bool MAX> __device__ __forceinline__ V row_reduce(V v, V* red)
+// The row's value of v over its TPR threads, by every thread.  `red`: one slot per wavefront (unused for TPR = 64).  One barrier: the caller alternates between
+// slots, so that those of the last reduction are free again only after the barrier of the next.
+template <int TPR, bool MAX, typename V> __device__ __forceinline__ V row_reduce(V v, V* red)
 {
     if constexpr (MAX) v = wave_max(v); else v = wave_sum(v);
     if constexpr (TPR > 64) {
-        constexpr int W = TPR / 64;
-        __syncthreads();                                   // the slots of the last reduction have been read
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
         v = red[0];
 #pragma unroll
-        for (int i = 1; i < W; ++i) v = MAX ? (V)fmax(v, red[i]) : v + red[i];
+        for (int i = 1; i < TPR / 64; ++i) v = MAX ? (v > red[i] ? v : red[i]) : v + red[i];
     }
     return v;
 }
 
-// mean of squares -> 1 / sqrt(mean + eps).  fp32 sums leave their range for |h| beyond 1e18 or below 1e-14: those rows are summed again in fp64.
-template <int TPR, int NE> __device__ __forceinline__ float rstd_of(const float (&h)[NE], int C, float eps, float* redf, double* redd, bool& broken)
+// fp32 sums of squares leave their range for |h| beyond 1e18 or below 1e-14: those rows are summed again in fp64.  (The same branch for all threads of a row.)
+template <int TPR, int NE> __device__ __forceinline__ float rstd_of(float s, const float (&h)[NE], int C, float eps, double* redd, bool& broken)
 {
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < NE; ++i) s = fmaf(h[i], h[i], s);
-    s = row_reduce<TPR, float, false>(s, redf);
     broken = false;
     if (s < 1e37f && s > 1e-25f) return rsqrtf(s / (float)C + eps);
     double d = 0.;
 #pragma unroll
     for (int i = 0; i < NE; ++i) d += (double)h[i] * (double)h[i];
-    d = row_reduce<TPR, double, false>(d, redd);
+    if constexpr (TPR > 64) __syncthreads();               // the slots' last values have been read
+    d = row_reduce<TPR, false>(d, redd);
+    if constexpr (TPR > 64) __syncthreads();
     broken = !(d <= 1.7976931348623157e308);              // a NaN or an infinity in the row
     return (float)(1.0 / sqrt(d / (double)C + (double)eps));
 }
@@ -62,10 +59,11 @@ template <int DT, int VEC, int TPR, int NV, bool INT8>
 __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_fwd_kernel(const NormArgs p)
 {
     constexpr int BLOCK = TPR == 64 ? 256 : TPR, RPB = BLOCK / TPR, NE = NV * VEC;
-    __shared__ float redf[16];
+    __shared__ float redf[2][16], redm[16];
     __shared__ double redd[16];
     typedef Pack<DT, VEC> P;
     const int lane = threadIdx.x % TPR;
+    int turn = 0;                                          // which slots: see row_reduce
     float w[NE];
 #pragma unroll
     for (int v = 0; v < NV; ++v)
@@ -75,31 +73,54 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_fwd_kernel(const No
             const float t = p.w[min(j, p.C - 1)];
             w[v * VEC + e] = j < p.C ? t : 0.f;
         }
-    for (long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR; row < p.rows; row += (long long)gridDim.x * RPB) {
+    const bool add = p.r != nullptr;
+    P px[NV], pr[NV];
+    auto load = [&](long long row) {                       // behind the row's end: its last access, counted as zeros below
         const elem_t<DT>* x = static_cast<const elem_t<DT>*>(p.x) + row * p.xs;
-        const elem_t<DT>* r = p.r ? static_cast<const elem_t<DT>*>(p.r) + row * p.rs : nullptr;
-        float h[NE];
-        P px[NV], pr[NV];
+        const elem_t<DT>* r = static_cast<const elem_t<DT>*>(p.r) + row * p.rs;
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {                     // all loads of the row first; behind its end: its last access, counted as zeros
+        for (int v = 0; v < NV; ++v) {
             const int j = min((v * TPR + lane) * VEC, p.C - VEC);
             px[v] = *reinterpret_cast<const P*>(x + j);
-            if (r) pr[v] = *reinterpret_cast<const P*>(r + j);
+            if (add) pr[v] = *reinterpret_cast<const P*>(r + j);
         }
+    };
+    const long long stride = (long long)gridDim.x * RPB;
+    long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
+    if (row < p.rows) load(row);
+    for (; row < p.rows; row += stride) {
+        float h[NE];
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int j = (v * TPR + lane) * VEC;
             const bool in = j < p.C;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                if (r) px[v].v[e] = narrow<DT>(widen<DT>(px[v].v[e]) + widen<DT>(pr[v].v[e]));         // the sum is kept, and normed, in the input's type
+                if (add) px[v].v[e] = narrow<DT>(widen<DT>(px[v].v[e]) + widen<DT>(pr[v].v[e]));         // the sum is kept, and normed, in the input's type
                 const float t = widen<DT>(px[v].v[e]);
                 h[v * VEC + e] = in ? t : 0.f;
             }
-            if (r && in) *reinterpret_cast<P*>(static_cast<elem_t<DT>*>(p.sum) + row * p.C + j) = px[v];
+            if (add && in) *reinterpret_cast<P*>(static_cast<elem_t<DT>*>(p.sum) + row * p.C + j) = px[v];
         }
+        if (row + stride < p.rows) load(row + stride);     // under way while this row is reduced and written
+        float sum = 0.f, most = 0.f;
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+            sum = fmaf(h[i], h[i], sum);
+            if constexpr (INT8) most = fmaxf(most, fabsf(h[i] * w[i]));
+        }
+        float top = 0.f;
+        if constexpr (INT8) {                              // both over the row with one barrier
+            top = wave_max(most);
+            if constexpr (TPR > 64) { if ((threadIdx.x & 63) == 0) redm[threadIdx.x >> 6] = top; }
+        }
+        sum = row_reduce<TPR, false>(sum, redf[turn]);
+        if constexpr (INT8 && TPR > 64)
+#pragma unroll
+            for (int i = 0; i < TPR / 64; ++i) top = fmaxf(top, redm[i]);
+        if constexpr (!INT8) turn ^= 1;
         bool broken;
-        const float rstd = rstd_of<TPR, NE>(h, p.C, p.eps, redf, redd, broken);
+        const float rstd = rstd_of<TPR, NE>(sum, h, p.C, p.eps, redd, broken);
         if constexpr (!INT8) {
             if (p.rstd && lane == 0) p.rstd[row] = rstd;
 #pragma unroll
@@ -115,15 +136,11 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_fwd_kernel(const No
         } else {
             // codes = rint(127 u / top), u = h w: rstd cancels.  In fp32 the quotient is off by at most 127 * 4 * 2^-24 = 3e-5; values within 1e-4 of the
             // border of two codes (2 in 10^4) are decided in fp64, where u is exact, so codes do not depend on how the sum of squares was rounded.
-            float most = 0.f;
-#pragma unroll
-            for (int i = 0; i < NE; ++i) most = fmaxf(most, fabsf(h[i] * w[i]));
-            const float top = row_reduce<TPR, float, true>(most, redf);
             double top64 = 0.;                             // rounding keeps order: the largest u in fp64 is among those whose rounded value is the largest
             if (most == top)
 #pragma unroll
                 for (int i = 0; i < NE; ++i) top64 = fmax(top64, fabs((double)h[i] * (double)w[i]));
-            top64 = row_reduce<TPR, double, true>(top64, redd);
+            top64 = row_reduce<TPR, true>(top64, redd);
             broken = broken || !(top64 < 3.4e38);
             const float c = 127.f / top;
             const bool plain = top > 1e-30f && !broken;    // 127 / top in range
@@ -166,7 +183,8 @@ template <int DT, int VEC, int TPR, int NV>
 __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_bwd_kernel(const NormBwdArgs p)
 {
     constexpr int BLOCK = TPR == 64 ? 256 : TPR, RPB = BLOCK / TPR, NE = NV * VEC;
-    __shared__ float redf[16];
+    __shared__ float redf[2][16];
+    int turn = 0;
     __shared__ float part[TPR == 64 ? 3 * 64 * NE : 1];
     typedef Pack<DT, VEC> P;
     const int lane = threadIdx.x % TPR;
@@ -204,7 +222,8 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_bwd_kernel(const No
                 dot = fmaf(g[i], n[i], dot);
             }
         }
-        dot = row_reduce<TPR, float, false>(dot, redf) / (float)p.C;
+        dot = row_reduce<TPR, false>(dot, redf[turn]) / (float)p.C;
+        turn ^= 1;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int j = (v * TPR + lane) * VEC;
@@ -284,29 +303,20 @@ template <int DT, int VEC> __global__ __launch_bounds__(256) void dequant_kernel
     }
 }
 
-// Threads of a row and accesses per thread.  Many rows: a wavefront per row as long as its 4 accesses reach.  Few rows (under 1024, the card is not filled and
-// a call is one row's latency): the most threads that have something to do.
-template <typename F> int with_shape(int C, long long rows, int vec, F&& f)
+// Threads of a row and accesses per thread: 16 values a thread at most (more spill).  A wavefront up to 1024 values, where its reductions need no barrier; then
+// 256 threads up to 4096, then 1024.  Few rows (under 1024: the card is not filled and a call is one row's latency): as many threads as have a whole access.
+template <int VEC, typename F> int with_shape(int C, long long rows, F&& f)
 {
-    const int acc = (C + vec - 1) / vec;
-    const bool few = rows < 1024;
-    const int lim64 = few ? 128 : 256;
-    if (vec > 1) {
-        if (acc <= 64) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
-        if (acc <= lim64 && acc <= 128) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
-        if (acc <= lim64) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
-        if (acc <= 512) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
-        if (acc <= 1024 && !few) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 4>());
-        if (acc <= 1024) return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 1>());
-        if (acc <= 2048) return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
-        return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
-    }
-    if (acc <= 64) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
-    if (acc <= 256) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
-    if (acc <= 1024 && !few) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 16>());
-    if (acc <= 1024) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 4>());
-    if (acc <= 4096) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 16>());
-    return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 16>());
+    constexpr int N1 = 1, N2 = VEC == 1 ? 4 : 2, N3 = 16 / VEC;
+    const int acc = (C + VEC - 1) / VEC;
+    auto by = [&](auto TPR) {
+        if (acc <= N1 * TPR.value) return f(TPR, std::integral_constant<int, N1>());
+        if (N2 < N3 && acc <= N2 * TPR.value) return f(TPR, std::integral_constant<int, N2>());
+        return f(TPR, std::integral_constant<int, N3>());
+    };
+    if (C <= 1024 && (rows >= 1024 || acc <= 128)) return by(std::integral_constant<int, 64>());
+    if (C <= 4096 && (rows >= 1024 || acc <= 512)) return by(std::integral_constant<int, 256>());
+    return by(std::integral_constant<int, 1024>());
 }
 
 template <int DT, bool INT8> int fwd_dt(const NormArgs& p, hipStream_t s)
@@ -315,7 +325,7 @@ template <int DT, bool INT8> int fwd_dt(const NormArgs& p, hipStream_t s)
     const void* out = INT8 ? (const void*)p.codes : p.y;
     const bool vec = p.C % V == 0 && p.xs % V == 0 && aligned(p.x, 16) && (!p.r || (p.rs % V == 0 && aligned(p.r, 16) && aligned(p.sum, 16))) && aligned(out, INT8 ? V : 16);
     auto go = [&](auto VC) {
-        return with_shape(p.C, p.rows, VC.value, [&](auto TPR, auto NV) {
+        return with_shape<VC.value>(p.C, p.rows, [&](auto TPR, auto NV) {
             constexpr int block = TPR.value == 64 ? 256 : TPR.value, rpb = block / TPR.value;
             const long long want = (p.rows + rpb - 1) / rpb, cap = 256 * (2048 / block);          // 32 wavefronts for each of 256 CUs
             rms_fwd_kernel<DT, VC.value, TPR.value, NV.value, INT8><<<(unsigned)(want < cap ? want : cap), block, 0, s>>>(p);
@@ -330,7 +340,7 @@ template <int DT> int bwd_dt(const NormBwdArgs& p, float* gw, hipStream_t s)
     constexpr int V = DT == SS_SEQ_F32 ? 4 : 8;
     const bool vec = p.C % V == 0 && aligned(p.gy, 16) && aligned(p.gs, 16) && aligned(p.h, 16) && aligned(p.gh, 16);
     auto go = [&](auto VC) {
-        return with_shape(p.C, p.rows, VC.value, [&](auto TPR, auto NV) {
+        return with_shape<VC.value>(p.C, p.rows, [&](auto TPR, auto NV) {
             constexpr int block = TPR.value == 64 ? 256 : TPR.value, rpb = block / TPR.value;
             const long long want = (p.rows + rpb - 1) / rpb;
             const unsigned grid = (unsigned)(want < kBwdBlocks ? want : kBwdBlocks);
