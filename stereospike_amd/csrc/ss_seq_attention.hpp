@@ -181,8 +181,9 @@ template <int DT, int ODT> int steps(const LeakyArgs& p, hipStream_t s)
 // fp32).  a and b are staged in LDS in that order, so W never leaves the registers; P is shared between the wavefronts through LDS in operand order.
 // Out comes out transposed: a lane stores four consecutive columns of one step.
 //
-// Rounding (bf16): P and W are rounded to bf16 as operands of (2) and (3), each term once; (4) splits lambda^(CH-j) c_j into three bf16 terms (24 bits), so the
-// state keeps fp32 accuracy.  fp32 and fp16 run on the fp32 matrix instructions: P and W may leave fp16's range, and the state has to keep fp32's accuracy.
+// Rounding (16-bit operands): P and W are rounded to the operands' type for (2) and (3), each term once; (4) splits lambda^(CH-j) c_j into three bf16 or two
+// fp16 terms, so the state keeps fp32 accuracy.  fp16's range is too short for P, W and c's terms: they are scaled by powers of two, taken from the largest value
+// of a tile of P, of a wavefront's columns of W, of a column of c.  fp32 operands run on the fp32 matrix instructions.
 // ---------------------------------------------------------------------------------------------------------------------------------------------------------
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef s16x4 __attribute__((address_space(3))) * lds_s16x4;
@@ -552,6 +553,26 @@ store(i0 + 16 * it + l16, col0 + 4 * g, (f32x4){0.f, 0.f, 0.f, 0.f});
 // of 16 rows, and the transposing 4 x 16 read) meet no bank twice.
 // ---------------------------------------------------------------------------------------------------------------------------------------------------------
 template <int SPR> __device__ __forceinline__ int swz(int row) { return SPR >= 16 ? ((row & 7) << 1) | ((row >> 3) & 1) : (((row >> 1) & 3) << 1) | ((row >> 3) & 1); }
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+template <int DT> __device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c)
+{
+    if constexpr (DT == SS_SEQ_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// a power of two that takes `most` into [2^14, 2^15), fp16's upper end, and its inverse; 1 for zero and for what is not finite
+__device__ __forceinline__ void fp16_scale(float most, float& up, float& down)
+{
+    int e = (int)(__float_as_uint(most) >> 23 & 255);      // biased exponent
+    e = e == 0 || e == 255 ? 141 : e < 30 ? 30 : e;
+    up = __uint_as_float((unsigned)(268 - e) << 23);       // 2^(14 - (e - 127))
+    down = __uint_as_float((unsigned)(e - 14) << 23);
+}
+__device__ __forceinline__ f16x8 half8(const f32x4& x, const f32x4& y, float up)
+{
+    return (f16x8){(_Float16)(x[0] * up), (_Float16)(x[1] * up), (_Float16)(x[2] * up), (_Float16)(x[3] * up),
+                   (_Float16)(y[0] * up), (_Float16)(y[1] * up), (_Float16)(y[2] * up), (_Float16)(y[3] * up)};
+}
 // this wavefront's LDS operations are done, then the barrier: unlike __syncthreads() it does not wait for loads on their way to LDS or for stores
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
@@ -563,6 +584,8 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
     __shared__ __attribute__((aligned(1024))) unsigned short lds[2 * BUF];
     __shared__ __attribute__((aligned(16))) unsigned short sp[STATE ? 8 : 2 * 64 * 8];       // P in operand order, by tile of 16 steps
     __shared__ __attribute__((aligned(16))) float rw[CH];                                    // lambda^(e - j) b_scale of the chunk's steps
+    __shared__ float p_down[4];                                                              // fp16: what undoes the scale of P's three tiles
+    constexpr bool H = DT == SS_SEQ_F16;
 
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g = lane >> 4;
     const int cb = blockIdx.x % plan.ncb, rest = blockIdx.x / plan.ncb;
@@ -708,10 +731,10 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
                 f32x4 s = {0.f, 0.f, 0.f, 0.f}, s2 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int k = 0; k < DA / 32; ++k) {
-                    const bf16x8 xa = *reinterpret_cast<const bf16x8*>(la + it * 16 * DA * 2 + (o1 ^ (64 * k)));
-                    const bf16x8 xb = *reinterpret_cast<const bf16x8*>(lb + jt * 16 * DA * 2 + (o1 ^ (64 * k)));
-                    if (k & 1) s2 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb, xa, s2, 0, 0, 0);
-                    else s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb, xa, s, 0, 0, 0);
+                    const s16x8 xa = *reinterpret_cast<const s16x8*>(la + it * 16 * DA * 2 + (o1 ^ (64 * k)));
+                    const s16x8 xb = *reinterpret_cast<const s16x8*>(lb + jt * 16 * DA * 2 + (o1 ^ (64 * k)));
+                    if (k & 1) s2 = mfma16<DT>(xb, xa, s2);
+                    else s = mfma16<DT>(xb, xa, s);
                 }
                 s += s2;
 #pragma unroll
@@ -719,66 +742,106 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
                     const int d = 16 * (it - jt) + l16 - 4 * g - r;      // i - j
                     s[r] = d < 0 ? 0.f : s[r] * (exp2f(gl * (float)d) * p.b_scale * p.o_scale);
                 }
-                typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-                *reinterpret_cast<u32x2*>(sp + (it * 64 + lane) * 8 + jt * 4) = (u32x2){round_pk(s[0], s[1]), round_pk(s[2], s[3])};
+                if constexpr (H) {
+                    float up, down;
+                    fp16_scale(wave_max(fmaxf(fmaxf(fabsf(s[0]), fabsf(s[1])), fmaxf(fabsf(s[2]), fabsf(s[3])))), up, down);
+                    *reinterpret_cast<f16x4*>(sp + (wv * 64 + lane) * 4) = (f16x4){(_Float16)(s[0] * up), (_Float16)(s[1] * up), (_Float16)(s[2] * up), (_Float16)(s[3] * up)};
+                    if (lane == 0) p_down[wv] = down;
+                } else {
+                    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+                    *reinterpret_cast<u32x2*>(sp + (it * 64 + lane) * 8 + jt * 4) = (u32x2){round_pk(s[0], s[1]), round_pk(s[2], s[3])};
+                }
             }
             // (3)
 #pragma unroll
             for (int it = 0; it < 2; ++it)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) acc[it][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            float up = 1.f, down = 1.f;
+            if constexpr (H) {
+                float most = 0.f;
+#pragma unroll
+                for (int kt = 0; kt < KA; ++kt)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(W[kt][nt][r]));
+                fp16_scale(wave_max(most), up, down);
+            }
 #pragma unroll
             for (int k = 0; k < KA / 2; ++k) {
-                bf16x8 xa[2];
+                s16x8 xa[2];
 #pragma unroll
                 for (int it = 0; it < 2; ++it) {
                     const char* q = la + it * 16 * DA * 2 + (o3 ^ (64 * k));
                     const char* q2 = la + it * 16 * DA * 2 + (o3 ^ (64 * k + 32));
-                    xa[it] = __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(*reinterpret_cast<const s16x4*>(q), *reinterpret_cast<const s16x4*>(q2), 0, 1, 2, 3, 4, 5, 6, 7));
+                    xa[it] = __builtin_shufflevector(*reinterpret_cast<const s16x4*>(q), *reinterpret_cast<const s16x4*>(q2), 0, 1, 2, 3, 4, 5, 6, 7);
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     const f32x4 x = W[2 * k][nt], z = W[2 * k + 1][nt];
-                    const bf16x8 fw = mk8(round_pk(x[0], x[1]), round_pk(x[2], x[3]), round_pk(z[0], z[1]), round_pk(z[2], z[3]));
+                    s16x8 fw;
+                    if constexpr (H) fw = __builtin_bit_cast(s16x8, half8(x, z, up));
+                    else fw = __builtin_bit_cast(s16x8, mk8(round_pk(x[0], x[1]), round_pk(x[2], x[3]), round_pk(z[0], z[1]), round_pk(z[2], z[3])));
 #pragma unroll
-                    for (int it = 0; it < 2; ++it) acc[it][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw, xa[it], acc[it][nt], 0, 0, 0);
+                    for (int it = 0; it < 2; ++it) acc[it][nt] = mfma16<DT>(fw, xa[it], acc[it][nt]);
                 }
             }
 #pragma unroll
             for (int it = 0; it < 2; ++it)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) acc[it][nt] *= row_scale[it];
+                for (int nt = 0; nt < NT; ++nt) acc[it][nt] *= row_scale[it] * down;
             lds_barrier();                                               // P is there
         }
         // (2) and (4) share the wavefront's columns of c
-        bf16x8 t0[NT], t1[NT], t2[NT];
+        s16x8 t0[NT], t1[NT], t2[NT];
+        float c_down[NT];
         {
             const f32x4 w0 = *reinterpret_cast<const f32x4*>(rw + 4 * g), w1 = *reinterpret_cast<const f32x4*>(rw + 16 + 4 * g);
-            bf16x8 fp[2];
-            if constexpr (!STATE) {
-#pragma unroll
-                for (int it = 0; it < 2; ++it) fp[it] = *reinterpret_cast<const bf16x8*>(sp + (it * 64 + lane) * 8);
-            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const char* q = lc + (oc ^ (32 * nt));
                 const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)q), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(q + 16 * DCB * 2));
                 const s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                if constexpr (!STATE) {
+                if constexpr (!STATE && H) {               // a product of 16 steps for each tile of P, its scale undone as it is added
+                    const f16x4 *fp = reinterpret_cast<const f16x4*>(sp) + lane, cl = __builtin_bit_cast(f16x4, lo), ch = __builtin_bit_cast(f16x4, hi);
+                    const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+                    acc[0][nt] += __builtin_amdgcn_mfma_f32_16x16x16f16(cl, fp[0], z, 0, 0, 0) * p_down[0];
+                    acc[1][nt] += __builtin_amdgcn_mfma_f32_16x16x16f16(cl, fp[64], z, 0, 0, 0) * p_down[1] + __builtin_amdgcn_mfma_f32_16x16x16f16(ch, fp[128], z, 0, 0, 0) * p_down[2];
+                } else if constexpr (!STATE) {
 #pragma unroll
-                    for (int it = 0; it < 2; ++it) acc[it][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, both), fp[it], acc[it][nt], 0, 0, 0);
+                    for (int it = 0; it < 2; ++it) acc[it][nt] = mfma16<DT>(both, *reinterpret_cast<const s16x8*>(sp + (it * 64 + lane) * 8), acc[it][nt]);
                 }
-                float x[8], z[8], u[8];
+                float v[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float v = __uint_as_float((unsigned)(unsigned short)both[i] << 16) * (i < 4 ? w0[i & 3] : w1[i & 3]);
-                    x[i] = top16(v);
-                    z[i] = v - x[i];
-                    u[i] = z[i] - top16(z[i]);
+                for (int i = 0; i < 8; ++i) v[i] = widen<DT>((unsigned short)both[i]) * (i < 4 ? w0[i & 3] : w1[i & 3]);
+                if constexpr (H) {
+                    float most = 0.f, up;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[i]));
+                    most = fmaxf(most, __shfl_xor(most, 16));
+                    most = fmaxf(most, __shfl_xor(most, 32));
+                    fp16_scale(most, up, c_down[nt]);
+                    f16x8 x, z;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        x[i] = (_Float16)(v[i] * up);
+                        z[i] = (_Float16)(v[i] * up - (float)x[i]);
+                    }
+                    t0[nt] = __builtin_bit_cast(s16x8, x);
+                    t1[nt] = __builtin_bit_cast(s16x8, z);
+                } else {
+                    float x[8], z[8], u[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        x[i] = top16(v[i]);
+                        z[i] = v[i] - x[i];
+                        u[i] = z[i] - top16(z[i]);
+                    }
+                    t0[nt] = __builtin_bit_cast(s16x8, mk8(pack_hi16(x[0], x[1]), pack_hi16(x[2], x[3]), pack_hi16(x[4], x[5]), pack_hi16(x[6], x[7])));
+                    t1[nt] = __builtin_bit_cast(s16x8, mk8(pack_hi16(z[0], z[1]), pack_hi16(z[2], z[3]), pack_hi16(z[4], z[5]), pack_hi16(z[6], z[7])));
+                    t2[nt] = __builtin_bit_cast(s16x8, mk8(pack_hi16(u[0], u[1]), pack_hi16(u[2], u[3]), pack_hi16(u[4], u[5]), pack_hi16(u[6], u[7])));
                 }
-                t0[nt] = mk8(pack_hi16(x[0], x[1]), pack_hi16(x[2], x[3]), pack_hi16(x[4], x[5]), pack_hi16(x[6], x[7]));
-                t1[nt] = mk8(pack_hi16(z[0], z[1]), pack_hi16(z[2], z[3]), pack_hi16(z[4], z[5]), pack_hi16(z[6], z[7]));
-                t2[nt] = mk8(pack_hi16(u[0], u[1]), pack_hi16(u[2], u[3]), pack_hi16(u[4], u[5]), pack_hi16(u[6], u[7]));
             }
         }
         if constexpr (!STATE)
@@ -791,13 +854,23 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
         for (int kt = 0; kt < KA; ++kt) {
             const char* q = lb + (o4 ^ (32 * kt));
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)q), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(q + 16 * DA * 2));
-            const bf16x8 fb = __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            const s16x8 fb = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            if constexpr (H) {
+                f32x4 d[NT];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) W[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, t2[nt], W[kt][nt] * keep, 0, 0, 0);
+                for (int nt = 0; nt < NT; ++nt) d[nt] = mfma16<DT>(fb, t1[nt], (f32x4){0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) W[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, t1[nt], W[kt][nt], 0, 0, 0);
+                for (int nt = 0; nt < NT; ++nt) d[nt] = mfma16<DT>(fb, t0[nt], d[nt]);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) W[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, t0[nt], W[kt][nt], 0, 0, 0);
+                for (int nt = 0; nt < NT; ++nt) W[kt][nt] = W[kt][nt] * keep + d[nt] * c_down[nt];
+            } else {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) W[kt][nt] = mfma16<DT>(fb, t2[nt], W[kt][nt] * keep);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) W[kt][nt] = mfma16<DT>(fb, t1[nt], W[kt][nt]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) W[kt][nt] = mfma16<DT>(fb, t0[nt], W[kt][nt]);
+            }
         }
         if (i0 + CH < stop) stage(buf ^ 1);
     }
@@ -839,10 +912,17 @@ __global__ __launch_bounds__(256) void leaky_scan_kernel(float* __restrict__ ws,
     const float leak = exp2f(fmaxf(log_decay[bh % H], -1e30f) * 1.44269504088896341f * (float)seg);
     float* at = ws + (long long)blockIdx.y * nstate * per + (blockIdx.x * 256 + threadIdx.x) * 4;
     f32x4 s = *reinterpret_cast<const f32x4*>(at);
-    for (int k = 1; k < nstate; ++k) {
-        at += per;
-        s = s * leak + *reinterpret_cast<const f32x4*>(at);
-        *reinterpret_cast<f32x4*>(at) = s;
+    constexpr int U = 16;                    // states in flight: with one at a time the scan is their latencies (63 of them: 23 us)
+    for (int k = 1; k < nstate; k += U) {
+        f32x4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const f32x4*>(at + (long long)min(u + 1, nstate - k) * per);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            s = s * leak + v[u];
+            if (k + u < nstate) *reinterpret_cast<f32x4*>(at + (long long)(u + 1) * per) = s;
+        }
+        at += (long long)U * per;
     }
 }
 
@@ -893,7 +973,7 @@ template <int DT> struct LeakyShape {
             constexpr int DA = DAC.value, WV = WVC.value;
             const unsigned heads = (unsigned)(p.B * p.H * r.ncb);
             if (r.nseg > 1) {
-                if constexpr (DT == SS_SEQ_BF16) tile<DA, WV / 4, true>(heads * (r.nseg - 1), p, r, vec && vec_out, ws, s);
+                if constexpr (DT != SS_SEQ_F32) tile<DA, WV / 4, true>(heads * (r.nseg - 1), p, r, vec && vec_out, ws, s);
                 else leaky_chunk_kernel<DT, DA, WV, true><<<heads * (r.nseg - 1), 64 * WV, 0, s>>>(p, r, vec, vec_out, ws);
                 if (int rc = launched()) return rc;
                 if (!r.fold) {
@@ -901,7 +981,7 @@ template <int DT> struct LeakyShape {
                     if (int rc = launched()) return rc;
                 }
             }
-            if constexpr (DT == SS_SEQ_BF16) tile<DA, WV / 4, false>(heads * r.nseg, p, r, vec && vec_out, ws, s);
+            if constexpr (DT != SS_SEQ_F32) tile<DA, WV / 4, false>(heads * r.nseg, p, r, vec && vec_out, ws, s);
             else leaky_chunk_kernel<DT, DA, WV, false><<<heads * r.nseg, 64 * WV, 0, s>>>(p, r, vec, vec_out, ws);
             return launched();
         };
