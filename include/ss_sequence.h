@@ -35,10 +35,7 @@ int ss_seq_abi_version(void);
  * S_{-1} = s_in (NULL: zero).  reverse = 1 takes s_in UNDECAYED at its first step and hands s_out decayed once more (the adjoint of the forward map);
  * s_out (NULL: not wanted) is the state after the last valid step, s_in itself if there is none.  out rows of steps >= n are written as zeros.
  *
- *   forward        a, b, c = q, k, v     b_scale 1, o_scale scale
- *   gradient of q  a, b, c = g, v, k     b_scale 1, o_scale scale, s_in transposed
- *   gradient of k  a, b, c = v, g, q     b_scale scale, o_scale 1, reverse, s_in = gradient of the last state, transposed
- *   gradient of v  a, b, c = k, q, g     b_scale scale, o_scale 1, reverse, s_in = gradient of the last state; s_out = gradient of the first state
+ *   forward: a, b, c = q, k, v, b_scale 1, o_scale scale.  Each token gradient is such a map too (ss_seq_leaky_bwd).
  *
  * a [T][B][H / a_group][DA], b [T][B][H / b_group][DA], c [T][B][H / c_group][DC], out [T][B][H][DC] with the strides given; head h reads operand head
  * h / group.  s_in / s_out: [B][H] matrices DA x DC, element (i, j) at i * s_*_row + j * s_*_col, matrices DA * DC apart.  s_in may be s_out itself
@@ -63,6 +60,34 @@ struct ss_seq_leaky_desc {
 };
 long long ss_seq_leaky_ws_floats(const struct ss_seq_leaky_desc* d);
 int ss_seq_leaky(const struct ss_seq_leaky_desc* d, void* stream);
+
+/*
+ * Gradients of the forward map o = leaky(q, k, v) with H query heads on Hk key / value heads, from g = dL/do and g_last = dL/d(last state) (NULL: zero):
+ *
+ *      g_q  a, b, c = g, v, k   forward, from s_in transposed           o_scale scale
+ *      g_k  a, b, c = v, g, q   reverse, from g_last transposed         b_scale scale
+ *      g_v  a, b, c = k, q, g   reverse, from g_last                    b_scale scale;   g_s, the gradient of s_in, is its last state
+ *
+ * g_k, g_v: summed over the query heads that share a head (in fp32, in their order), rounded once.  g_q [T][B][H][Dk], g_k [T][B][Hk][Dk],
+ * g_v [T][B][Hk][Dv] contiguous in dtype, each NULL if not wanted; g_s fp32 [B][H][Dk][Dv] or NULL, wants g_v.  s_in: [B][H][Dk][Dv] contiguous or NULL, as
+ * the forward pass had it.  states: the workspace of the forward pass (same sizes, type and lengths), as it left it.
+ */
+struct ss_seq_leaky_bwd_desc {
+    unsigned size;                       /* sizeof(struct ss_seq_leaky_bwd_desc) */
+    int dtype, T, B, H, Hk, Dk, Dv;
+    float scale;
+    const void *q, *k, *v, *g;
+    long long q_t, q_b, q_h, k_t, k_b, k_h, v_t, v_b, v_h, g_t, g_b, g_h;
+    void *g_q, *g_k, *g_v;
+    const float* log_decay;
+    const int* lengths;
+    const float *s_in, *g_last;
+    float* g_s;
+    const float* states;                 /* NULL if ss_seq_leaky_ws_floats() was 0 */
+    float* ws;                           /* ss_seq_leaky_bwd_ws_floats() floats, 16-byte aligned, NULL if that is 0 */
+};
+long long ss_seq_leaky_bwd_ws_floats(const struct ss_seq_leaky_bwd_desc* d);
+int ss_seq_leaky_bwd(const struct ss_seq_leaky_bwd_desc* d, void* stream);
 
 /* out[r][j] = sum over the `group` consecutive rows of x [rows * group][D] (fp32), rounded once to dtype: the gradients of heads that several heads read */
 int ss_seq_group_sum(const float* x, void* out, long long rows, int group, int D, int dtype, void* stream);

@@ -29,7 +29,14 @@ class LeakyDesc(C.Structure):
                 [(n, C.c_int) for n in ('s_in_row', 's_in_col', 's_out_row', 's_out_col')] + [('ws', C.c_void_p)])
 
 
-EXPORTS = ('ss_seq_abi_version', 'ss_seq_leaky_ws_floats', 'ss_seq_leaky', 'ss_seq_group_sum', 'ss_seq_rms_norm_fwd', 'ss_seq_rms_norm_ws_floats',
+class LeakyBwdDesc(C.Structure):
+    """struct ss_seq_leaky_bwd_desc (include/ss_sequence.h)."""
+    _fields_ = ([('size', C.c_uint)] + [(n, C.c_int) for n in ('dtype', 'T', 'B', 'H', 'Hk', 'Dk', 'Dv')] + [('scale', C.c_float)] +
+                [(n, C.c_void_p) for n in 'qkvg'] + [(f'{n}_{s}', C.c_longlong) for n in 'qkvg' for s in 'tbh'] +
+                [(n, C.c_void_p) for n in ('g_q', 'g_k', 'g_v', 'log_decay', 'lengths', 's_in', 'g_last', 'g_s', 'states', 'ws')])
+
+
+EXPORTS = ('ss_seq_abi_version', 'ss_seq_leaky_ws_floats', 'ss_seq_leaky', 'ss_seq_leaky_bwd_ws_floats', 'ss_seq_leaky_bwd', 'ss_seq_group_sum', 'ss_seq_rms_norm_fwd', 'ss_seq_rms_norm_ws_floats',
            'ss_seq_rms_norm_bwd', 'ss_seq_rms_norm_int8', 'ss_seq_dequant_int8', 'ss_seq_int8_linear_ws_ints', 'ss_seq_int8_linear')
 
 
@@ -42,8 +49,9 @@ def lib():
         raise SSNeuronError(f'{LIB_PATH} not found: the HIP extension is not built.  Run `python -c "import __graft_entry__ as g; g.build()"` or '
                             f'`make -C stereospike_amd/csrc` (hipcc --offload-arch=gfx950).  There is no CPU fallback.')
     L = C.CDLL(LIB_PATH)
-    p, i32, i64, f32, desc = C.c_void_p, C.c_int, C.c_longlong, C.c_float, C.POINTER(LeakyDesc)
+    p, i32, i64, f32, desc, bdesc = C.c_void_p, C.c_int, C.c_longlong, C.c_float, C.POINTER(LeakyDesc), C.POINTER(LeakyBwdDesc)
     for name, res, args in (('ss_seq_abi_version', i32, []), ('ss_seq_leaky_ws_floats', i64, [desc]), ('ss_seq_leaky', i32, [desc, p]),
+                            ('ss_seq_leaky_bwd_ws_floats', i64, [bdesc]), ('ss_seq_leaky_bwd', i32, [bdesc, p]),
                             ('ss_seq_group_sum', i32, [p, p, i64, i32, i32, i32, p]),
                             ('ss_seq_rms_norm_fwd', i32, [p, i64, p, i64, p, p, p, p, i64, i32, f32, i32, p]),
                             ('ss_seq_rms_norm_ws_floats', i64, [i64, i32, i32]),
@@ -81,36 +89,44 @@ def _call(name, dev, *args):
         _check(rc, name)
 
 
-def leaky(a, b, c, out, log_decay, b_scale, o_scale, reverse=False, lengths=None, s_in=None, s_in_t=False, s_out=None, s_out_t=False):
-    """One leaky map (struct ss_seq_leaky_desc): a, b, c, out [T, B, heads, D] views with a contiguous last axis ([B, heads, D]: one step); states
-    [B, H, rows, columns] contiguous, or transposed (`*_t`: the matrix is stored [DC, DA])."""
-    sa, sb, sc, so = a.stride(), b.stride(), c.stride(), out.stride()
+def leaky(q, k, v, out, log_decay, scale, lengths=None, s_in=None, s_out=None):
+    """The forward map: q, k, v, out [T, B, heads, D] views with a contiguous last axis ([B, heads, D]: one step); states [B, H, Dk, Dv] contiguous.
+    Returns the workspace, which holds the states between segments (None where there are none)."""
+    sq, sk, sv, so = q.stride(), k.stride(), v.stride(), out.stride()
     if len(so) == 3:
-        T, (B, H, DC) = 1, out.shape
-        sa, sb, sc, so = (0, *sa), (0, *sb), (0, *sc), (0, *so)
+        T, (B, H, Dv) = 1, out.shape
+        sq, sk, sv, so = (0, *sq), (0, *sk), (0, *sv), (0, *so)
     else:
-        T, B, H, DC = out.shape
-    DA = a.shape[-1]
-    dt = DT_CODE[a.dtype]
-    d = LeakyDesc(_DESC_SIZE, dt, DT_CODE[out.dtype], T, B, H, DA, DC, reverse, b_scale, o_scale, a.data_ptr(), b.data_ptr(), c.data_ptr(), out.data_ptr(),
-                  sa[0], sa[1], sa[2], sb[0], sb[1], sb[2], sc[0], sc[1], sc[2], so[0], so[1], so[2], H // a.shape[-2], H // b.shape[-2], H // c.shape[-2],
-                  log_decay.data_ptr(), _p(lengths), _p(s_in), _p(s_out), 1 if s_in_t else DC, DA if s_in_t else 1, 1 if s_out_t else DC, DA if s_out_t else 1)
+        T, B, H, Dv = out.shape
+    dt, group = DT_CODE[q.dtype], H // k.shape[-2]
+    d = LeakyDesc(_DESC_SIZE, dt, dt, T, B, H, q.shape[-1], Dv, 0, 1.0, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                  sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], so[0], so[1], so[2], 1, group, group,
+                  log_decay.data_ptr(), _p(lengths), _p(s_in), _p(s_out), Dv, 1, Dv, 1)
     ref = C.byref(d)
+    ws = None
     if T > 1:
         n = (_lib or lib()).ss_seq_leaky_ws_floats(ref)
         if n:
-            ws = torch.empty(n, dtype=torch.float32, device=a.device)
+            ws = torch.empty(n, dtype=torch.float32, device=q.device)
             d.ws = ws.data_ptr()
-    _call('ss_seq_leaky', a.device, ref)
+    _call('ss_seq_leaky', q.device, ref)
+    return ws
 
 
-_DESC_SIZE = C.sizeof(LeakyDesc)
+def leaky_bwd(q, k, v, g, g_q, g_k, g_v, log_decay, scale, lengths, s_in, g_last, g_s, states):
+    """Gradients of `leaky` (None: not wanted); g_q, g_k, g_v contiguous."""
+    T, B, H, Dk = q.shape
+    d = LeakyBwdDesc(_BWD_SIZE, DT_CODE[q.dtype], T, B, H, k.shape[2], Dk, v.shape[3], scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
+                     *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride()[:3], _p(g_q), _p(g_k), _p(g_v), log_decay.data_ptr(), _p(lengths),
+                     _p(s_in), _p(g_last), _p(g_s), _p(states))
+    ref = C.byref(d)
+    n = (_lib or lib()).ss_seq_leaky_bwd_ws_floats(ref)
+    ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
+    d.ws = _p(ws)
+    _call('ss_seq_leaky_bwd', q.device, ref)
 
 
-def group_sum(x, out, group):
-    """x fp32 [rows * group, D] contiguous -> out [rows, D]: sums of `group` consecutive rows."""
-    D = x.shape[-1]
-    _call('ss_seq_group_sum', x.device, x.data_ptr(), out.data_ptr(), out.numel() // D, group, D, DT_CODE[out.dtype])
+_DESC_SIZE, _BWD_SIZE = C.sizeof(LeakyDesc), C.sizeof(LeakyBwdDesc)
 
 
 def rms_norm_fwd(x, residual, weight, y, total, rstd, eps):

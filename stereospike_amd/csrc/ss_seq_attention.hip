@@ -34,6 +34,24 @@ LeakyArgs args_of(const ss_seq_leaky_desc* d)
             d->s_in_row, d->s_in_col, d->s_out_row, d->s_out_col, d->out_dtype == SS_SEQ_F32};
 }
 
+bool bwd_ok(const ss_seq_leaky_bwd_desc* d)
+{
+    if (!d || d->size != sizeof(ss_seq_leaky_bwd_desc)) return false;
+    if (d->dtype != SS_SEQ_F32 && d->dtype != SS_SEQ_F16 && d->dtype != SS_SEQ_BF16) return false;
+    if (d->T < 1 || d->B < 1 || d->H < 1 || d->Hk < 1 || d->H % d->Hk || (long long)d->B * d->H > 65535) return false;
+    if (d->Dk < 1 || d->Dk > 256 || d->Dv < 1 || d->Dv > 256) return false;
+    if (!d->q || !d->k || !d->v || !d->g || !d->log_decay || (d->g_s && !d->g_v)) return false;
+    return true;
+}
+
+LeakyBwdArgs bwd_of(const ss_seq_leaky_bwd_desc* d)
+{
+    const int group = d->H / d->Hk;
+    return {d->T, d->B, d->H, d->Hk, d->Dk, d->Dv, d->scale, {d->q, d->q_t, d->q_b, d->q_h, 1}, {d->k, d->k_t, d->k_b, d->k_h, group},
+            {d->v, d->v_t, d->v_b, d->v_h, group}, {d->g, d->g_t, d->g_b, d->g_h, 1}, d->g_q, d->g_k, d->g_v, d->log_decay, d->lengths,
+            d->s_in, d->g_last, d->g_s, d->states, d->ws};
+}
+
 }  // namespace
 
 extern "C" {
@@ -51,6 +69,21 @@ int ss_seq_leaky(const ss_seq_leaky_desc* d, void* stream)
     const LeakyArgs p = args_of(d);
     hipStream_t s = static_cast<hipStream_t>(stream);
     return d->dtype == SS_SEQ_F32 ? ss_seq_leaky_f32(p, d->ws, s) : d->dtype == SS_SEQ_F16 ? ss_seq_leaky_f16(p, d->ws, s) : ss_seq_leaky_bf16(p, d->ws, s);
+}
+
+long long ss_seq_leaky_bwd_ws_floats(const ss_seq_leaky_bwd_desc* d)
+{
+    if (!bwd_ok(d)) return 0;
+    const LeakyBwdArgs p = bwd_of(d);
+    return d->dtype == SS_SEQ_F32 ? ss_seq_leaky_bwd_ws_f32(p) : d->dtype == SS_SEQ_F16 ? ss_seq_leaky_bwd_ws_f16(p) : ss_seq_leaky_bwd_ws_bf16(p);
+}
+
+int ss_seq_leaky_bwd(const ss_seq_leaky_bwd_desc* d, void* stream)
+{
+    if (!bwd_ok(d)) return SS_SEQ_EINVAL;
+    const LeakyBwdArgs p = bwd_of(d);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return d->dtype == SS_SEQ_F32 ? ss_seq_leaky_bwd_f32(p, s) : d->dtype == SS_SEQ_F16 ? ss_seq_leaky_bwd_f16(p, s) : ss_seq_leaky_bwd_bf16(p, s);
 }
 
 int ss_seq_group_sum(const float* x, void* out, long long rows, int group, int D, int dtype, void* stream)

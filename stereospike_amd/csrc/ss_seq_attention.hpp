@@ -23,6 +23,30 @@ struct LeakyArgs {
     int out_f32;
 };
 
+struct LeakyView {
+    const void* p;
+    long long t, b, h;                       // strides
+    int group;                               // query heads that read a head of it
+};
+struct LeakyBwdArgs {
+    int T, B, H, Hk, Dk, Dv;
+    float scale;
+    LeakyView q, k, v, g;
+    void *g_q, *g_k, *g_v;
+    const float* log_decay;
+    const int* lengths;
+    const float *s_in, *g_last;
+    float* g_s;
+    const float* states;
+    float* ws;
+};
+
+long long ss_seq_leaky_bwd_ws_f32(const LeakyBwdArgs&);
+long long ss_seq_leaky_bwd_ws_f16(const LeakyBwdArgs&);
+long long ss_seq_leaky_bwd_ws_bf16(const LeakyBwdArgs&);
+int ss_seq_leaky_bwd_f32(const LeakyBwdArgs&, hipStream_t);
+int ss_seq_leaky_bwd_f16(const LeakyBwdArgs&, hipStream_t);
+int ss_seq_leaky_bwd_bf16(const LeakyBwdArgs&, hipStream_t);
 long long ss_seq_leaky_ws_f32(const LeakyArgs&);
 long long ss_seq_leaky_ws_f16(const LeakyArgs&);
 long long ss_seq_leaky_ws_bf16(const LeakyArgs&);
@@ -192,7 +216,23 @@ struct LeakyPlan {
     int nseg, seg;                           // segments and their steps (a multiple of the chunk)
     int ncb;                                 // column blocks
     int fold;                                // the output pass joins the segments' states itself (no scan launch)
+    // the states between segments, as the state pass of this map or of the map with b and c exchanged (trans) left them: per head and column block of `dcb`
+    // columns, nseg - 1 matrices in accumulator order (wavefronts of 16 nt columns, `ka` row tiles)
+    int trans, ka, nt, dcb, sncb;
 };
+// the 16 x 16 tile of rows 16 rt, columns 16 ct of a state left in accumulator order: its first element
+__device__ __forceinline__ long long state_tile(const LeakyPlan& p, long long bh, int s, int rt, int ct)
+{
+    const int cb = 16 * ct / p.dcb, t = ct - cb * (p.dcb / 16), w = t / p.nt, n = t - w * p.nt;
+    return ((bh * p.sncb + cb) * (p.nseg - 1) + s) * (16ll * p.ka * p.dcb) + ((w * p.ka + rt) * p.nt + n) * 256;
+}
+// this lane's four values of the tile (rows 4 g .. + 3 of column l16) of the state that entered segment s + 1, or of its transpose
+__device__ __forceinline__ f32x4 state_read(const LeakyPlan& p, const float* __restrict__ ws, long long bh, int s, int rt, int ct, int lane)
+{
+    if (!p.trans) return *reinterpret_cast<const f32x4*>(ws + state_tile(p, bh, s, rt, ct) + lane * 4);
+    const float* at = ws + state_tile(p, bh, s, ct, rt) + ((lane & 15) >> 2) * 64 + (lane >> 4) * 16 + (lane & 3);
+    return (f32x4){at[0], at[4], at[8], at[12]};
+}
 
 __device__ __forceinline__ unsigned pack_hi16(float lo, float hi) { return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u); }
 __device__ __forceinline__ float top16(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFF0000u); }
@@ -239,8 +279,6 @@ __global__ __launch_bounds__(64 * WV, STATE ? (DA <= 128 ? 4 : 2) : DT == SS_SEQ
     // ---- the state that enters the segment
     f32x4 W[KA];
     {
-        const long long per = (long long)DA * DCB;
-        const float* mine = ws + ((long long)bh * plan.ncb + cb) * (plan.nseg - 1) * per + wv * KA * 256 + lane * 4;
         if (seg == 0) {
             const float* s_in = p.s_in ? p.s_in + (long long)bh * p.DA * p.DC : nullptr;
             const float first = p.reverse || n == 0 ? 1.f : exp2f(gl);
@@ -256,15 +294,12 @@ __global__ __launch_bounds__(64 * WV, STATE ? (DA <= 128 ? 4 : 2) : DT == SS_SEQ
             for (int kt = 0; kt < KA; ++kt)
 W[kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
         } else if (start < n) {
-            const int from = plan.fold ? 0 : seg - 1;
             const float leak = exp2f(gl * (float)plan.seg);
 #pragma unroll
-            for (int kt = 0; kt < KA; ++kt)
-W[kt] = *reinterpret_cast<const f32x4*>(mine + from * per + kt * 256);
-            for (int s = from + 1; s < seg; ++s)
+            for (int kt = 0; kt < KA; ++kt) W[kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            for (int s = plan.fold ? 0 : seg - 1; s < seg; ++s)
 #pragma unroll
-                for (int kt = 0; kt < KA; ++kt)
-W[kt] = W[kt] * leak + *reinterpret_cast<const f32x4*>(mine + s * per + kt * 256);
+                for (int kt = 0; kt < KA; ++kt) W[kt] = W[kt] * leak + state_read(plan, ws, bh, s, kt, col0 / 16, lane);
         }
     }
 
@@ -604,8 +639,6 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
     // ---- the state that enters the segment
     f32x4 W[KA][NT];
     {
-        const long long per = (long long)DA * DCB;
-        const float* mine = ws + ((long long)bh * plan.ncb + cb) * (plan.nseg - 1) * per + wv * KA * NT * 256 + lane * 4;
 #pragma unroll
         for (int kt = 0; kt < KA; ++kt)
 #pragma unroll
@@ -632,7 +665,7 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
 #pragma unroll
                 for (int kt = 0; kt < KA; ++kt)
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) W[kt][nt] = W[kt][nt] * leak + *reinterpret_cast<const f32x4*>(mine + s * per + (kt * NT + nt) * 256);
+                    for (int nt = 0; nt < NT; ++nt) W[kt][nt] = W[kt][nt] * leak + state_read(plan, ws, bh, s, kt, col0 / 16 + nt, lane);
         }
     }
 
@@ -931,62 +964,125 @@ constexpr int kStepsMax = 8;                 // calls of fewer steps walk the re
 
 template <int DT> struct LeakyShape {
     static constexpr int CH = 32;
-    static LeakyPlan plan(const LeakyArgs& p)
+    static int pad(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+    static int blocks(int d) { return d <= 128 ? 1 : 2; }
+    static LeakyPlan plan(int T, int B, int H, int DA, int DC)
     {
         LeakyPlan r;
-        r.ncb = p.DC <= 128 ? 1 : 2;
-        const int chunks = (p.T + CH - 1) / CH;
-        const long long base = (long long)p.B * p.H * r.ncb;
+        r.ncb = r.sncb = blocks(DC);
+        const int chunks = (T + CH - 1) / CH;
+        const long long base = (long long)B * H * r.ncb;
         // segments: until there are enough workgroups, but not under 256 steps, where a segment's state costs as much traffic as its steps
         long long nseg = (kLeakyTarget + base - 1) / base;
-        const int most = (p.T + 255) / 256;
+        const int most = (T + 255) / 256;
         if (nseg > most) nseg = most;
         if (nseg < 1) nseg = 1;
         const int per = (int)((chunks + nseg - 1) / nseg);
         r.seg = per * CH;
         r.nseg = (chunks + per - 1) / per;
         r.fold = r.nseg <= 5;
+        r.trans = 0;
+        r.ka = pad(DA) / 16;
+        r.dcb = DC <= 64 ? 64 : 128;
+        r.nt = DT == SS_SEQ_F32 || DC <= 64 ? 1 : 2;
         return r;
     }
-    static int da(const LeakyArgs& p) { return p.DA <= 64 ? 64 : p.DA <= 128 ? 128 : 256; }
-    static int dcb(const LeakyArgs& p) { return p.DC <= 64 ? 64 : 128; }
-    static long long ws_floats(const LeakyArgs& p)
+    static long long state_floats(int T, int B, int H, int DA, int DC)
     {
-        if (p.T < kStepsMax) return 0;
-        const LeakyPlan r = plan(p);
-        return (long long)p.B * p.H * r.ncb * (r.nseg - 1) * da(p) * dcb(p);
+        if (T < kStepsMax) return 0;
+        const LeakyPlan r = plan(T, B, H, DA, DC);
+        return (long long)B * H * (r.nseg - 1) * (r.ncb * r.dcb) * pad(DA);
     }
-    template <int DA, int NT, bool STATE> static void tile(unsigned grid, const LeakyArgs& p, const LeakyPlan& r, bool vec, float* ws, hipStream_t s)
+    template <int DA, int WV, bool STATE> static int launch(const LeakyArgs& p, const LeakyPlan& r, float* ws, hipStream_t s)
     {
-        if (vec) leaky_tile_kernel<DT, DA, NT, STATE, true><<<grid, 256, 0, s>>>(p, r, ws);
-        else leaky_tile_kernel<DT, DA, NT, STATE, false><<<grid, 256, 0, s>>>(p, r, ws);
+        auto ok = [&](const void* q, long long t, long long b, long long h) { return aligned(q, 16) && t % 8 == 0 && b % 8 == 0 && h % 8 == 0; };
+        const int vec = p.DA % 8 == 0 && p.DC % 8 == 0 && (STATE || ok(p.a, p.a_t, p.a_b, p.a_h)) && ok(p.b, p.b_t, p.b_b, p.b_h) && ok(p.c, p.c_t, p.c_b, p.c_h);
+        const int vec_out = STATE || (p.DC % 4 == 0 && p.o_t % 4 == 0 && p.o_b % 4 == 0 && p.o_h % 4 == 0 && aligned(p.out, 16));
+        const unsigned grid = (unsigned)(p.B * p.H * r.ncb) * (STATE ? r.nseg - 1 : r.nseg);
+        if constexpr (DT == SS_SEQ_F32) leaky_chunk_kernel<DT, DA, WV, STATE><<<grid, 64 * WV, 0, s>>>(p, r, vec, vec_out, ws);
+        else if (vec && vec_out) leaky_tile_kernel<DT, DA, WV / 4, STATE, true><<<grid, 256, 0, s>>>(p, r, ws);
+        else leaky_tile_kernel<DT, DA, WV / 4, STATE, false><<<grid, 256, 0, s>>>(p, r, ws);
+        return launched();
+    }
+    template <bool STATE> static int pass(const LeakyArgs& p, const LeakyPlan& r, float* ws, hipStream_t s)
+    {
+        auto by_dc = [&](auto DAC) { return p.DC <= 64 ? launch<DAC.value, 4, STATE>(p, r, ws, s) : launch<DAC.value, 8, STATE>(p, r, ws, s); };
+        return p.DA <= 64 ? by_dc(std::integral_constant<int, 64>()) : p.DA <= 128 ? by_dc(std::integral_constant<int, 128>()) : by_dc(std::integral_constant<int, 256>());
+    }
+    // the states that enter the segments, into ws (nothing where there is one segment)
+    static int states(const LeakyArgs& p, const LeakyPlan& r, float* ws, hipStream_t s)
+    {
+        if (r.nseg == 1) return SS_SEQ_OK;
+        if (!ws || !aligned(ws, 16)) return SS_SEQ_EINVAL;
+        if (int rc = pass<true>(p, r, ws, s)) return rc;
+        if (r.fold) return SS_SEQ_OK;
+        const int per = pad(p.DA) * r.dcb;
+        leaky_scan_kernel<<<dim3(per / 1024, (unsigned)(p.B * p.H * r.ncb)), 256, 0, s>>>(ws, p.log_decay, p.H, r.ncb, per, r.nseg - 1, r.seg);
+        return launched();
     }
     static int run(const LeakyArgs& p, float* ws, hipStream_t s)
     {
         if (p.T < kStepsMax) return p.out_f32 ? steps<DT, SS_SEQ_F32>(p, s) : steps<DT, DT>(p, s);
-        const LeakyPlan r = plan(p);
-        if (r.nseg > 1 && (!ws || !aligned(ws, 16))) return SS_SEQ_EINVAL;
-        auto ok = [&](const void* q, long long t, long long b, long long h) { return aligned(q, 16) && t % 8 == 0 && b % 8 == 0 && h % 8 == 0; };
-        const int vec = p.DA % 8 == 0 && p.DC % 8 == 0 && ok(p.a, p.a_t, p.a_b, p.a_h) && ok(p.b, p.b_t, p.b_b, p.b_h) && ok(p.c, p.c_t, p.c_b, p.c_h);
-        const int vec_out = p.DC % 4 == 0 && p.o_t % 4 == 0 && p.o_b % 4 == 0 && p.o_h % 4 == 0 && aligned(p.out, 16);
-        auto go = [&](auto DAC, auto WVC) {
-            constexpr int DA = DAC.value, WV = WVC.value;
-            const unsigned heads = (unsigned)(p.B * p.H * r.ncb);
-            if (r.nseg > 1) {
-                if constexpr (DT != SS_SEQ_F32) tile<DA, WV / 4, true>(heads * (r.nseg - 1), p, r, vec && vec_out, ws, s);
-                else leaky_chunk_kernel<DT, DA, WV, true><<<heads * (r.nseg - 1), 64 * WV, 0, s>>>(p, r, vec, vec_out, ws);
-                if (int rc = launched()) return rc;
-                if (!r.fold) {
-                    leaky_scan_kernel<<<dim3(DA * WV * 16 / 1024, heads), 256, 0, s>>>(ws, p.log_decay, p.H, r.ncb, DA * WV * 16, r.nseg - 1, r.seg);
-                    if (int rc = launched()) return rc;
-                }
-            }
-            if constexpr (DT != SS_SEQ_F32) tile<DA, WV / 4, false>(heads * r.nseg, p, r, vec && vec_out, ws, s);
-            else leaky_chunk_kernel<DT, DA, WV, false><<<heads * r.nseg, 64 * WV, 0, s>>>(p, r, vec, vec_out, ws);
-            return launched();
+        const LeakyPlan r = plan(p.T, p.B, p.H, p.DA, p.DC);
+        if (int rc = states(p, r, ws, s)) return rc;
+        return pass<false>(p, r, ws, s);
+    }
+
+    // ---- the gradients: three maps.  dq reads the forward pass's states transposed; dk and dv run backwards in time and share the states of (q, g).
+    static long long bwd_floats(const LeakyBwdArgs& d)
+    {
+        const long long part = d.H == d.Hk ? 0 : (long long)d.T * d.B * d.H * (d.Dk > d.Dv ? d.Dk : d.Dv);
+        return (part + 3) / 4 * 4 + state_floats(d.T, d.B, d.H, d.Dk, d.Dv);
+    }
+    static int bwd(const LeakyBwdArgs& d, hipStream_t s)
+    {
+        const int group = d.H / d.Hk;
+        const long long part = group == 1 ? 0 : ((long long)d.T * d.B * d.H * (d.Dk > d.Dv ? d.Dk : d.Dv) + 3) / 4 * 4;
+        float *shared = d.ws, *rstate = d.ws + part;
+        const bool tiles = d.T >= kStepsMax;
+        const LeakyPlan fwd = plan(d.T, d.B, d.H, d.Dk, d.Dv);
+        if (bwd_floats(d) && (!d.ws || !aligned(d.ws, 16))) return SS_SEQ_EINVAL;
+        if (tiles && fwd.nseg > 1 && d.g_q && (!d.states || !aligned(d.states, 16))) return SS_SEQ_EINVAL;
+        // contiguous results: [T][B][heads][D]
+        auto map = [&](int DA, int DC, int reverse, float bs, float os, const LeakyView& a, const LeakyView& b, const LeakyView& c, void* out, bool f32) {
+            LeakyArgs p{};
+            p.T = d.T; p.B = d.B; p.H = d.H; p.DA = DA; p.DC = DC; p.reverse = reverse; p.b_scale = bs; p.o_scale = os;
+            p.a = a.p; p.a_t = a.t; p.a_b = a.b; p.a_h = a.h; p.a_group = a.group;
+            p.b = b.p; p.b_t = b.t; p.b_b = b.b; p.b_h = b.h; p.b_group = b.group;
+            p.c = c.p; p.c_t = c.t; p.c_b = c.b; p.c_h = c.h; p.c_group = c.group;
+            p.out = out; p.o_h = DC; p.o_b = (long long)d.H * DC; p.o_t = p.o_b * d.B;
+            p.log_decay = d.log_decay; p.lengths = d.lengths; p.out_f32 = f32;
+            return p;
         };
-        auto by_dc = [&](auto DAC) { return p.DC <= 64 ? go(DAC, std::integral_constant<int, 4>()) : go(DAC, std::integral_constant<int, 8>()); };
-        return p.DA <= 64 ? by_dc(std::integral_constant<int, 64>()) : p.DA <= 128 ? by_dc(std::integral_constant<int, 128>()) : by_dc(std::integral_constant<int, 256>());
+        auto go = [&](const LeakyArgs& p, float* states, bool trans) {
+            if (!tiles) return p.out_f32 ? steps<DT, SS_SEQ_F32>(p, s) : steps<DT, DT>(p, s);
+            LeakyPlan r = fwd;                             // the forward pass's segments, whatever this map's own sizes
+            r.ncb = blocks(p.DC);
+            r.trans = trans;
+            return pass<false>(p, r, states, s);
+        };
+        auto sum = [&](void* out, int D) { return ss_seq_group_sum(shared, out, (long long)d.T * d.B * d.Hk, group, D, DT, s); };
+        if (d.g_q) {
+            LeakyArgs p = map(d.Dv, d.Dk, 0, 1.f, d.scale, d.g, d.v, d.k, d.g_q, DT == SS_SEQ_F32);
+            p.s_in = d.s_in; p.s_in_row = 1; p.s_in_col = d.Dv;
+            if (int rc = go(p, const_cast<float*>(d.states), true)) return rc;
+        }
+        if (!d.g_k && !d.g_v) return SS_SEQ_OK;
+        LeakyArgs pv = map(d.Dk, d.Dv, 1, d.scale, 1.f, d.k, d.q, d.g, group == 1 ? d.g_v : shared, group > 1 || DT == SS_SEQ_F32);
+        pv.s_in = d.g_last; pv.s_in_row = d.Dv; pv.s_in_col = 1;
+        pv.s_out = d.g_s; pv.s_out_row = d.Dv; pv.s_out_col = 1;
+        if (tiles) if (int rc = states(pv, fwd, rstate, s)) return rc;
+        if (d.g_v) {
+            if (int rc = go(pv, rstate, false)) return rc;
+            if (group > 1) if (int rc = sum(d.g_v, d.Dv)) return rc;
+        }
+        if (d.g_k) {
+            LeakyArgs p = map(d.Dv, d.Dk, 1, d.scale, 1.f, d.v, d.g, d.q, group == 1 ? d.g_k : shared, group > 1 || DT == SS_SEQ_F32);
+            p.s_in = d.g_last; p.s_in_row = 1; p.s_in_col = d.Dv;
+            if (int rc = go(p, rstate, true)) return rc;
+            if (group > 1) if (int rc = sum(d.g_k, d.Dk)) return rc;
+        }
+        return SS_SEQ_OK;
     }
 };
 

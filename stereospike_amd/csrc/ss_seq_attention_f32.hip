@@ -1,5 +1,7 @@
 // ss_seq_attention_f32.hip — leaky attention on fp32 operands (ss_seq_attention.hpp).
 #include "ss_seq_attention.hpp"
 
-long long ss_seq_leaky_ws_f32(const LeakyArgs& p) { return LeakyShape<SS_SEQ_F32>::ws_floats(p); }
+long long ss_seq_leaky_ws_f32(const LeakyArgs& p) { return LeakyShape<SS_SEQ_F32>::state_floats(p.T, p.B, p.H, p.DA, p.DC); }
 int ss_seq_leaky_f32(const LeakyArgs& p, float* ws, hipStream_t s) { return LeakyShape<SS_SEQ_F32>::run(p, ws, s); }
+long long ss_seq_leaky_bwd_ws_f32(const LeakyBwdArgs& d) { return LeakyShape<SS_SEQ_F32>::bwd_floats(d); }
+int ss_seq_leaky_bwd_f32(const LeakyBwdArgs& d, hipStream_t s) { return LeakyShape<SS_SEQ_F32>::bwd(d, s); }

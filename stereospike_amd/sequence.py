@@ -75,46 +75,36 @@ class _LeakyAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, state, log_decay, scale, lengths):
         ctx.set_materialize_grads(False)
         q, k, v = _last_contiguous(q), _last_contiguous(k), _last_contiguous(v)
-        T, B, H, Dk = q.shape
+        B, H, Dk = q.shape[1:]
         Dv = v.shape[3]
-        state_c = None if state is None else state.contiguous()
-        out = torch.empty((T, B, H, Dv), dtype=q.dtype, device=q.device)
+        if state is not None:
+            state = state.contiguous()
+        out = torch.empty((q.shape[0], B, H, Dv), dtype=q.dtype, device=q.device)
         last = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=q.device)
-        _seqlib.leaky(q, k, v, out, log_decay, 1.0, scale, lengths=lengths, s_in=state_c, s_out=last)
-        ctx.save_for_backward(q, k, v, state_c, log_decay, lengths)
-        ctx.scale = scale
+        states = _seqlib.leaky(q, k, v, out, log_decay, scale, lengths, state, last)
+        if any(ctx.needs_input_grad):
+            ctx.save_for_backward(q, k, v, state, log_decay, lengths, states)
+            ctx.scale = scale
         return out, last
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g, g_last):
-        q, k, v, state, log_decay, lengths = ctx.saved_tensors
-        need_q, need_k, need_v, need_s = ctx.needs_input_grad[:4]
-        g = torch.zeros((*q.shape[:3], v.shape[3]), dtype=q.dtype, device=q.device) if g is None else _last_contiguous(g)
-        g_last = None if g_last is None else g_last.float().contiguous()
-        H, Hk, scale = q.shape[2], k.shape[2], ctx.scale
-        g_q = g_k = g_v = g_s = None
-        if need_q:
-            g_q = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            _seqlib.leaky(g, v, k, g_q, log_decay, 1.0, scale, lengths=lengths, s_in=state, s_in_t=True)
+        return _attention_grads_once(ctx, g, g_last) if torch.is_grad_enabled() else _attention_grads(ctx, g, g_last)
 
-        def shared(like, a, b, c, **kw):
-            # heads that read the same key / value head: their gradients in fp32, summed in the heads' order, rounded once
-            full = like.shape[:2] + (H, like.shape[3])
-            part = torch.empty(full, dtype=like.dtype if H == Hk else torch.float32, device=like.device)
-            _seqlib.leaky(a, b, c, part, log_decay, scale, 1.0, reverse=True, lengths=lengths, s_in=g_last, **kw)
-            if H == Hk:
-                return part
-            out = torch.empty(like.shape, dtype=like.dtype, device=like.device)
-            _seqlib.group_sum(part, out, H // Hk)
-            return out
 
-        if need_k:
-            g_k = shared(k, v, g, q, s_in_t=True)
-        if need_v or need_s:
-            g_s = torch.empty((*q.shape[1:3], q.shape[3], v.shape[3]), dtype=torch.float32, device=q.device) if need_s else None
-            g_v = shared(v, k, q, g, s_out=g_s)
-        return g_q, g_k, g_v if need_v else None, g_s, None, None, None
+def _attention_grads(ctx, g, g_last):
+    q, k, v, state, log_decay, lengths, states = ctx.saved_tensors
+    need_q, need_k, need_v, need_s = ctx.needs_input_grad[:4]
+    g = torch.zeros((*q.shape[:3], v.shape[3]), dtype=q.dtype, device=q.device) if g is None else _last_contiguous(g)
+    if g_last is not None:
+        g_last = g_last.contiguous()
+    g_q, g_k, g_v = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None for t, need in ((q, need_q), (k, need_k), (v, need_v or need_s)))
+    g_s = torch.empty(state.shape, dtype=torch.float32, device=q.device) if need_s else None
+    _seqlib.leaky_bwd(q, k, v, g, g_q, g_k, g_v, log_decay, ctx.scale, lengths, state, g_last, g_s, states)
+    return g_q, g_k, g_v if need_v else None, g_s, None, None, None
+
+
+_attention_grads_once = once_differentiable(_attention_grads)        # under create_graph: a second derivative is refused, not silently zero
 
 
 def leaky_attention(q_seq: torch.Tensor, k_seq: torch.Tensor, v_seq: torch.Tensor, log_decay: torch.Tensor, scale: Optional[float] = None,
@@ -152,7 +142,7 @@ def leaky_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
         raise SSNeuronError('state: tensor must be contiguous (it is updated in place)')
     out = torch.empty((B, H, Dv), dtype=q.dtype, device=q.device)
     if B:
-        _seqlib.leaky(_last_contiguous(q), _last_contiguous(k), _last_contiguous(v), out, log_decay.contiguous(), 1.0, Dk ** -0.5 if scale is None else float(scale),
+        _seqlib.leaky(_last_contiguous(q), _last_contiguous(k), _last_contiguous(v), out, log_decay.contiguous(), Dk ** -0.5 if scale is None else float(scale),
                       s_in=state, s_out=state)
         if not state.is_inference():
             torch.autograd.graph.increment_version(state)  # an autograd graph that saved this state must notice
@@ -202,17 +192,23 @@ class _AddRMSNorm(torch.autograd.Function):
         return (y, total) if residual is not None else y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_y, g_sum=None):
-        h, weight, rstd = ctx.saved_tensors
-        need_x, need_r, need_w, _ = ctx.needs_input_grad
-        g_h = torch.empty(ctx.shape, dtype=h.dtype, device=h.device)
-        g_w = torch.empty_like(weight) if need_w else None
-        if rstd.shape[0]:
-            _seqlib.rms_norm_bwd(None if g_y is None else g_y.contiguous(), None if g_sum is None else g_sum.contiguous(), _rows(h), weight, rstd, g_h, g_w)
-        elif need_w:
-            g_w.zero_()
-        return g_h if need_x else None, g_h if need_r else None, g_w, None
+        return _norm_grads_once(ctx, g_y, g_sum) if torch.is_grad_enabled() else _norm_grads(ctx, g_y, g_sum)
+
+
+def _norm_grads(ctx, g_y, g_sum):
+    h, weight, rstd = ctx.saved_tensors
+    need_x, need_r, need_w, _ = ctx.needs_input_grad
+    g_h = torch.empty(ctx.shape, dtype=h.dtype, device=h.device)
+    g_w = torch.empty_like(weight) if need_w else None
+    if rstd.shape[0]:
+        _seqlib.rms_norm_bwd(None if g_y is None else g_y.contiguous(), None if g_sum is None else g_sum.contiguous(), _rows(h), weight, rstd, g_h, g_w)
+    elif need_w:
+        g_w.zero_()
+    return g_h if need_x else None, g_h if need_r else None, g_w, None
+
+
+_norm_grads_once = once_differentiable(_norm_grads)
 
 
 def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
