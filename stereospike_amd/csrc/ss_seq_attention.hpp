@@ -959,7 +959,6 @@ __global__ __launch_bounds__(256) void leaky_scan_kernel(float* __restrict__ ws,
     }
 }
 
-constexpr int kLeakyTarget = 512;            // workgroups wanted: two on each of 256 CUs (prompt of 4096 steps, 64 heads: 256 129 us, 384 122, 512 108, 768 122, 1024 140)
 constexpr int kStepsMax = 8;                 // calls of fewer steps walk the recurrence
 
 template <int DT> struct LeakyShape {
@@ -970,14 +969,22 @@ template <int DT> struct LeakyShape {
     {
         LeakyPlan r;
         r.ncb = r.sncb = blocks(DC);
+        // Segments: the count with the least estimated time, in chunks.  A round of workgroups (two on a CU; one for fp32, whose matrix instructions one workgroup
+        // fills) takes a segment's chunks and two for its state; the state pass half of that; joining costs half a chunk per state in the output pass up to 5
+        // segments, else a scan; each further launch two.  (64 heads, 4096 steps, bf16: 4 segments 123 us, 8 108, 16 135; 48 heads, 777 steps, fp32 training:
+        // 4 segments 262 us, 5 215, 7 268.)
         const int chunks = (T + CH - 1) / CH;
-        const long long base = (long long)B * H * r.ncb;
-        // segments: until there are enough workgroups, but not under 256 steps, where a segment's state costs as much traffic as its steps
-        long long nseg = (kLeakyTarget + base - 1) / base;
-        const int most = (T + 255) / 256;
-        if (nseg > most) nseg = most;
-        if (nseg < 1) nseg = 1;
-        const int per = (int)((chunks + nseg - 1) / nseg);
+        const double base = (double)B * H * r.ncb, slots = DT == SS_SEQ_F32 ? 256. : 512.;
+        int best = 1;
+        double least = 0.;
+        for (int n = 1; n <= 128 && n <= chunks; ++n) {
+            const double per = (chunks + n - 1) / n;
+            double t = ceil(base * n / slots) * (per + 2. + (n <= 5 ? 0.5 * (n - 1) : 0.));
+            if (n > 1) t += ceil(base * (n - 1) / slots) * (0.5 * per + 1.) + 2.;
+            if (n > 5) t += 4. + n / 16.;
+            if (n == 1 || t < least) { best = n; least = t; }
+        }
+        const int per = (chunks + best - 1) / best;
         r.seg = per * CH;
         r.nseg = (chunks + per - 1) / per;
         r.fold = r.nseg <= 5;

@@ -480,6 +480,54 @@ def test_training_block_gradients():
         assert (a.cpu().double() - b).norm() <= 5000 * U * b.norm()
 
 
+def test_nothing_to_do():
+    """No step, no stream, no row: the shapes, and no launch."""
+    q, g = torch.zeros(3, 2, 4, 8, device=DEV), torch.zeros(4, device=DEV)
+    k, v = torch.zeros(3, 2, 2, 8, device=DEV), torch.zeros(3, 2, 2, 6, device=DEV)
+    s = torch.ones(2, 4, 8, 6, device=DEV)
+    o, last = sequence.leaky_attention(q[:0], k[:0], v[:0], g, state=s, return_state=True)
+    assert o.shape == (0, 2, 4, 6) and torch.equal(last, s)
+    assert sequence.leaky_attention(q[:, :0], k[:, :0], v[:, :0], g).shape == (3, 0, 4, 6)
+    assert sequence.leaky_attention_step(q[0, :0], k[0, :0], v[0, :0], g, s[:0]).shape == (0, 4, 6)
+    x, w = torch.zeros(3, 8, device=DEV, requires_grad=True), torch.ones(8, device=DEV, requires_grad=True)
+    y, _ = sequence.add_rms_norm(x[:0], w)
+    assert y.shape == (0, 8) and not torch.autograd.grad(y.sum(), w)[0].any()
+    assert [t.shape for t in sequence.add_rms_norm_int8(x[:0], w, x[:0])] == [(0, 8), (0,), (0, 8)]
+    c = torch.zeros(0, 8, dtype=torch.int8, device=DEV)
+    assert sequence.int8_linear(c, torch.ones(0, device=DEV), torch.zeros(5, 8, dtype=torch.int8, device=DEV), torch.ones(5, device=DEV)).shape == (0, 5)
+    assert sequence.dequantize_int8(c, torch.ones(0, device=DEV)).shape == (0, 8)
+
+
+def test_refusals_on_the_device():
+    """The library hands unfit operands back before it launches; the error names the operand."""
+    q, g = torch.zeros(3, 2, 4, 8, device=DEV), torch.zeros(4, device=DEV)
+    for bad, what in (((q, q[:2], q, g), 'k: expected shape'), ((q, q.half(), q, g), 'k: expected'), ((q, q, q.cpu(), g), 'v'), ((q, q, q, g[:2]), 'log_decay'),
+                      ((q, q, q, g.clone().requires_grad_()), 'no gradient'), ((q, q, None, g), 'v')):
+        with pytest.raises(sequence.SSNeuronError, match=what):
+            sequence.leaky_attention(*bad)
+    with pytest.raises(sequence.SSNeuronError, match='contiguous'):
+        sequence.leaky_attention_step(q[0], q[0], q[0], g, torch.zeros(2, 4, 8, 8, device=DEV).transpose(2, 3))
+    with pytest.raises(sequence.SSNeuronError, match='weight'):
+        sequence.add_rms_norm(q, torch.ones(8, device=DEV).half())
+    with pytest.raises(sequence.SSNeuronError, match='scales'):
+        sequence.int8_linear(q.to(torch.int8), torch.ones(3, device=DEV), torch.zeros(5, 8, dtype=torch.int8, device=DEV), torch.ones(5, device=DEV))
+
+
+def test_gradients_are_not_differentiated_again():
+    q = torch.randn(4, 1, 1, 8, device=DEV, requires_grad=True)
+    o = sequence.leaky_attention(q, q, q, torch.zeros(1, device=DEV))
+    first, = torch.autograd.grad(o.square().sum(), q, create_graph=True)
+    plain, = torch.autograd.grad(sequence.leaky_attention(q, q, q, torch.zeros(1, device=DEV)).square().sum(), q)
+    assert torch.equal(first, plain)
+    with pytest.raises(RuntimeError, match='differentiate twice'):
+        first.sum().backward()
+    w = torch.ones(8, device=DEV, requires_grad=True)
+    y, _ = sequence.add_rms_norm(q, w)
+    first, = torch.autograd.grad(y.square().sum(), w, create_graph=True)
+    with pytest.raises(RuntimeError, match='differentiate twice'):
+        first.sum().backward()
+
+
 def test_other_stream_and_repeat():
     """On a side stream, and twice on the same inputs: the same bits."""
     q, k, v, decay, s, _ = (t.to(DEV) if t is not None else None for t in leaky_case(300, 2, 4, 2, 64, 64, torch.bfloat16, True, False))
