@@ -19,7 +19,7 @@ bool desc_ok(const ss_seq_leaky_desc* d)
     if (!d || d->size != sizeof(ss_seq_leaky_desc)) return false;
     if (d->dtype != SS_SEQ_F32 && d->dtype != SS_SEQ_F16 && d->dtype != SS_SEQ_BF16) return false;
     if (d->out_dtype != d->dtype && d->out_dtype != SS_SEQ_F32) return false;
-    if (d->T < 1 || d->B < 1 || d->H < 1 || (long long)d->B * d->H > 65535 || d->DA < 1 || d->DA > 256 || d->DC < 1 || d->DC > 256) return false;
+    if (d->T < 1 || d->T > (1 << 30) || d->B < 1 || d->H < 1 || (long long)d->B * d->H > 65535 || d->DA < 1 || d->DA > 256 || d->DC < 1 || d->DC > 256) return false;
     if (d->a_group < 1 || d->b_group < 1 || d->c_group < 1 || d->H % d->a_group || d->H % d->b_group || d->H % d->c_group) return false;
     if (!d->a || !d->b || !d->c || !d->out || !d->log_decay) return false;
     if (d->T > 1 && d->s_in && d->s_in == d->s_out) return false;        // a segment may read the first state after another wrote the last
@@ -38,7 +38,7 @@ bool bwd_ok(const ss_seq_leaky_bwd_desc* d)
 {
     if (!d || d->size != sizeof(ss_seq_leaky_bwd_desc)) return false;
     if (d->dtype != SS_SEQ_F32 && d->dtype != SS_SEQ_F16 && d->dtype != SS_SEQ_BF16) return false;
-    if (d->T < 1 || d->B < 1 || d->H < 1 || d->Hk < 1 || d->H % d->Hk || (long long)d->B * d->H > 65535) return false;
+    if (d->T < 1 || d->T > (1 << 30) || d->B < 1 || d->H < 1 || d->Hk < 1 || d->H % d->Hk || (long long)d->B * d->H > 65535) return false;
     if (d->Dk < 1 || d->Dk > 256 || d->Dv < 1 || d->Dv > 256) return false;
     if (!d->q || !d->k || !d->v || !d->g || !d->log_decay || (d->g_s && !d->g_v)) return false;
     return true;

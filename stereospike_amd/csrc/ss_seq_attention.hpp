@@ -521,6 +521,7 @@ W[kt] *= keep;
                 }
             }
         } else {
+            bool wild = false;
 #pragma unroll
             for (int jt = 0; jt < IT; ++jt) {
                 const f32x4 w = *reinterpret_cast<const f32x4*>(rw + 16 * jt + 4 * g);
@@ -528,14 +529,21 @@ W[kt] *= keep;
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
 fc[r] = sc[(16 * jt + 4 * g + r) * SC + wv * 16 + l16];
-                if constexpr (!STATE)
+                float fin[4];                                            // without what is not finite: 0 * NaN would reach steps before it
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const bool odd = !(fabsf(fc[r]) < __builtin_inff());
+                    fin[r] = odd ? 0.f : fc[r];
+                    wild = wild || odd;
+                }
+                if constexpr (!STATE) {
 #pragma unroll
                     for (int it = jt; it < IT; ++it) {
                         const f32x4 fp = *reinterpret_cast<const f32x4*>(sp + ((it * IT + jt) * 64 + lane) * 4);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-acc[it] = __builtin_amdgcn_mfma_f32_16x16x4f32(fc[r], fp[r], acc[it], 0, 0, 0);
+                        for (int r = 0; r < 4; ++r) acc[it] = __builtin_amdgcn_mfma_f32_16x16x4f32(fin[r], fp[r], acc[it], 0, 0, 0);
                     }
+                }
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
 fc[r] *= w[r];
@@ -547,6 +555,19 @@ fc[r] *= w[r];
 W[kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb, fc[r], W[kt], 0, 0, 0);
                     }
             }
+            if (!STATE && __any(wild))                                   // rare: those terms one by one, where j <= i
+#pragma unroll 1
+                for (int j = 0; j < CH; ++j)
+#pragma unroll
+                    for (int it = 0; it < IT; ++it) {
+                        if (j > 16 * it + l16) continue;
+                        const float pij = sp[((it * IT + (j >> 4)) * 64 + 16 * (j >> 2 & 3) + l16) * 4 + (j & 3)];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float c = sc[j * SC + wv * 16 + 4 * g + r];
+                            if (!(fabsf(c) < __builtin_inff())) acc[it][r] += pij * c;
+                        }
+                    }
         }
         if constexpr (!STATE)
 #pragma unroll
@@ -829,6 +850,7 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
         // (2) and (4) share the wavefront's columns of c
         s16x8 t0[NT], t1[NT], t2[NT];
         float c_down[NT];
+        bool wild = false;
         {
             const f32x4 w0 = *reinterpret_cast<const f32x4*>(rw + 4 * g), w1 = *reinterpret_cast<const f32x4*>(rw + 16 + 4 * g);
 #pragma unroll
@@ -836,14 +858,18 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
                 const char* q = lc + (oc ^ (32 * nt));
                 const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)q), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(q + 16 * DCB * 2));
                 const s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                // what is not finite (exponent all ones) is left out of the product (2): 0 * NaN would reach steps before it
+                constexpr int EXP = H ? 0x7C00 : 0x7F80;
+                const s16x8 odd = (both & (short)EXP) == (short)EXP, fin = both & ~odd;
+                wild = wild || __builtin_reduce_or(odd) != 0;
                 if constexpr (!STATE && H) {               // a product of 16 steps for each tile of P, its scale undone as it is added
-                    const f16x4 *fp = reinterpret_cast<const f16x4*>(sp) + lane, cl = __builtin_bit_cast(f16x4, lo), ch = __builtin_bit_cast(f16x4, hi);
+                    const f16x4 *fp = reinterpret_cast<const f16x4*>(sp) + lane, cl = __builtin_bit_cast(f16x4, (s16x4)__builtin_shufflevector(fin, fin, 0, 1, 2, 3)), ch = __builtin_bit_cast(f16x4, (s16x4)__builtin_shufflevector(fin, fin, 4, 5, 6, 7));
                     const f32x4 z = {0.f, 0.f, 0.f, 0.f};
                     acc[0][nt] += __builtin_amdgcn_mfma_f32_16x16x16f16(cl, fp[0], z, 0, 0, 0) * p_down[0];
                     acc[1][nt] += __builtin_amdgcn_mfma_f32_16x16x16f16(cl, fp[64], z, 0, 0, 0) * p_down[1] + __builtin_amdgcn_mfma_f32_16x16x16f16(ch, fp[128], z, 0, 0, 0) * p_down[2];
                 } else if constexpr (!STATE) {
 #pragma unroll
-                    for (int it = 0; it < 2; ++it) acc[it][nt] = mfma16<DT>(both, *reinterpret_cast<const s16x8*>(sp + (it * 64 + lane) * 8), acc[it][nt]);
+                    for (int it = 0; it < 2; ++it) acc[it][nt] = mfma16<DT>(fin, *reinterpret_cast<const s16x8*>(sp + (it * 64 + lane) * 8), acc[it][nt]);
                 }
                 float v[8];
 #pragma unroll
@@ -877,6 +903,23 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
                 }
             }
         }
+        if (!STATE && __any(wild))                                       // rare: those terms one by one, where j <= i
+#pragma unroll 1
+            for (int j = 0; j < CH; ++j)
+#pragma unroll
+                for (int it = 0; it < 2; ++it) {
+                    if (j > 16 * it + l16) continue;
+                    const int jl = 16 * (j >> 2 & 3) + l16;              // the lane that holds P_ij
+                    const float pij = H ? widen<DT>(sp[((it + (j >> 4)) * 64 + jl) * 4 + (j & 3)]) * p_down[it + (j >> 4)] : widen<DT>(sp[(it * 64 + jl) * 8 + (j >> 4) * 4 + (j & 3)]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int col = wv * 16 * NT + 16 * nt + 4 * g + r;
+                            const float c = widen<DT>(*reinterpret_cast<const unsigned short*>(lc + j * DCB * 2 + (((col >> 3) ^ swz<SC>(j)) << 4) + ((col & 7) << 1)));
+                            if (!(fabsf(c) < __builtin_inff())) acc[it][nt][r] += pij * c;
+                        }
+                }
         if constexpr (!STATE)
 #pragma unroll
             for (int it = 0; it < 2; ++it)
@@ -941,9 +984,9 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
 // ws[s] (what segment s adds to the state) -> the state that enters segment s + 1
 __global__ __launch_bounds__(256) void leaky_scan_kernel(float* __restrict__ ws, const float* __restrict__ log_decay, int H, int ncb, int per, int nstate, int seg)
 {
-    const int bh = blockIdx.y / ncb;
+    const unsigned parts = per / 1024, head = blockIdx.x / parts, bh = head / ncb;
     const float leak = exp2f(fmaxf(log_decay[bh % H], -1e30f) * 1.44269504088896341f * (float)seg);
-    float* at = ws + (long long)blockIdx.y * nstate * per + (blockIdx.x * 256 + threadIdx.x) * 4;
+    float* at = ws + (long long)head * nstate * per + ((blockIdx.x - head * parts) * 256 + threadIdx.x) * 4;
     f32x4 s = *reinterpret_cast<const f32x4*>(at);
     constexpr int U = 16;                    // states in flight: with one at a time the scan is their latencies (63 of them: 23 us)
     for (int k = 1; k < nstate; k += U) {
@@ -1024,7 +1067,7 @@ template <int DT> struct LeakyShape {
         if (int rc = pass<true>(p, r, ws, s)) return rc;
         if (r.fold) return SS_SEQ_OK;
         const int per = pad(p.DA) * r.dcb;
-        leaky_scan_kernel<<<dim3(per / 1024, (unsigned)(p.B * p.H * r.ncb)), 256, 0, s>>>(ws, p.log_decay, p.H, r.ncb, per, r.nseg - 1, r.seg);
+        leaky_scan_kernel<<<(unsigned)(p.B * p.H * r.ncb) * (per / 1024), 256, 0, s>>>(ws, p.log_decay, p.H, r.ncb, per, r.nseg - 1, r.seg);
         return launched();
     }
     static int run(const LeakyArgs& p, float* ws, hipStream_t s)

@@ -21,7 +21,7 @@ typedef std::optional<Tensor> Maybe;
 
 namespace {
 
-constexpr int64_t kMaxHead = 256, kMaxWidth = 16384, kMaxK = 131071, kMaxStates = 65535;
+constexpr int64_t kMaxHead = 256, kMaxWidth = 16384, kMaxK = 131071, kMaxStates = 65535, kMaxSteps = 1 << 30, kMaxSide = 1 << 30;
 
 struct SeqError : std::runtime_error { using std::runtime_error::runtime_error; };
 
@@ -70,6 +70,7 @@ bool attention_ok(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
     if (k.device() != q.device() || v.device() != q.device() || k.scalar_type() != dt || v.scalar_type() != dt) return false;
     for (int64_t i = 0; i < dims - 2; ++i) if (k.size(i) != q.size(i) || v.size(i) != q.size(i)) return false;
     if (k.size(-2) != Hk || k.size(-1) != Dk || H < 1 || Hk < 1 || H % Hk || Dk < 1 || Dk > kMaxHead || Dv < 1 || Dv > kMaxHead || B * H > kMaxStates) return false;
+    if (dims == 4 && q.size(0) > kMaxSteps) return false;
     if (!is(log_decay, q, at::kFloat, {H})) return false;
     if (state.defined() && !is(state, q, at::kFloat, {B, H, Dk, Dv})) return false;
     return !lengths.defined() || is(lengths, q, at::kInt, {B});
@@ -300,7 +301,7 @@ std::optional<Tensor> int8_linear(const Tensor& codes, const Tensor& scales, con
     const Tensor& bias = given(bias0);
     if (!codes.is_cuda() || codes.scalar_type() != at::kChar || codes.dim() < 1 || weight.dim() != 2 || code_of(out_dtype) < 0) return std::nullopt;
     const int64_t N = weight.size(0), K = weight.size(1);
-    if (!is(weight, codes, at::kChar, {N, K}) || codes.size(-1) != K || N < 1 || K < 1 || K > kMaxK) return std::nullopt;
+    if (!is(weight, codes, at::kChar, {N, K}) || codes.size(-1) != K || N < 1 || N > kMaxSide || K < 1 || K > kMaxK || codes.numel() / K > kMaxSide) return std::nullopt;
     if (!is(scales, codes, at::kFloat, codes.sizes().slice(0, codes.dim() - 1)) || !is(weight_scale, codes, at::kFloat, {N})) return std::nullopt;
     if (bias.defined() && !is(bias, codes, at::kFloat, {N})) return std::nullopt;
     if (records({scales, weight_scale, bias})) return std::nullopt;

@@ -71,6 +71,8 @@ def _refuse_attention(q, k, v, log_decay, state, lengths, lead):
         raise SSNeuronError(f'head sizes {Dk} and {Dv}: 1 .. {_seqlib.MAX_HEAD_DIM} are implemented')
     if B * H > _seqlib.MAX_STATES:
         raise SSNeuronError(f'B * heads = {B * H}: at most {_seqlib.MAX_STATES} states in one call')
+    if lead == 2 and q.shape[0] > _seqlib.MAX_STEPS:
+        raise SSNeuronError(f'{q.shape[0]} steps: at most {_seqlib.MAX_STEPS} in one call')
     _operand(log_decay, 'log_decay', dev, torch.float32, (H,))
     if lead == 2 and log_decay.requires_grad and torch.is_grad_enabled():
         raise SSNeuronError('log_decay: the decay of a head is a constant of the layer (as tau of a LIFNode); it has no gradient — pass log_decay.detach()')
@@ -183,6 +185,8 @@ def int8_linear(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor,
             _operand(bias, 'bias', dev, torch.float32, (N,))
         if not 1 <= K <= _seqlib.MAX_INT8_K or N < 1:
             raise SSNeuronError(f'weight: [N, K] = [{N}, {K}]; N >= 1 and 1 <= K <= {_seqlib.MAX_INT8_K} (sums stay within 32 bits) are implemented')
+        if max(N, codes.numel() // K) > _seqlib.MAX_SIDE:
+            raise SSNeuronError(f'{codes.numel() // K} rows, {N} channels: at most {_seqlib.MAX_SIDE} of each')
         if out_dtype not in _FLOATS:
             raise SSNeuronError(f'out_dtype: expected float32, float16 or bfloat16, got {out_dtype}')
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (scales, weight_scale, bias)):

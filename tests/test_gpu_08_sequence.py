@@ -127,6 +127,40 @@ def test_leaky_attention_long(dtype):
     leaky_check(5000, 1, 2, 2, 16, 24, dtype, state=True, ragged=False, grads=False)
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('what', [math.nan, math.inf])
+def test_what_is_not_finite_reaches_no_earlier_step(dtype, what):
+    """A value that is not finite at step 37 of 100 (inside a tile): outputs and states before it are bit for bit those without it; the gradients behind a gradient
+    that is not finite likewise."""
+    q, k, v, decay, _, _ = (t.to(DEV) if t is not None else None for t in leaky_case(100, 2, 2, 2, 24, 40, dtype, False, False, seed=11))
+    decay = torch.tensor([-0.01, -0.2], device=DEV)
+    clean = sequence.leaky_attention(q, k, v, decay)
+    for operand in range(3):
+        use = [q.clone(), k.clone(), v.clone()]
+        use[operand][37, 0, 1, 5] = what
+        o = sequence.leaky_attention(*use, decay)
+        assert torch.equal(o[:37], clean[:37]) and torch.equal(o[:, 1], clean[:, 1]) and torch.equal(o[:, 0, 0], clean[:, 0, 0])
+        assert not torch.isfinite(o[37, 0, 1]).all()
+        if operand == 0:                                                        # a query reads, and leaves nothing behind
+            assert torch.equal(o[38:], clean[38:])
+        else:
+            assert not torch.isfinite(o[38, 0, 1]).all()
+        if operand == 2:                                                        # a value's column is its own
+            rest = torch.arange(40, device=DEV) != 5
+            assert torch.equal(o[..., rest], clean[..., rest])
+    use = [t.clone().requires_grad_() for t in (q, k, v)]
+    g = normal(gen(12), 100, 2, 2, 40, dtype=dtype).to(DEV)
+    o = sequence.leaky_attention(*use, decay)
+    want = torch.autograd.grad(o, use, g, retain_graph=True)
+    bad = g.clone()
+    bad[37, 0, 1, 5] = what
+    got = torch.autograd.grad(o, use, bad)
+    assert torch.equal(got[0][:37], want[0][:37]) and torch.equal(got[0][38:], want[0][38:])
+    for a, b in zip(got[1:], want[1:]):
+        assert torch.equal(a[38:], b[38:]) and torch.equal(a[:, 1], b[:, 1])
+        assert not torch.isfinite(a[37, 0, 1]).all()
+
+
 def test_leaky_gradient_against_differences():
     """The map is linear in each operand: a central difference of the definition along a direction is its derivative, up to the definition's fp64."""
     q, k, v, decay, s, n = leaky_case(70, 3, 2, 1, 12, 10, torch.float32, True, True, seed=5)
