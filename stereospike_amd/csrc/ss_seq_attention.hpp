@@ -730,33 +730,54 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
         put(at, rb, std::integral_constant<int, SA>());
         put(at + BA, rc, std::integral_constant<int, SC>());
     };
-    auto store = [&](int i, int col, const f32x4& v) {                   // four columns of step i
-        if (i >= p.T) return;
-        const bool live = i < n;
-        const long long t = live && p.reverse ? n - 1 - i : i;
-        const long long at = b * p.o_b + h * p.o_h + t * p.o_t + col;
-        const f32x4 o = live ? v : (f32x4){0.f, 0.f, 0.f, 0.f};
-        if (p.out_f32) {
-            float* q = static_cast<float*>(p.out) + at;
-            if constexpr (VEC) { if (col < p.DC) *reinterpret_cast<f32x4*>(q) = o; }
-            else
+    auto put_out = [&](void* q, const f32x4& o) {
+        if (p.out_f32) *static_cast<f32x4*>(q) = o;
+        else *static_cast<u16x4*>(q) = (u16x4){narrow<DT>(o[0]), narrow<DT>(o[1]), narrow<DT>(o[2]), narrow<DT>(o[3])};
+    };
+    // the chunk's outputs: a lane has four columns of steps 16 it + l16
+    auto store = [&](int i0, const f32x4 (&v)[2][NT]) {
+        const int es = p.out_f32 ? 4 : 2;
+        char* out = static_cast<char*>(p.out) + (b * p.o_b + h * p.o_h + col0) * es;
+        if (VEC && i0 + CH <= stop && col0 + 16 * NT <= p.DC) {
+            char* to = out + (long long)(p.reverse ? n - CH - i0 : i0) * p.o_t * es;
+            const unsigned step = (unsigned)p.o_t * es;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) if (col + e < p.DC) q[e] = o[e];
-        } else {
-            unsigned short* q = static_cast<unsigned short*>(p.out) + at;
-            if constexpr (VEC) {
-                if (col < p.DC) *reinterpret_cast<u16x4*>(q) = (u16x4){narrow<DT>(o[0]), narrow<DT>(o[1]), narrow<DT>(o[2]), narrow<DT>(o[3])};
-            } else
+            for (int it = 0; it < 2; ++it)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) if (col + e < p.DC) q[e] = narrow<DT>(o[e]);
+                for (int nt = 0; nt < NT; ++nt)
+                    put_out(to + ((unsigned)(p.reverse ? CH - 1 - 16 * it - l16 : 16 * it + l16) * step + (unsigned)((16 * nt + 4 * g) * es)), v[it][nt]);
+            return;
         }
+#pragma unroll
+        for (int it = 0; it < 2; ++it)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const int i = i0 + 16 * it + l16, col = 16 * nt + 4 * g, left = p.DC - col0 - col;
+                if (i >= p.T || left <= 0) continue;
+                const bool live = i < n;                                 // steps behind the last: zeros
+                char* q = out + ((long long)(live && p.reverse ? n - 1 - i : i) * p.o_t + col) * es;
+                const f32x4 o = live ? v[it][nt] : (f32x4){0.f, 0.f, 0.f, 0.f};
+                if constexpr (VEC) put_out(q, o);
+                else
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (e < left) {
+                            if (p.out_f32) reinterpret_cast<float*>(q)[e] = o[e];
+                            else reinterpret_cast<unsigned short*>(q)[e] = narrow<DT>(o[e]);
+                        }
+            }
     };
 
     if constexpr (!STATE) { if (tid < 128) *reinterpret_cast<f32x4*>(sp + tid * 8) = (f32x4){0.f, 0.f, 0.f, 0.f}; }      // the half of P above the diagonal stays zero
     if (tid < CH) rw[tid] = exp2f(gl * (float)(CH - tid)) * p.b_scale;
-    float row_scale[2];                                                  // lambda^i o_scale of this lane's steps
+    // lambda^i o_scale of this lane's steps; lambda^(i - j) and both scales for this lane's entries of the wavefront's tile of P (0: above the diagonal)
+    const int it1 = (wv + 1) >> 1, jt1 = wv >> 1;
+    float row_scale[2], p_scale[4];
 #pragma unroll
     for (int it = 0; it < 2; ++it) row_scale[it] = exp2f(gl * (float)(16 * it + l16)) * p.o_scale;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) p_scale[r] = exp2f(gl * (float)max(16 * (it1 - jt1) + l16 - 4 * g - r, 0)) * p.b_scale * p.o_scale;
+    const float keep_all = exp2f(gl * (float)CH);
     // byte offsets of this lane's operands in a buffer; 32 (64) bytes of the row further on is an XOR of the slot
     const int fa = swz<SA>(l16), o1 = l16 * DA * 2 + ((g ^ fa) << 4), o3 = l16 * DA * 2 + (((g >> 1) ^ fa) << 4) + ((g & 1) << 3);
     const int tr = 4 * g + (l16 >> 2), y = (l16 & 3) >> 1;
@@ -781,7 +802,7 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
         if constexpr (!STATE) {
             // (1) wavefronts 0 .. 2: the tiles (0, 0), (1, 0), (1, 1)
             if (wv < 3) {
-                const int it = (wv + 1) >> 1, jt = wv >> 1;
+                const int it = it1, jt = jt1;
                 f32x4 s = {0.f, 0.f, 0.f, 0.f}, s2 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int k = 0; k < DA / 32; ++k) {
@@ -793,8 +814,7 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
                 s += s2;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int d = 16 * (it - jt) + l16 - 4 * g - r;      // i - j
-                    s[r] = d < 0 ? 0.f : s[r] * (exp2f(gl * (float)d) * p.b_scale * p.o_scale);
+                    s[r] = 16 * (it - jt) + l16 - 4 * g - r < 0 ? 0.f : s[r] * p_scale[r];
                 }
                 if constexpr (H) {
                     float up, down;
@@ -858,10 +878,18 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
                 const char* q = lc + (oc ^ (32 * nt));
                 const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)q), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(q + 16 * DCB * 2));
                 const s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                // what is not finite (exponent all ones) is left out of the product (2): 0 * NaN would reach steps before it
-                constexpr int EXP = H ? 0x7C00 : 0x7F80;
-                const s16x8 odd = (both & (short)EXP) == (short)EXP, fin = both & ~odd;
-                wild = wild || __builtin_reduce_or(odd) != 0;
+                // what is not finite (exponent all ones: one more carries into the sign's place) is left out of the product (2): 0 * NaN would reach steps before it
+                s16x8 fin = both;
+                if constexpr (!STATE) {
+                    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+                    constexpr unsigned EXP = H ? 0x7C007C00u : 0x7F807F80u, ONE = H ? 0x04000400u : 0x00800080u;
+                    const u32x4 c2 = __builtin_bit_cast(u32x4, both), t = (c2 & EXP) + ONE;
+                    if (__any(((t[0] | t[1] | t[2] | t[3]) & 0x80008000u) != 0)) {
+                        wild = true;
+                        const s16x8 odd = (both & (short)EXP) == (short)EXP;
+                        fin = both & ~odd;
+                    }
+                }
                 if constexpr (!STATE && H) {               // a product of 16 steps for each tile of P, its scale undone as it is added
                     const f16x4 *fp = reinterpret_cast<const f16x4*>(sp) + lane, cl = __builtin_bit_cast(f16x4, (s16x4)__builtin_shufflevector(fin, fin, 0, 1, 2, 3)), ch = __builtin_bit_cast(f16x4, (s16x4)__builtin_shufflevector(fin, fin, 4, 5, 6, 7));
                     const f32x4 z = {0.f, 0.f, 0.f, 0.f};
@@ -903,7 +931,7 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
                 }
             }
         }
-        if (!STATE && __any(wild))                                       // rare: those terms one by one, where j <= i
+        if (!STATE && wild)                                       // rare: those terms one by one, where j <= i
 #pragma unroll 1
             for (int j = 0; j < CH; ++j)
 #pragma unroll
@@ -920,12 +948,8 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
                             if (!(fabsf(c) < __builtin_inff())) acc[it][nt][r] += pij * c;
                         }
                 }
-        if constexpr (!STATE)
-#pragma unroll
-            for (int it = 0; it < 2; ++it)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) store(i0 + 16 * it + l16, col0 + 16 * nt + 4 * g, acc[it][nt]);
-        const float keep = exp2f(gl * (float)e);
+        if constexpr (!STATE) store(i0, acc);
+        const float keep = e == CH ? keep_all : exp2f(gl * (float)e);
 #pragma unroll
         for (int kt = 0; kt < KA; ++kt) {
             const char* q = lb + (o4 ^ (32 * kt));
@@ -961,11 +985,12 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
     } else {
         // steps of the segment behind the stream's last: zeros (the loop above has written its own chunks to their end)
         const int end = start + plan.seg < p.T ? start + plan.seg : p.T;
-        for (; i0 < end; i0 += CH)
+        f32x4 none[2][NT];
 #pragma unroll
-            for (int it = 0; it < 2; ++it)
+        for (int it = 0; it < 2; ++it)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) store(i0 + 16 * it + l16, col0 + 16 * nt + 4 * g, (f32x4){0.f, 0.f, 0.f, 0.f});
+            for (int nt = 0; nt < NT; ++nt) none[it][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (; i0 < end; i0 += CH) store(i0, none);
         if (p.s_out && ((start < n && n <= start + plan.seg) || (n == 0 && seg == 0))) {
             float* s_out = p.s_out + (long long)bh * p.DA * p.DC;
 #pragma unroll
@@ -1046,7 +1071,8 @@ template <int DT> struct LeakyShape {
     template <int DA, int WV, bool STATE> static int launch(const LeakyArgs& p, const LeakyPlan& r, float* ws, hipStream_t s)
     {
         auto ok = [&](const void* q, long long t, long long b, long long h) { return aligned(q, 16) && t % 8 == 0 && b % 8 == 0 && h % 8 == 0; };
-        const int vec = p.DA % 8 == 0 && p.DC % 8 == 0 && (STATE || ok(p.a, p.a_t, p.a_b, p.a_h)) && ok(p.b, p.b_t, p.b_b, p.b_h) && ok(p.c, p.c_t, p.c_b, p.c_h);
+        const auto near = [](long long t) { return t >= 0 && t < (1 << 24); };  // 32 rows within 32-bit offsets
+        const int vec = near(p.a_t) && near(p.b_t) && near(p.c_t) && near(p.o_t) && p.DA % 8 == 0 && p.DC % 8 == 0 && (STATE || ok(p.a, p.a_t, p.a_b, p.a_h)) && ok(p.b, p.b_t, p.b_b, p.b_h) && ok(p.c, p.c_t, p.c_b, p.c_h);
         const int vec_out = STATE || (p.DC % 4 == 0 && p.o_t % 4 == 0 && p.o_b % 4 == 0 && p.o_h % 4 == 0 && aligned(p.out, 16));
         const unsigned grid = (unsigned)(p.B * p.H * r.ncb) * (STATE ? r.nseg - 1 : r.nseg);
         if constexpr (DT == SS_SEQ_F32) leaky_chunk_kernel<DT, DA, WV, STATE><<<grid, 64 * WV, 0, s>>>(p, r, vec, vec_out, ws);
