@@ -66,8 +66,7 @@ template <int DT, int ODT, int R, bool V4> __global__ __launch_bounds__(256) voi
     const int bh = blockIdx.y, b = bh / p.H, h = bh % p.H, j0 = blockIdx.x * 64 + 4 * x;
     int n = p.T;
     if (p.lengths) { n = p.lengths[b]; n = n < 0 ? 0 : n > p.T ? p.T : n; }
-    // lambda S as S + S * expm1(g) while lambda is over a half: a rounded lambda near 1 would drift over many steps (2^-25 of it each)
-    const float g_h = fmaxf(p.log_decay[h], -1e30f), lam = expf(g_h), leak = g_h > -0.69f ? expm1f(g_h) : lam, kept = g_h > -0.69f ? 1.f : 0.f;
+    const float lam = expf(p.log_decay[h]);
     const elem_t<DT>* pa = static_cast<const elem_t<DT>*>(p.a) + b * p.a_b + (h / p.a_group) * p.a_h;
     const elem_t<DT>* pb = static_cast<const elem_t<DT>*>(p.b) + b * p.b_b + (h / p.b_group) * p.b_h;
     const elem_t<DT>* pc = static_cast<const elem_t<DT>*>(p.c) + b * p.c_b + (h / p.c_group) * p.c_h;
@@ -97,7 +96,7 @@ template <int DT, int ODT, int R, bool V4> __global__ __launch_bounds__(256) voi
         for (int r = 0; r < R; ++r) {
             const int row = g + 16 * r;                    // rows behind DA: sa, sb are zero there
             f32x4 s = S[r];
-            if (leaks) s = s * leak + s * kept;
+            if (leaks) s = s * lam;
             s += sb[row] * c;
             o += sa[row] * s;
             S[r] = s;
@@ -143,7 +142,7 @@ template <int DT, int ODT, int R> __global__ __launch_bounds__(256) void leaky_s
     const float* from = live ? s_in : s_in - j0;
 #pragma unroll
     for (int r = 0; r < R; ++r) S[r] = *reinterpret_cast<const f32x4*>(from + (long long)min(g + 16 * r, p.DA - 1) * p.s_in_row);
-    const float lam = expf(fmaxf(p.log_decay[h], -1e30f));
+    const float lam = expf(p.log_decay[h]);
     if (tid < p.DA) {
         sa[tid] = widen<DT>(static_cast<const elem_t<DT>*>(p.a)[b * p.a_b + (h / p.a_group) * p.a_h + tid]) * p.o_scale;
         sb[tid] = widen<DT>(static_cast<const elem_t<DT>*>(p.b)[b * p.b_b + (h / p.b_group) * p.b_h + tid]) * p.b_scale;
@@ -212,6 +211,9 @@ template <int DT, int ODT> int steps(const LeakyArgs& p, hipStream_t s)
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef s16x4 __attribute__((address_space(3))) * lds_s16x4;
 
+// log2 of lambda; minus infinity becomes a number, so that lambda^0 is 1
+__device__ __forceinline__ float log2_decay(float log_decay) { return (log_decay < -1e30f ? -1e30f : log_decay) * 1.44269504088896341f; }
+
 struct LeakyPlan {
     int nseg, seg;                           // segments and their steps (a multiple of the chunk)
     int ncb;                                 // column blocks
@@ -247,20 +249,19 @@ __device__ __forceinline__ unsigned round_pk(float lo, float hi)
     return __builtin_bit_cast(unsigned, (bf16x2){(__bf16)lo, (__bf16)hi});
 }
 
-template <int DT, int DA, int WV, bool STATE>
-__global__ __launch_bounds__(64 * WV, STATE ? (DA <= 128 ? 4 : 2) : DT == SS_SEQ_BF16 ? (DA == 64 && WV == 4 ? 3 : 2) : (DA <= 128 ? 4 : 2)) void leaky_chunk_kernel(const LeakyArgs p, const LeakyPlan plan, const int vec, const int vec_out, float* __restrict__ ws)
+// The tile form on fp32 operands: the 16x16x4 fp32 matrix instructions, a workgroup of WV (4 or 8) wavefronts with 16 columns each, two workgroups on a CU.
+// Bound by those instructions (157 TFLOP/s), so the 16-row tiles behind DA and the wavefronts behind DC are left out.
+template <int DA, int WV, bool STATE>
+__global__ __launch_bounds__(64 * WV, DA == 64 || (DA == 128 && WV == 8) ? 4 : 2) void leaky_chunk_kernel(const LeakyArgs p, const LeakyPlan plan, const int vec, const int vec_out, float* __restrict__ ws)
 {
-    constexpr bool BF = DT == SS_SEQ_BF16;
-    constexpr int CH = BF ? 64 : 32, NTH = 64 * WV, DCB = 16 * WV, IT = CH / 16, KA = DA / 16;
-    typedef typename std::conditional<BF, unsigned short, float>::type LT;
-    constexpr int SA = DA + (BF ? 8 : 4), SC = DCB + (BF ? 8 : 4);       // LDS rows 16 bytes longer than a power of two
-    constexpr int NA = CH * DA / 8, NC = CH * DCB / 8, GA = (NA + NTH - 1) / NTH, GC = NC / NTH;       // 8-element granules, and those of a thread
-    __shared__ __attribute__((aligned(16))) LT sa[STATE ? 8 : CH * SA];
-    __shared__ __attribute__((aligned(16))) LT sb[CH * SA];
-    __shared__ __attribute__((aligned(16))) LT sc[CH * SC];
-    __shared__ __attribute__((aligned(16))) LT sp[STATE ? 8 : (BF ? IT * (IT / 2) * 64 * 8 : IT * IT * 64 * 4)];
+    constexpr int CH = 32, NTH = 64 * WV, DCB = 16 * WV, KA = DA / 16;
+    constexpr int SA = DA + 4, SC = DCB + 4;                             // LDS rows 16 bytes longer than a power of two
+    constexpr int GA = CH * DA / 4 / NTH, GC = CH * DCB / 4 / NTH;       // 16-byte granules of a thread
+    __shared__ __attribute__((aligned(16))) float sa[STATE ? 8 : CH * SA];
+    __shared__ __attribute__((aligned(16))) float sb[CH * SA];
+    __shared__ __attribute__((aligned(16))) float sc[CH * SC];
+    __shared__ __attribute__((aligned(16))) float sp[STATE ? 8 : 3 * 64 * 4];                // P: the tiles (0, 0), (1, 0), (1, 1)
     __shared__ __attribute__((aligned(16))) float rw[CH];                // lambda^(e - j) b_scale of the chunk's steps
-    typedef Pack<DT, 8> G;
 
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g = lane >> 4;
     const int cb = blockIdx.x % plan.ncb, rest = blockIdx.x / plan.ncb;
@@ -269,130 +270,86 @@ __global__ __launch_bounds__(64 * WV, STATE ? (DA <= 128 ? 4 : 2) : DT == SS_SEQ
     if (p.lengths) { n = p.lengths[b]; n = n < 0 ? 0 : n > p.T ? p.T : n; }
     const int start = seg * plan.seg, stop = n < start + plan.seg ? n : start + plan.seg;      // this segment's valid steps
     if (STATE && n <= start + plan.seg) return;                          // no later segment reads this one's state
-    const float gl = fmaxf(p.log_decay[h], -1e30f) * 1.44269504088896341f;                     // log2 lambda
-    const int c0 = cb * DCB, col0 = c0 + wv * 16;
-    const elem_t<DT>* pa = static_cast<const elem_t<DT>*>(p.a) + b * p.a_b + (h / p.a_group) * p.a_h;
-    const elem_t<DT>* pb = static_cast<const elem_t<DT>*>(p.b) + b * p.b_b + (h / p.b_group) * p.b_h;
-    const elem_t<DT>* pc = static_cast<const elem_t<DT>*>(p.c) + b * p.c_b + (h / p.c_group) * p.c_h + c0;
+    const float gl = log2_decay(p.log_decay[h]);
+    const int c0 = cb * DCB, col0 = c0 + wv * 16, ka = (p.DA + 15) / 16;
+    const bool on = col0 < p.DC;                                         // this wavefront has columns
+    const float* pa = static_cast<const float*>(p.a) + b * p.a_b + (h / p.a_group) * p.a_h;
+    const float* pb = static_cast<const float*>(p.b) + b * p.b_b + (h / p.b_group) * p.b_h;
+    const float* pc = static_cast<const float*>(p.c) + b * p.c_b + (h / p.c_group) * p.c_h + c0;
     const int dc = p.DC - c0 < DCB ? p.DC - c0 : DCB;
 
     // ---- the state that enters the segment
     f32x4 W[KA];
-    {
-        if (seg == 0) {
-            const float* s_in = p.s_in ? p.s_in + (long long)bh * p.DA * p.DC : nullptr;
+#pragma unroll
+    for (int kt = 0; kt < KA; ++kt) W[kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    if (seg == 0) {
+        if (p.s_in) {
+            const float* s_in = p.s_in + (long long)bh * p.DA * p.DC;
             const float first = p.reverse || n == 0 ? 1.f : exp2f(gl);
 #pragma unroll
             for (int kt = 0; kt < KA; ++kt)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int i = 16 * kt + 4 * g + r, j = col0 + l16;
-                        W[kt][r] = s_in && i < p.DA && j < p.DC ? s_in[i * p.s_in_row + j * p.s_in_col] * first : 0.f;
-                    }
-        } else if constexpr (STATE) {
+                for (int r = 0; r < 4; ++r) {
+                    const int i = 16 * kt + 4 * g + r, j = col0 + l16;
+                    const bool in = i < p.DA && j < p.DC;
+                    const float v = s_in[in ? i * p.s_in_row + j * p.s_in_col : 0];
+                    W[kt][r] = in ? v * first : 0.f;
+                }
+        }
+    } else if (!STATE && start < n && on) {
+        const float leak = exp2f(gl * (float)plan.seg);
+        for (int s = plan.fold ? 0 : seg - 1; s < seg; ++s)
 #pragma unroll
             for (int kt = 0; kt < KA; ++kt)
-W[kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
-        } else if (start < n) {
-            const float leak = exp2f(gl * (float)plan.seg);
-#pragma unroll
-            for (int kt = 0; kt < KA; ++kt) W[kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
-            for (int s = plan.fold ? 0 : seg - 1; s < seg; ++s)
-#pragma unroll
-                for (int kt = 0; kt < KA; ++kt) W[kt] = W[kt] * leak + state_read(plan, ws, bh, s, kt, col0 / 16, lane);
-        }
+                if (kt < ka) W[kt] = W[kt] * leak + state_read(plan, ws, bh, s, kt, col0 / 16, lane);
     }
 
     // ---- staging: global -> registers (one chunk ahead) -> LDS
-    G ra[STATE ? 1 : GA], rb[GA], rc[GC];
-    auto fetch = [&](const elem_t<DT>* base, long long st, int i, int q, int d, G& o) {
-        const bool in = i < stop && 8 * q < d;
-        if (vec) {
-            if (in) o = *reinterpret_cast<const G*>(base + (long long)(p.reverse ? n - 1 - i : i) * st + 8 * q);
-            else
+    f32x4 ra[STATE ? 1 : GA], rb[GA], rc[GC];
+    auto fetch = [&](f32x4* dst, const float* base, long long st, int i0, int d, auto SPRC) {
+        constexpr int SPR = SPRC.value;                                  // granules of a row
 #pragma unroll
-                for (int e = 0; e < 8; ++e) o.v[e] = 0;
-        } else {
-            const elem_t<DT>* src = base + (long long)(p.reverse ? n - 1 - i : i) * st + 8 * q;
+        for (int u = 0; u < CH * SPR / NTH; ++u) {
+            const int x = tid + NTH * u, q = x % SPR, i = i0 + x / SPR;
+            const float* src = base + (long long)(p.reverse ? n - 1 - i : i) * st + 4 * q;
+            dst[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            if (i < stop && 4 * q < d) {
+                if (vec) dst[u] = *reinterpret_cast<const f32x4*>(src);
+                else
 #pragma unroll
-            for (int e = 0; e < 8; ++e) { o.v[e] = 0; if (in && 8 * q + e < d) o.v[e] = src[e]; }
-        }
-    };
-    auto load = [&](int i0) {
-#pragma unroll
-        for (int u = 0; u < GA; ++u) {
-            const int id = tid + NTH * u, row = id / (DA / 8), q = id % (DA / 8);
-            if (NA % NTH && id >= NA) break;
-            if constexpr (!STATE) fetch(pa, p.a_t, i0 + row, q, p.DA, ra[u]);
-            fetch(pb, p.b_t, i0 + row, q, p.DA, rb[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < GC; ++u) {
-            const int id = tid + NTH * u, row = id / (DCB / 8), q = id % (DCB / 8);
-            fetch(pc, p.c_t, i0 + row, q, dc, rc[u]);
-        }
-    };
-    auto put = [&](LT* dst, const G& v, int row, int q) {                // rows of a, b: operand order within blocks of 32 (bf16)
-        if constexpr (BF) {
-            LT* at = dst + row * SA + (q >> 2) * 32 + ((q & 3) >> 1) * 4 + (q & 1) * 16;
-            *reinterpret_cast<u16x4*>(at) = (u16x4){v.v[0], v.v[1], v.v[2], v.v[3]};
-            *reinterpret_cast<u16x4*>(at + 8) = (u16x4){v.v[4], v.v[5], v.v[6], v.v[7]};
-        } else {
-            LT* at = dst + row * SA + 8 * q;
-            *reinterpret_cast<f32x4*>(at) = (f32x4){widen<DT>(v.v[0]), widen<DT>(v.v[1]), widen<DT>(v.v[2]), widen<DT>(v.v[3])};
-            *reinterpret_cast<f32x4*>(at + 4) = (f32x4){widen<DT>(v.v[4]), widen<DT>(v.v[5]), widen<DT>(v.v[6]), widen<DT>(v.v[7])};
-        }
-    };
-    auto stage = [&]() {
-#pragma unroll
-        for (int u = 0; u < GA; ++u) {
-            const int id = tid + NTH * u, row = id / (DA / 8), q = id % (DA / 8);
-            if (NA % NTH && id >= NA) break;
-            if constexpr (!STATE) put(sa, ra[u], row, q);
-            put(sb, rb[u], row, q);
-        }
-#pragma unroll
-        for (int u = 0; u < GC; ++u) {
-            const int id = tid + NTH * u, row = id / (DCB / 8), q = id % (DCB / 8);
-            if constexpr (BF) *reinterpret_cast<G*>(sc + row * SC + 8 * q) = rc[u];
-            else {
-                *reinterpret_cast<f32x4*>(sc + row * SC + 8 * q) = (f32x4){widen<DT>(rc[u].v[0]), widen<DT>(rc[u].v[1]), widen<DT>(rc[u].v[2]), widen<DT>(rc[u].v[3])};
-                *reinterpret_cast<f32x4*>(sc + row * SC + 8 * q + 4) = (f32x4){widen<DT>(rc[u].v[4]), widen<DT>(rc[u].v[5]), widen<DT>(rc[u].v[6]), widen<DT>(rc[u].v[7])};
+                    for (int e = 0; e < 4; ++e) if (4 * q + e < d) dst[u][e] = src[e];
             }
         }
     };
-    auto store = [&](int i, int it_nt_col, const f32x4& v) {             // four columns of step i
-        if (i >= p.T) return;
-        const bool live = i < n;
-        const long long t = live && p.reverse ? n - 1 - i : i;
-        const long long at = b * p.o_b + h * p.o_h + t * p.o_t + it_nt_col;
-        const f32x4 o = live ? v : (f32x4){0.f, 0.f, 0.f, 0.f};
-        if (p.out_f32) {
-            float* q = static_cast<float*>(p.out) + at;
-            if (vec_out && it_nt_col < p.DC) *reinterpret_cast<f32x4*>(q) = o;
-            else
+    auto put = [&](float* dst, const f32x4* v, int stride, auto SPRC) {
+        constexpr int SPR = SPRC.value;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) if (it_nt_col + e < p.DC) q[e] = o[e];
-        } else {
-            elem_t<DT>* q = static_cast<elem_t<DT>*>(p.out) + at;
-            if (vec_out && it_nt_col < p.DC) {
-                Pack<DT, 4> w;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w.v[e] = narrow<DT>(o[e]);
-                *reinterpret_cast<Pack<DT, 4>*>(q) = w;
-            } else
-#pragma unroll
-                for (int e = 0; e < 4; ++e) if (it_nt_col + e < p.DC) q[e] = narrow<DT>(o[e]);
+        for (int u = 0; u < CH * SPR / NTH; ++u) {
+            const int x = tid + NTH * u;
+            *reinterpret_cast<f32x4*>(dst + x / SPR * stride + 4 * (x % SPR)) = v[u];
         }
     };
-
-    if constexpr (!STATE && BF) {                                        // the halves of P's operands that lie above the diagonal stay zero
-        for (int i = tid; i < IT * (IT / 2) * 64; i += NTH) *reinterpret_cast<f32x4*>(sp + i * 8) = (f32x4){0.f, 0.f, 0.f, 0.f};
-    }
-    float row_scale[IT];                                                 // lambda^i o_scale of this lane's steps
-    if constexpr (!STATE)
+    typedef std::integral_constant<int, DA / 4> QA;
+    typedef std::integral_constant<int, DCB / 4> QC;
+    auto load = [&](int i0) {
+        if constexpr (!STATE) fetch(ra, pa, p.a_t, i0, p.DA, QA());
+        fetch(rb, pb, p.b_t, i0, p.DA, QA());
+        fetch(rc, pc, p.c_t, i0, dc, QC());
+    };
+    auto store = [&](int i, int col, const f32x4& v) {                   // four columns of step i
+        if (i >= p.T || col >= p.DC) return;
+        const bool live = i < n;
+        float* q = static_cast<float*>(p.out) + b * p.o_b + h * p.o_h + (live && p.reverse ? n - 1 - i : i) * p.o_t + col;
+        const f32x4 o = live ? v : (f32x4){0.f, 0.f, 0.f, 0.f};
+        if (vec_out) *reinterpret_cast<f32x4*>(q) = o;
+        else
 #pragma unroll
-        for (int it = 0; it < IT; ++it) row_scale[it] = exp2f(gl * (float)(16 * it + l16)) * p.o_scale;
+            for (int e = 0; e < 4; ++e) if (col + e < p.DC) q[e] = o[e];
+    };
+
+    float row_scale[2];                                                  // lambda^i o_scale of this lane's steps
+#pragma unroll
+    for (int it = 0; it < 2; ++it) row_scale[it] = exp2f(gl * (float)(16 * it + l16)) * p.o_scale;
     if (tid < CH) rw[tid] = exp2f(gl * (float)(CH - tid)) * p.b_scale;
 
     load(start);
@@ -400,203 +357,129 @@ W[kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
     for (; i0 < stop; i0 += CH) {
         const int cnt = stop - i0 < CH ? stop - i0 : CH;
         // the last chunk of the stream leaves the state as it is after its last step (forward) or leaked once more (reverse)
-        const bool final = i0 + cnt == n;
-        const int e = final && !p.reverse ? cnt - 1 : cnt;
+        const int e = i0 + cnt == n && !p.reverse ? cnt - 1 : cnt;
         __syncthreads();                                                 // the last chunk has been read
-        stage();
+        if constexpr (!STATE) put(sa, ra, SA, QA());
+        put(sb, rb, SA, QA());
+        put(sc, rc, SC, QC());
         if (e != CH && tid < CH) rw[tid] = exp2f(gl * (float)(e > tid ? e - tid : 0)) * p.b_scale;
         __syncthreads();
         if (i0 + CH < stop) load(i0 + CH);
 
-        f32x4 acc[STATE ? 1 : IT];
+        f32x4 acc[2];
         if constexpr (!STATE) {
-            // (1) the tiles on and below the diagonal, dealt to the wavefronts
+            // (1) wavefronts 0 .. 2: a tile of P each
+            if (wv < 3) {
+                const int it = (wv + 1) >> 1, jt = wv >> 1;
+                f32x4 s = {0.f, 0.f, 0.f, 0.f};
+                const float *qa = sa + (16 * it + l16) * SA + 4 * g, *qb = sb + (16 * jt + l16) * SA + 4 * g;
 #pragma unroll
-            for (int z = 0; z < (IT * (IT + 1) / 2 + WV - 1) / WV; ++z) {
-                const int idx = wv + WV * z;
-                if (idx < IT * (IT + 1) / 2) {
-                    const int it = idx < 1 ? 0 : idx < 3 ? 1 : idx < 6 ? 2 : 3, jt = idx - it * (it + 1) / 2;
-                    f32x4 s = {0.f, 0.f, 0.f, 0.f};
-                    const LT* qa = sa + (16 * it + l16) * SA;
-                    const LT* qb = sb + (16 * jt + l16) * SA;
-                    if constexpr (BF) {
+                for (int k = 0; k < KA; ++k)
+                    if (k < ka) {
+                        const f32x4 fb = *reinterpret_cast<const f32x4*>(qb + 16 * k), fa = *reinterpret_cast<const f32x4*>(qa + 16 * k);
 #pragma unroll
-                        for (int k = 0; k < DA / 32; ++k)
-                            s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(qb + 32 * k + 8 * g), *reinterpret_cast<const bf16x8*>(qa + 32 * k + 8 * g), s, 0, 0, 0);
-                    } else {
+                        for (int r = 0; r < 4; ++r) s = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[r], fa[r], s, 0, 0, 0);
+                    }
 #pragma unroll
-                        for (int k = 0; k < KA; ++k) {
-                            const f32x4 fb = *reinterpret_cast<const f32x4*>(qb + 16 * k + 4 * g), fa = *reinterpret_cast<const f32x4*>(qa + 16 * k + 4 * g);
+                for (int r = 0; r < 4; ++r) {
+                    const int d = 16 * (it - jt) + l16 - 4 * g - r;      // i - j
+                    s[r] = d < 0 ? 0.f : s[r] * (exp2f(gl * (float)d) * p.b_scale * p.o_scale);
+                }
+                *reinterpret_cast<f32x4*>(sp + (wv * 64 + lane) * 4) = s;
+            }
+            // (3)
+            acc[0] = acc[1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            if (on) {
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) s = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[r], fa[r], s, 0, 0, 0);
+                for (int k = 0; k < KA; ++k)
+                    if (k < ka) {
+                        const float* q = sa + l16 * SA + 16 * k + 4 * g;
+                        const f32x4 f0 = *reinterpret_cast<const f32x4*>(q), f1 = *reinterpret_cast<const f32x4*>(q + 16 * SA);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            acc[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(W[k][r], f0[r], acc[0], 0, 0, 0);
+                            acc[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(W[k][r], f1[r], acc[1], 0, 0, 0);
                         }
                     }
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int d = 16 * (it - jt) + l16 - 4 * g - r;  // i - j
-                        s[r] = d < 0 ? 0.f : s[r] * (exp2f(gl * (float)d) * p.b_scale * p.o_scale);
-                    }
-                    if constexpr (BF) {
-                        typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-                        *reinterpret_cast<u32x2*>(sp + ((it * (IT / 2) + (jt >> 1)) * 64 + lane) * 8 + (jt & 1) * 4) = (u32x2){round_pk(s[0], s[1]), round_pk(s[2], s[3])};
-                    } else *reinterpret_cast<f32x4*>(sp + ((it * IT + jt) * 64 + lane) * 4) = s;
-                }
+                for (int it = 0; it < 2; ++it) acc[it] *= row_scale[it];
             }
-            // (3)
-#pragma unroll
-            for (int it = 0; it < IT; ++it)
-acc[it] = (f32x4){0.f, 0.f, 0.f, 0.f};
-            if constexpr (BF) {
-#pragma unroll
-                for (int k = 0; k < KA / 2; ++k) {
-                    bf16x8 fw;
-{
-                        const f32x4 x = W[2 * k], y = W[2 * k + 1];
-                        fw = mk8(round_pk(x[0], x[1]), round_pk(x[2], x[3]), round_pk(y[0], y[1]), round_pk(y[2], y[3]));
-                    }
-#pragma unroll
-                    for (int it = 0; it < IT; ++it) {
-                        const bf16x8 fa = *reinterpret_cast<const bf16x8*>(sa + (16 * it + l16) * SA + 32 * k + 8 * g);
-acc[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw, fa, acc[it], 0, 0, 0);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < KA; ++k)
-#pragma unroll
-                    for (int it = 0; it < IT; ++it) {
-                        const f32x4 fa = *reinterpret_cast<const f32x4*>(sa + (16 * it + l16) * SA + 16 * k + 4 * g);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-acc[it] = __builtin_amdgcn_mfma_f32_16x16x4f32(W[k][r], fa[r], acc[it], 0, 0, 0);
-                    }
-            }
-#pragma unroll
-            for (int it = 0; it < IT; ++it)
-acc[it] *= row_scale[it];
             __syncthreads();                                             // P is there
         }
+        if (!on) continue;
         // (2) and (4) share the wavefront's columns of c
         const float keep = exp2f(gl * (float)e);
 #pragma unroll
+        for (int kt = 0; kt < KA; ++kt) W[kt] *= keep;
+        bool wild = false;
+        float fc[2][4];
+#pragma unroll
+        for (int jt = 0; jt < 2; ++jt) {
+            const f32x4 w = *reinterpret_cast<const f32x4*>(rw + 16 * jt + 4 * g);
+            float fin[4];                                                // without what is not finite: 0 * NaN would reach steps before it
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                fc[jt][r] = sc[(16 * jt + 4 * g + r) * SC + wv * 16 + l16];
+                const bool odd = !(fabsf(fc[jt][r]) < __builtin_inff());
+                fin[r] = odd ? 0.f : fc[jt][r];
+                wild = wild || odd;
+                fc[jt][r] *= w[r];
+            }
+            if constexpr (!STATE) {
+#pragma unroll
+                for (int it = jt; it < 2; ++it) {
+                    const f32x4 fp = *reinterpret_cast<const f32x4*>(sp + ((it + jt) * 64 + lane) * 4);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[it] = __builtin_amdgcn_mfma_f32_16x16x4f32(fin[r], fp[r], acc[it], 0, 0, 0);
+                }
+            }
+        }
+#pragma unroll
         for (int kt = 0; kt < KA; ++kt)
-W[kt] *= keep;
-        if constexpr (BF) {
+            if (kt < ka) {
 #pragma unroll
-            for (int kk = 0; kk < CH / 32; ++kk) {
-                bf16x8 t0, t1, t2;
-                const f32x4 w0 = *reinterpret_cast<const f32x4*>(rw + 32 * kk + 4 * g), w1 = *reinterpret_cast<const f32x4*>(rw + 32 * kk + 16 + 4 * g);
-{
-                    const LT* q = sc + (32 * kk + 4 * g + (l16 >> 2)) * SC + wv * 16 + 4 * (l16 & 3);
-                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)q), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(q + 16 * SC));
-                    const s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                    if constexpr (!STATE) {
-                        const bf16x8 fc = __builtin_bit_cast(bf16x8, both);
+                for (int jt = 0; jt < 2; ++jt)
 #pragma unroll
-                        for (int it = 2 * kk; it < IT; ++it)
-                            acc[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fc, *reinterpret_cast<const bf16x8*>(sp + ((it * (IT / 2) + kk) * 64 + lane) * 8), acc[it], 0, 0, 0);
-                    }
-                    float x[8], y[8], z[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float v = __uint_as_float((unsigned)(unsigned short)both[i] << 16) * (i < 4 ? w0[i & 3] : w1[i & 3]);
-                        x[i] = top16(v);
-                        y[i] = v - x[i];
-                        z[i] = y[i] - top16(y[i]);
-                    }
-                    t0 = mk8(pack_hi16(x[0], x[1]), pack_hi16(x[2], x[3]), pack_hi16(x[4], x[5]), pack_hi16(x[6], x[7]));
-                    t1 = mk8(pack_hi16(y[0], y[1]), pack_hi16(y[2], y[3]), pack_hi16(y[4], y[5]), pack_hi16(y[6], y[7]));
-                    t2 = mk8(pack_hi16(z[0], z[1]), pack_hi16(z[2], z[3]), pack_hi16(z[4], z[5]), pack_hi16(z[6], z[7]));
-                }
-#pragma unroll
-                for (int kt = 0; kt < KA; ++kt) {
-                    const LT* q = sb + (32 * kk + 4 * g + (l16 >> 2)) * SA + 32 * (kt >> 1) + 8 * (l16 & 3) + 4 * (kt & 1);
-                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)q), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(q + 16 * SA));
-                    const bf16x8 fb = __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-{
-                        W[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, t2, W[kt], 0, 0, 0);
-                        W[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, t1, W[kt], 0, 0, 0);
-                        W[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, t0, W[kt], 0, 0, 0);
-                    }
-                }
+                    for (int r = 0; r < 4; ++r) W[kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(sb[(16 * jt + 4 * g + r) * SA + 16 * kt + l16], fc[jt][r], W[kt], 0, 0, 0);
             }
-        } else {
-            bool wild = false;
-#pragma unroll
-            for (int jt = 0; jt < IT; ++jt) {
-                const f32x4 w = *reinterpret_cast<const f32x4*>(rw + 16 * jt + 4 * g);
-                float fc[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-fc[r] = sc[(16 * jt + 4 * g + r) * SC + wv * 16 + l16];
-                float fin[4];                                            // without what is not finite: 0 * NaN would reach steps before it
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const bool odd = !(fabsf(fc[r]) < __builtin_inff());
-                    fin[r] = odd ? 0.f : fc[r];
-                    wild = wild || odd;
-                }
-                if constexpr (!STATE) {
-#pragma unroll
-                    for (int it = jt; it < IT; ++it) {
-                        const f32x4 fp = *reinterpret_cast<const f32x4*>(sp + ((it * IT + jt) * 64 + lane) * 4);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) acc[it] = __builtin_amdgcn_mfma_f32_16x16x4f32(fin[r], fp[r], acc[it], 0, 0, 0);
-                    }
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-fc[r] *= w[r];
-#pragma unroll
-                for (int kt = 0; kt < KA; ++kt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float fb = sb[(16 * jt + 4 * g + r) * SA + 16 * kt + l16];
-W[kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb, fc[r], W[kt], 0, 0, 0);
-                    }
-            }
-            if (!STATE && __any(wild))                                   // rare: those terms one by one, where j <= i
+        if constexpr (!STATE) {
+            if (__any(wild))                                             // rare: those terms one by one, where j <= i
 #pragma unroll 1
                 for (int j = 0; j < CH; ++j)
 #pragma unroll
-                    for (int it = 0; it < IT; ++it) {
+                    for (int it = 0; it < 2; ++it) {
                         if (j > 16 * it + l16) continue;
-                        const float pij = sp[((it * IT + (j >> 4)) * 64 + 16 * (j >> 2 & 3) + l16) * 4 + (j & 3)];
+                        const float pij = sp[((it + (j >> 4)) * 64 + 16 * (j >> 2 & 3) + l16) * 4 + (j & 3)];
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             const float c = sc[j * SC + wv * 16 + 4 * g + r];
                             if (!(fabsf(c) < __builtin_inff())) acc[it][r] += pij * c;
                         }
                     }
-        }
-        if constexpr (!STATE)
 #pragma unroll
-            for (int it = 0; it < IT; ++it)
-store(i0 + 16 * it + l16, col0 + 4 * g, acc[it]);
+            for (int it = 0; it < 2; ++it) store(i0 + 16 * it + l16, col0 + 4 * g, acc[it]);
+        }
     }
 
     if constexpr (STATE) {
-        const long long per = (long long)DA * DCB;
-        float* mine = ws + (((long long)bh * plan.ncb + cb) * (plan.nseg - 1) + seg) * per + wv * KA * 256 + lane * 4;
+        float* mine = ws + (((long long)bh * plan.ncb + cb) * (plan.nseg - 1) + seg) * ((long long)DA * DCB) + wv * KA * 256 + lane * 4;
 #pragma unroll
-        for (int kt = 0; kt < KA; ++kt)
-*reinterpret_cast<f32x4*>(mine + kt * 256) = W[kt];
+        for (int kt = 0; kt < KA; ++kt) *reinterpret_cast<f32x4*>(mine + kt * 256) = W[kt];
     } else {
         // steps of the segment behind the stream's last: zeros (the loop above has written its own chunks to their end)
         const int end = start + plan.seg < p.T ? start + plan.seg : p.T;
         for (; i0 < end; i0 += CH)
 #pragma unroll
-            for (int it = 0; it < IT; ++it)
-store(i0 + 16 * it + l16, col0 + 4 * g, (f32x4){0.f, 0.f, 0.f, 0.f});
+            for (int it = 0; it < 2; ++it) store(i0 + 16 * it + l16, col0 + 4 * g, (f32x4){0.f, 0.f, 0.f, 0.f});
         if (p.s_out && ((start < n && n <= start + plan.seg) || (n == 0 && seg == 0))) {
             float* s_out = p.s_out + (long long)bh * p.DA * p.DC;
 #pragma unroll
             for (int kt = 0; kt < KA; ++kt)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int i = 16 * kt + 4 * g + r, j = col0 + l16;
-                        if (i < p.DA && j < p.DC) s_out[i * p.s_out_row + j * p.s_out_col] = W[kt][r];
-                    }
+                for (int r = 0; r < 4; ++r) {
+                    const int i = 16 * kt + 4 * g + r, j = col0 + l16;
+                    if (i < p.DA && j < p.DC) s_out[i * p.s_out_row + j * p.s_out_col] = W[kt][r];
+                }
         }
     }
 }
@@ -650,7 +533,7 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
     if (p.lengths) { n = p.lengths[b]; n = n < 0 ? 0 : n > p.T ? p.T : n; }
     const int start = seg * plan.seg, stop = n < start + plan.seg ? n : start + plan.seg;    // this segment's valid steps
     if (STATE && n <= start + plan.seg) return;                          // no later segment reads this one's state
-    const float gl = fmaxf(p.log_decay[h], -1e30f) * 1.44269504088896341f;                   // log2 lambda
+    const float gl = log2_decay(p.log_decay[h]);
     const int c0 = cb * DCB, col0 = c0 + wv * 16 * NT;
     const unsigned short* pa = static_cast<const unsigned short*>(p.a) + b * p.a_b + (h / p.a_group) * p.a_h;
     const unsigned short* pb = static_cast<const unsigned short*>(p.b) + b * p.b_b + (h / p.b_group) * p.b_h;
@@ -1010,7 +893,7 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
 __global__ __launch_bounds__(256) void leaky_scan_kernel(float* __restrict__ ws, const float* __restrict__ log_decay, int H, int ncb, int per, int nstate, int seg)
 {
     const unsigned parts = per / 1024, head = blockIdx.x / parts, bh = head / ncb;
-    const float leak = exp2f(fmaxf(log_decay[bh % H], -1e30f) * 1.44269504088896341f * (float)seg);
+    const float leak = exp2f(log2_decay(log_decay[bh % H]) * (float)seg);
     float* at = ws + (long long)head * nstate * per + ((blockIdx.x - head * parts) * 256 + threadIdx.x) * 4;
     f32x4 s = *reinterpret_cast<const f32x4*>(at);
     constexpr int U = 16;                    // states in flight: with one at a time the scan is their latencies (63 of them: 23 us)
@@ -1070,12 +953,13 @@ template <int DT> struct LeakyShape {
     }
     template <int DA, int WV, bool STATE> static int launch(const LeakyArgs& p, const LeakyPlan& r, float* ws, hipStream_t s)
     {
-        auto ok = [&](const void* q, long long t, long long b, long long h) { return aligned(q, 16) && t % 8 == 0 && b % 8 == 0 && h % 8 == 0; };
-        const auto near = [](long long t) { return t >= 0 && t < (1 << 24); };  // 32 rows within 32-bit offsets
-        const int vec = near(p.a_t) && near(p.b_t) && near(p.c_t) && near(p.o_t) && p.DA % 8 == 0 && p.DC % 8 == 0 && (STATE || ok(p.a, p.a_t, p.a_b, p.a_h)) && ok(p.b, p.b_t, p.b_b, p.b_h) && ok(p.c, p.c_t, p.c_b, p.c_h);
-        const int vec_out = STATE || (p.DC % 4 == 0 && p.o_t % 4 == 0 && p.o_b % 4 == 0 && p.o_h % 4 == 0 && aligned(p.out, 16));
+        // rows of whole 16-byte granules; a chunk of the output within 32-bit offsets
+        constexpr int E = DT == SS_SEQ_F32 ? 4 : 8;
+        auto ok = [&](const void* q, long long t, long long b, long long h) { return aligned(q, 16) && t % E == 0 && b % E == 0 && h % E == 0; };
+        const int vec = p.DA % E == 0 && p.DC % E == 0 && (STATE || ok(p.a, p.a_t, p.a_b, p.a_h)) && ok(p.b, p.b_t, p.b_b, p.b_h) && ok(p.c, p.c_t, p.c_b, p.c_h);
+        const int vec_out = STATE || (p.DC % 4 == 0 && p.o_t % 4 == 0 && p.o_b % 4 == 0 && p.o_h % 4 == 0 && aligned(p.out, 16) && p.o_t >= 0 && p.o_t < (1 << 24));
         const unsigned grid = (unsigned)(p.B * p.H * r.ncb) * (STATE ? r.nseg - 1 : r.nseg);
-        if constexpr (DT == SS_SEQ_F32) leaky_chunk_kernel<DT, DA, WV, STATE><<<grid, 64 * WV, 0, s>>>(p, r, vec, vec_out, ws);
+        if constexpr (DT == SS_SEQ_F32) leaky_chunk_kernel<DA, WV, STATE><<<grid, 64 * WV, 0, s>>>(p, r, vec, vec_out, ws);
         else if (vec && vec_out) leaky_tile_kernel<DT, DA, WV / 4, STATE, true><<<grid, 256, 0, s>>>(p, r, ws);
         else leaky_tile_kernel<DT, DA, WV / 4, STATE, false><<<grid, 256, 0, s>>>(p, r, ws);
         return launched();
