@@ -59,7 +59,7 @@ namespace {
 
 // The recurrence itself, one step after the other with the state in registers: HBM-bound on reading and writing the state when T is small (the single-step
 // call).  A workgroup owns 64 columns of one head's state: thread (g, x) holds rows g + 16 r of columns 4 x .. 4 x + 3.
-template <int DT, int ODT, int R, bool V4> __global__ __launch_bounds__(256) void leaky_steps_kernel(const LeakyArgs p)
+template <int DT, int ODT, int R, bool V4> __global__ __launch_bounds__(256, 4) void leaky_steps_kernel(const LeakyArgs p)
 {
     __shared__ float sa[256], sb[256], red[4][64];
     const int tid = threadIdx.x, x = tid & 15, g = tid >> 4;
@@ -222,6 +222,18 @@ struct LeakyPlan {
     // columns, nseg - 1 matrices in accumulator order (wavefronts of 16 nt columns, `ka` row tiles)
     int trans, ka, nt, dcb, sncb;
 };
+struct LeakyMap {
+    LeakyArgs p;
+    LeakyPlan plan;
+    float* ws;                               // the states between segments
+    int vec, vec_out;                        // 16-byte accesses to the operands, to the output
+};
+// the maps of one launch: `per` workgroups each
+struct LeakyMaps {
+    LeakyMap m[3];
+    unsigned per;
+};
+
 // the 16 x 16 tile of rows 16 rt, columns 16 ct of a state left in accumulator order: its first element
 __device__ __forceinline__ long long state_tile(const LeakyPlan& p, long long bh, int s, int rt, int ct)
 {
@@ -252,7 +264,7 @@ __device__ __forceinline__ unsigned round_pk(float lo, float hi)
 // The tile form on fp32 operands: the 16x16x4 fp32 matrix instructions, a workgroup of WV (4 or 8) wavefronts with 16 columns each, two workgroups on a CU.
 // Bound by those instructions (157 TFLOP/s), so the 16-row tiles behind DA and the wavefronts behind DC are left out.
 template <int DA, int WV, bool STATE>
-__global__ __launch_bounds__(64 * WV, DA == 64 || (DA == 128 && WV == 8) ? 4 : 2) void leaky_chunk_kernel(const LeakyArgs p, const LeakyPlan plan, const int vec, const int vec_out, float* __restrict__ ws)
+__global__ __launch_bounds__(64 * WV, DA == 64 || (DA == 128 && WV == 8) ? 4 : 2) void leaky_chunk_kernel(const LeakyMaps maps)
 {
     constexpr int CH = 32, NTH = 64 * WV, DCB = 16 * WV, KA = DA / 16;
     constexpr int SA = DA + 4, SC = DCB + 4;                             // LDS rows 16 bytes longer than a power of two
@@ -264,7 +276,12 @@ __global__ __launch_bounds__(64 * WV, DA == 64 || (DA == 128 && WV == 8) ? 4 : 2
     __shared__ __attribute__((aligned(16))) float rw[CH];                // lambda^(e - j) b_scale of the chunk's steps
 
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g = lane >> 4;
-    const int cb = blockIdx.x % plan.ncb, rest = blockIdx.x / plan.ncb;
+    const unsigned which = blockIdx.x / maps.per, block = blockIdx.x - which * maps.per;
+    const LeakyMap& map = maps.m[which];
+    const LeakyArgs& p = map.p;
+    const LeakyPlan& plan = map.plan;
+    float* __restrict__ ws = map.ws;
+    const int cb = block % plan.ncb, rest = block / plan.ncb;
     const int nst = STATE ? plan.nseg - 1 : plan.nseg, seg = rest % nst, bh = rest / nst, b = bh / p.H, h = bh - b * p.H;
     int n = p.T;
     if (p.lengths) { n = p.lengths[b]; n = n < 0 ? 0 : n > p.T ? p.T : n; }
@@ -314,7 +331,7 @@ __global__ __launch_bounds__(64 * WV, DA == 64 || (DA == 128 && WV == 8) ? 4 : 2
             const float* src = base + (long long)(p.reverse ? n - 1 - i : i) * st + 4 * q;
             dst[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
             if (i < stop && 4 * q < d) {
-                if (vec) dst[u] = *reinterpret_cast<const f32x4*>(src);
+                if (map.vec) dst[u] = *reinterpret_cast<const f32x4*>(src);
                 else
 #pragma unroll
                     for (int e = 0; e < 4; ++e) if (4 * q + e < d) dst[u][e] = src[e];
@@ -341,7 +358,7 @@ __global__ __launch_bounds__(64 * WV, DA == 64 || (DA == 128 && WV == 8) ? 4 : 2
         const bool live = i < n;
         float* q = static_cast<float*>(p.out) + b * p.o_b + h * p.o_h + (live && p.reverse ? n - 1 - i : i) * p.o_t + col;
         const f32x4 o = live ? v : (f32x4){0.f, 0.f, 0.f, 0.f};
-        if (vec_out) *reinterpret_cast<f32x4*>(q) = o;
+        if (map.vec_out) *reinterpret_cast<f32x4*>(q) = o;
         else
 #pragma unroll
             for (int e = 0; e < 4; ++e) if (col + e < p.DC) q[e] = o[e];
@@ -516,7 +533,7 @@ __device__ __forceinline__ f16x8 half8(const f32x4& x, const f32x4& y, float up)
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 template <int DT, int DA, int NT, bool STATE, bool VEC>
-__global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel(const LeakyArgs p, const LeakyPlan plan, float* __restrict__ ws)
+__global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel(const LeakyMaps maps)
 {
     constexpr int CH = 32, DCB = 64 * NT, KA = DA / 16, SA = DA / 8, SC = DCB / 8;          // SA, SC: granules of a row
     constexpr int BA = CH * DA, BC = CH * DCB, BUF = (STATE ? 1 : 2) * BA + BC;              // elements of a buffer: [a] b c
@@ -527,7 +544,12 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
     constexpr bool H = DT == SS_SEQ_F16;
 
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g = lane >> 4;
-    const int cb = blockIdx.x % plan.ncb, rest = blockIdx.x / plan.ncb;
+    const unsigned which = blockIdx.x / maps.per, block = blockIdx.x - which * maps.per;
+    const LeakyMap& map = maps.m[which];
+    const LeakyArgs& p = map.p;
+    const LeakyPlan& plan = map.plan;
+    float* __restrict__ ws = map.ws;
+    const int cb = block % plan.ncb, rest = block / plan.ncb;
     const int nst = STATE ? plan.nseg - 1 : plan.nseg, seg = rest % nst, bh = rest / nst, b = bh / p.H, h = bh - b * p.H;
     int n = p.T;
     if (p.lengths) { n = p.lengths[b]; n = n < 0 ? 0 : n > p.T ? p.T : n; }
@@ -951,30 +973,43 @@ template <int DT> struct LeakyShape {
         const LeakyPlan r = plan(T, B, H, DA, DC);
         return (long long)B * H * (r.nseg - 1) * (r.ncb * r.dcb) * pad(DA);
     }
-    template <int DA, int WV, bool STATE> static int launch(const LeakyArgs& p, const LeakyPlan& r, float* ws, hipStream_t s)
+    static LeakyMap map_of(const LeakyArgs& p, const LeakyPlan& r, float* ws, bool state)
     {
         // rows of whole 16-byte granules; a chunk of the output within 32-bit offsets
         constexpr int E = DT == SS_SEQ_F32 ? 4 : 8;
         auto ok = [&](const void* q, long long t, long long b, long long h) { return aligned(q, 16) && t % E == 0 && b % E == 0 && h % E == 0; };
-        const int vec = p.DA % E == 0 && p.DC % E == 0 && (STATE || ok(p.a, p.a_t, p.a_b, p.a_h)) && ok(p.b, p.b_t, p.b_b, p.b_h) && ok(p.c, p.c_t, p.c_b, p.c_h);
-        const int vec_out = STATE || (p.DC % 4 == 0 && p.o_t % 4 == 0 && p.o_b % 4 == 0 && p.o_h % 4 == 0 && aligned(p.out, 16) && p.o_t >= 0 && p.o_t < (1 << 24));
-        const unsigned grid = (unsigned)(p.B * p.H * r.ncb) * (STATE ? r.nseg - 1 : r.nseg);
-        if constexpr (DT == SS_SEQ_F32) leaky_chunk_kernel<DA, WV, STATE><<<grid, 64 * WV, 0, s>>>(p, r, vec, vec_out, ws);
-        else if (vec && vec_out) leaky_tile_kernel<DT, DA, WV / 4, STATE, true><<<grid, 256, 0, s>>>(p, r, ws);
-        else leaky_tile_kernel<DT, DA, WV / 4, STATE, false><<<grid, 256, 0, s>>>(p, r, ws);
+        const int vec = p.DA % E == 0 && p.DC % E == 0 && (state || ok(p.a, p.a_t, p.a_b, p.a_h)) && ok(p.b, p.b_t, p.b_b, p.b_h) && ok(p.c, p.c_t, p.c_b, p.c_h);
+        const int vec_out = state || (p.DC % 4 == 0 && p.o_t % 4 == 0 && p.o_b % 4 == 0 && p.o_h % 4 == 0 && aligned(p.out, 16) && p.o_t >= 0 && p.o_t < (1 << 24));
+        return {p, r, ws, vec, vec_out};
+    }
+    template <int DA, int WV, bool STATE> static int launch(LeakyMaps& maps, int count, hipStream_t s)
+    {
+        const LeakyPlan& r = maps.m[0].plan;               // maps of one launch have the same segments and column blocks
+        maps.per = (unsigned)(maps.m[0].p.B * maps.m[0].p.H * r.ncb) * (STATE ? r.nseg - 1 : r.nseg);
+        const unsigned grid = maps.per * count;
+        if constexpr (DT == SS_SEQ_F32) leaky_chunk_kernel<DA, WV, STATE><<<grid, 64 * WV, 0, s>>>(maps);
+        else {
+            bool all = true;
+            for (int i = 0; i < count; ++i) all = all && maps.m[i].vec && maps.m[i].vec_out;
+            if (all) leaky_tile_kernel<DT, DA, WV / 4, STATE, true><<<grid, 256, 0, s>>>(maps);
+            else leaky_tile_kernel<DT, DA, WV / 4, STATE, false><<<grid, 256, 0, s>>>(maps);
+        }
         return launched();
     }
-    template <bool STATE> static int pass(const LeakyArgs& p, const LeakyPlan& r, float* ws, hipStream_t s)
+    // `count` maps of the same padded sizes in one launch
+    template <bool STATE> static int pass(LeakyMaps& maps, int count, hipStream_t s)
     {
-        auto by_dc = [&](auto DAC) { return p.DC <= 64 ? launch<DAC.value, 4, STATE>(p, r, ws, s) : launch<DAC.value, 8, STATE>(p, r, ws, s); };
-        return p.DA <= 64 ? by_dc(std::integral_constant<int, 64>()) : p.DA <= 128 ? by_dc(std::integral_constant<int, 128>()) : by_dc(std::integral_constant<int, 256>());
+        const int DA = maps.m[0].p.DA, DC = maps.m[0].p.DC;
+        auto by_dc = [&](auto DAC) { return DC <= 64 ? launch<DAC.value, 4, STATE>(maps, count, s) : launch<DAC.value, 8, STATE>(maps, count, s); };
+        return DA <= 64 ? by_dc(std::integral_constant<int, 64>()) : DA <= 128 ? by_dc(std::integral_constant<int, 128>()) : by_dc(std::integral_constant<int, 256>());
     }
     // the states that enter the segments, into ws (nothing where there is one segment)
     static int states(const LeakyArgs& p, const LeakyPlan& r, float* ws, hipStream_t s)
     {
         if (r.nseg == 1) return SS_SEQ_OK;
         if (!ws || !aligned(ws, 16)) return SS_SEQ_EINVAL;
-        if (int rc = pass<true>(p, r, ws, s)) return rc;
+        LeakyMaps one{{map_of(p, r, ws, true)}, 0};
+        if (int rc = pass<true>(one, 1, s)) return rc;
         if (r.fold) return SS_SEQ_OK;
         const int per = pad(p.DA) * r.dcb;
         leaky_scan_kernel<<<(unsigned)(p.B * p.H * r.ncb) * (per / 1024), 256, 0, s>>>(ws, p.log_decay, p.H, r.ncb, per, r.nseg - 1, r.seg);
@@ -985,20 +1020,20 @@ template <int DT> struct LeakyShape {
         if (p.T < kStepsMax) return p.out_f32 ? steps<DT, SS_SEQ_F32>(p, s) : steps<DT, DT>(p, s);
         const LeakyPlan r = plan(p.T, p.B, p.H, p.DA, p.DC);
         if (int rc = states(p, r, ws, s)) return rc;
-        return pass<false>(p, r, ws, s);
+        LeakyMaps one{{map_of(p, r, ws, false)}, 0};
+        return pass<false>(one, 1, s);
     }
 
-    // ---- the gradients: three maps.  dq reads the forward pass's states transposed; dk and dv run backwards in time and share the states of (q, g).
-    static long long bwd_floats(const LeakyBwdArgs& d)
-    {
-        const long long part = d.H == d.Hk ? 0 : (long long)d.T * d.B * d.H * (d.Dk > d.Dv ? d.Dk : d.Dv);
-        return (part + 3) / 4 * 4 + state_floats(d.T, d.B, d.H, d.Dk, d.Dv);
-    }
+    // ---- the gradients: three maps.  dq reads the forward pass's states transposed; dk and dv run backwards in time and share the states of (q, g).  dq and
+    // dk are of one shape and run in one launch, with dv where its padded sizes are theirs: the ends of one map's streams fill with the next map's workgroups
+    // (48 heads of 80 and 96, 777 ragged steps, fp32: three launches 196 us a training step, one 158).
+    static long long round4(long long n) { return (n + 3) / 4 * 4; }
+    static long long heads_floats(const LeakyBwdArgs& d, int D) { return d.H == d.Hk ? 0 : round4((long long)d.T * d.B * d.H * D); }
+    static long long bwd_floats(const LeakyBwdArgs& d) { return heads_floats(d, d.Dk) + heads_floats(d, d.Dv) + state_floats(d.T, d.B, d.H, d.Dk, d.Dv); }
     static int bwd(const LeakyBwdArgs& d, hipStream_t s)
     {
         const int group = d.H / d.Hk;
-        const long long part = group == 1 ? 0 : ((long long)d.T * d.B * d.H * (d.Dk > d.Dv ? d.Dk : d.Dv) + 3) / 4 * 4;
-        float *shared = d.ws, *rstate = d.ws + part;
+        float *each_k = d.ws, *each_v = each_k + heads_floats(d, d.Dk), *rstate = each_v + heads_floats(d, d.Dv);      // gradients by query head
         const bool tiles = d.T >= kStepsMax;
         const LeakyPlan fwd = plan(d.T, d.B, d.H, d.Dk, d.Dv);
         if (bwd_floats(d) && (!d.ws || !aligned(d.ws, 16))) return SS_SEQ_EINVAL;
@@ -1014,34 +1049,40 @@ template <int DT> struct LeakyShape {
             p.log_decay = d.log_decay; p.lengths = d.lengths; p.out_f32 = f32;
             return p;
         };
-        auto go = [&](const LeakyArgs& p, float* states, bool trans) {
-            if (!tiles) return p.out_f32 ? steps<DT, SS_SEQ_F32>(p, s) : steps<DT, DT>(p, s);
-            LeakyPlan r = fwd;                             // the forward pass's segments, whatever this map's own sizes
-            r.ncb = blocks(p.DC);
-            r.trans = trans;
-            return pass<false>(p, r, states, s);
-        };
-        auto sum = [&](void* out, int D) { return ss_seq_group_sum(shared, out, (long long)d.T * d.B * d.Hk, group, D, DT, s); };
-        if (d.g_q) {
-            LeakyArgs p = map(d.Dv, d.Dk, 0, 1.f, d.scale, d.g, d.v, d.k, d.g_q, DT == SS_SEQ_F32);
-            p.s_in = d.s_in; p.s_in_row = 1; p.s_in_col = d.Dv;
-            if (int rc = go(p, const_cast<float*>(d.states), true)) return rc;
-        }
-        if (!d.g_k && !d.g_v) return SS_SEQ_OK;
-        LeakyArgs pv = map(d.Dk, d.Dv, 1, d.scale, 1.f, d.k, d.q, d.g, group == 1 ? d.g_v : shared, group > 1 || DT == SS_SEQ_F32);
+        LeakyArgs pv = map(d.Dk, d.Dv, 1, d.scale, 1.f, d.k, d.q, d.g, group == 1 ? d.g_v : each_v, group > 1 || DT == SS_SEQ_F32);
         pv.s_in = d.g_last; pv.s_in_row = d.Dv; pv.s_in_col = 1;
         pv.s_out = d.g_s; pv.s_out_row = d.Dv; pv.s_out_col = 1;
-        if (tiles) if (int rc = states(pv, fwd, rstate, s)) return rc;
-        if (d.g_v) {
-            if (int rc = go(pv, rstate, false)) return rc;
-            if (group > 1) if (int rc = sum(d.g_v, d.Dv)) return rc;
+        LeakyArgs pq = map(d.Dv, d.Dk, 0, 1.f, d.scale, d.g, d.v, d.k, d.g_q, DT == SS_SEQ_F32);
+        pq.s_in = d.s_in; pq.s_in_row = 1; pq.s_in_col = d.Dv;
+        LeakyArgs pk = map(d.Dv, d.Dk, 1, d.scale, 1.f, d.v, d.g, d.q, group == 1 ? d.g_k : each_k, group > 1 || DT == SS_SEQ_F32);
+        pk.s_in = d.g_last; pk.s_in_row = 1; pk.s_in_col = d.Dv;
+        if (!tiles) {
+            auto go = [&](const LeakyArgs& p) { return p.out_f32 ? steps<DT, SS_SEQ_F32>(p, s) : steps<DT, DT>(p, s); };
+            if (d.g_q) if (int rc = go(pq)) return rc;
+            if (d.g_v) if (int rc = go(pv)) return rc;
+            if (d.g_k) if (int rc = go(pk)) return rc;
+        } else {
+            if (d.g_k || d.g_v) if (int rc = states(pv, fwd, rstate, s)) return rc;
+            LeakyMaps maps{};
+            int count = 0;
+            auto add = [&](const LeakyArgs& p, float* ws, int trans) {
+                LeakyPlan r = fwd;                         // the forward pass's segments, whatever this map's own sizes
+                r.ncb = blocks(p.DC);
+                r.trans = trans;
+                maps.m[count++] = map_of(p, r, ws, false);
+            };
+            if (d.g_q) add(pq, const_cast<float*>(d.states), 1);
+            if (d.g_k) add(pk, rstate, 1);
+            if (d.g_v && pad(d.Dk) != pad(d.Dv) && count) {
+                if (int rc = pass<false>(maps, count, s)) return rc;
+                count = 0;
+            }
+            if (d.g_v) add(pv, rstate, 0);
+            if (int rc = count ? pass<false>(maps, count, s) : SS_SEQ_OK) return rc;
         }
-        if (d.g_k) {
-            LeakyArgs p = map(d.Dv, d.Dk, 1, d.scale, 1.f, d.v, d.g, d.q, group == 1 ? d.g_k : shared, group > 1 || DT == SS_SEQ_F32);
-            p.s_in = d.g_last; p.s_in_row = 1; p.s_in_col = d.Dv;
-            if (int rc = go(p, rstate, true)) return rc;
-            if (group > 1) if (int rc = sum(d.g_k, d.Dk)) return rc;
-        }
+        auto sum = [&](const float* each, void* out, int D) { return ss_seq_group_sum(each, out, (long long)d.T * d.B * d.Hk, group, D, DT, s); };
+        if (group > 1 && d.g_k) if (int rc = sum(each_k, d.g_k, d.Dk)) return rc;
+        if (group > 1 && d.g_v) if (int rc = sum(each_v, d.g_v, d.Dv)) return rc;
         return SS_SEQ_OK;
     }
 };
