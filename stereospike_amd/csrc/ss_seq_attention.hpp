@@ -516,6 +516,8 @@ template <int DT> __device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, f32x
     if constexpr (DT == SS_SEQ_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
+// |x|, 0 for what is not finite
+__device__ __forceinline__ float finite(float x) { return fabsf(x) < __builtin_inff() ? fabsf(x) : 0.f; }
 // a power of two that takes `most` into [2^14, 2^15), fp16's upper end, and its inverse; 1 for zero and for what is not finite
 __device__ __forceinline__ void fp16_scale(float most, float& up, float& down)
 {
@@ -723,7 +725,7 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
                 }
                 if constexpr (H) {
                     float up, down;
-                    fp16_scale(wave_max(fmaxf(fmaxf(fabsf(s[0]), fabsf(s[1])), fmaxf(fabsf(s[2]), fabsf(s[3])))), up, down);
+                    fp16_scale(wave_max(fmaxf(fmaxf(finite(s[0]), finite(s[1])), fmaxf(finite(s[2]), finite(s[3])))), up, down);
                     *reinterpret_cast<f16x4*>(sp + (wv * 64 + lane) * 4) = (f16x4){(_Float16)(s[0] * up), (_Float16)(s[1] * up), (_Float16)(s[2] * up), (_Float16)(s[3] * up)};
                     if (lane == 0) p_down[wv] = down;
                 } else {
@@ -745,7 +747,18 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(W[kt][nt][r]));
-                fp16_scale(wave_max(most), up, down);
+                most = wave_max(most);
+                if (most == __builtin_inff()) {                          // rare: the others' scale without what is infinite
+                    most = 0.f;
+#pragma unroll
+                    for (int kt = 0; kt < KA; ++kt)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) most = fmaxf(most, finite(W[kt][nt][r]));
+                    most = wave_max(most);
+                }
+                fp16_scale(most, up, down);
             }
 #pragma unroll
             for (int k = 0; k < KA / 2; ++k) {

@@ -402,7 +402,7 @@ long long ss_seq_int8_linear_ws_ints(const signed char* a, long long lda, const 
 int ss_seq_int8_linear(const signed char* a, long long lda, const float* a_scale, const signed char* w, long long ldw, const float* w_scale,
                        const float* bias, void* out, long long M, int N, int K, int out_dtype, int* ws, void* stream)
 {
-    if (M < 0 || M > (1 << 30) || N <= 0 || N > (1 << 30) || ((M + 127) / 128) * ((N + 127ll) / 128) > 0x7FFFFFFFll || K <= 0 || K >= 131072 || lda < 0 || ldw < 0) return SS_SEQ_EINVAL;
+    if (M < 0 || M > (1 << 27) || N <= 0 || N > (1 << 27) || ((M + 127) / 128) * ((N + 127ll) / 128) >= (1 << 24) || K <= 0 || K >= 131072 || lda < 0 || ldw < 0) return SS_SEQ_EINVAL;
     if (out_dtype != SS_SEQ_F32 && out_dtype != SS_SEQ_F16 && out_dtype != SS_SEQ_BF16) return SS_SEQ_EINVAL;
     if (M == 0) return SS_SEQ_OK;
     if (!a || !a_scale || !w || !w_scale || !out) return SS_SEQ_EINVAL;

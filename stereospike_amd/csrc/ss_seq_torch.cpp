@@ -21,7 +21,7 @@ typedef std::optional<Tensor> Maybe;
 
 namespace {
 
-constexpr int64_t kMaxHead = 256, kMaxWidth = 16384, kMaxK = 131071, kMaxStates = 65535, kMaxSteps = 1 << 30, kMaxSide = 1 << 30;
+constexpr int64_t kMaxHead = 256, kMaxWidth = 16384, kMaxK = 131071, kMaxStates = 65535, kMaxSteps = 1 << 30, kMaxSide = 1 << 27;
 
 struct SeqError : std::runtime_error { using std::runtime_error::runtime_error; };
 

@@ -169,7 +169,7 @@ def int8_linear(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor,
                 out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """out[..., n] = (sum_k codes[..., k] * weight[n, k]) * scales[...] * weight_scale[n] + bias[n], the sum exact in 32-bit integers.
 
-    codes int8 [..., K] (spike counts are codes of scale 1), scales fp32 [...], weight int8 [N, K], weight_scale fp32 [N], bias fp32 [N]; K < 131072.  Scaled in
+    codes int8 [..., K] (spike counts are codes of scale 1), scales fp32 [...], weight int8 [N, K], weight_scale fp32 [N], bias fp32 [N]; K < 131072, at most 2^27 rows and channels.  Scaled in
     fp32, rounded once to out_dtype (float32 / float16 / bfloat16).  No gradients."""
     def refuse():
         _require_hip(codes, 'codes')

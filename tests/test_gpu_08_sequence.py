@@ -161,6 +161,67 @@ def test_what_is_not_finite_reaches_no_earlier_step(dtype, what):
         assert not torch.isfinite(a[37, 0, 1]).all()
 
 
+@pytest.mark.parametrize('T', [7, 8, 9, 31, 32, 33])
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_leaky_attention_around_a_tile(T, dtype):
+    """The shortest call in tiles and its neighbours, a tile and one step less or more; widths one behind a multiple of 64."""
+    leaky_check(T, 7, 2, 1, 65, 129, dtype, state=True, ragged=True, grads=True)
+
+
+@pytest.mark.parametrize('T', [1, 3, 40, 700])
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_a_decay_that_is_not_a_number_stays_in_its_head(T, dtype):
+    q, k, v, _, s, _ = (t.to(DEV) if t is not None else None for t in leaky_case(T, 2, 3, 3, 16, 24, dtype, True, False, seed=13))
+    decay = torch.tensor([-0.1, math.nan, -0.01], device=DEV)
+    o, last = sequence.leaky_attention(q, k, v, decay, state=s, return_state=True)
+    clean, clean_last = sequence.leaky_attention(q, k, v, torch.tensor([-0.1, -0.3, -0.01], device=DEV), state=s, return_state=True)
+    assert o[:, :, 1].isnan().all() and last[:, 1].isnan().all()
+    assert torch.equal(o[:, :, ::2], clean[:, :, ::2]) and torch.equal(last[:, ::2], clean_last[:, ::2])
+    if T == 1:
+        o = sequence.leaky_attention_step(q[0], k[0], v[0], decay, s)
+        assert o[:, 1].isnan().all() and s[:, 1].isnan().all() and torch.isfinite(s[:, ::2]).all()
+
+
+@pytest.mark.parametrize('T', [1, 2, 7, 40])
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_an_infinite_state_stays_in_its_place(T, dtype):
+    """S leaks as S * lambda, so an infinity stays one; the other rows and columns of the head keep their values."""
+    q, k, v, _, s, _ = (t.to(DEV) if t is not None else None for t in leaky_case(T, 2, 1, 1, 16, 24, dtype, True, False, seed=14))
+    decay = torch.tensor([-0.05], device=DEV)
+    clean, clean_last = sequence.leaky_attention(q, k, v, decay, state=s, return_state=True)
+    bad = s.clone()
+    bad[1, 0, 3, 5] = math.inf
+    o, last = sequence.leaky_attention(q, k, v, decay, state=bad, return_state=True)
+    hit = torch.zeros_like(last, dtype=torch.bool)
+    hit[1, 0, 3, 5] = True
+    assert (last[hit] == math.inf).all() and torch.equal(last[~hit], clean_last[~hit])
+    hit = torch.zeros_like(o, dtype=torch.bool)
+    hit[:, 1, 0, 5] = True
+    assert torch.equal(o[hit], (q[:, 1, 0, 3].sign() * math.inf)) and torch.equal(o[~hit], clean[~hit])
+
+
+def test_fp16_states_beyond_the_type():
+    """States and token-by-token weights beyond fp16's largest number (65504), with outputs within it: scaled by powers of two.  An infinite value in a column, or
+    an infinite query, leaves the other columns' and rows' scales alone."""
+    q, k, v, _, _, _ = (t.to(DEV) if t is not None else None for t in leaky_case(100, 1, 2, 2, 24, 40, torch.float16, False, False, seed=15))
+    decay = torch.tensor([0., -0.01], device=DEV)
+    for q, v in ((q * 0.02, v * 1e4), (q * 3e3, v * 1e-3)):
+        k = k * 30 if v.abs().max() < 1 else k
+        clean, last = sequence.leaky_attention(q, k, v, decay, return_state=True)
+        want, _ = leaky_ref(q, k, v, decay, 24 ** -0.5)
+        size, _ = leaky_ref(q.abs(), k.abs(), v.abs(), decay, 24 ** -0.5)
+        within(clean, want, size * (400 * U + HALF[torch.float16]) + want.abs() * HALF[torch.float16] * 1.02 + TINY[torch.float16], 'o')
+        assert last.abs().max() > 65504 or (q.float() @ k.float().transpose(-1, -2)).abs().max() > 65504
+        bad = v.clone()
+        bad[37, 0, 1, 5] = math.inf
+        rest = torch.arange(40, device=DEV) != 5
+        assert torch.equal(sequence.leaky_attention(q, k, bad, decay)[..., rest], clean[..., rest])
+        bad = q.clone()
+        bad[37, 0, 1, 5] = math.inf
+        rest = torch.arange(100, device=DEV) != 37
+        assert torch.equal(sequence.leaky_attention(bad, k, v, decay)[rest], clean[rest])
+
+
 def test_leaky_gradient_against_differences():
     """The map is linear in each operand: a central difference of the definition along a direction is its derivative, up to the definition's fp64."""
     q, k, v, decay, s, n = leaky_case(70, 3, 2, 1, 12, 10, torch.float32, True, True, seed=5)
@@ -625,6 +686,115 @@ def test_captured_calls_replay():
             assert torch.equal(ys, want) and torch.equal(state, eager_state)
             wp, ws = prompt()
             assert torch.equal(yp, wp) and torch.equal(sp, ws)
+
+
+def test_captured_gradients_replay():
+    """Attention -> add + norm and all their gradients in one graph, on leaves of its own; replayed with eager passes between: the eager result each time."""
+    g = gen(16)
+    T, B, H, D = 90, 2, 4, 32
+    sets = [[normal(g, T, B, n, D, dtype=torch.bfloat16).to(DEV) for n in (H, 2, 2, H, H)] + [normal(g, B, H, D, D).to(DEV) for _ in range(2)] for _ in range(3)]
+    data, w, decay = [t.clone() for t in sets[0]], (1 + normal(g, D, std=0.1)).to(DEV), torch.tensor([-0.01, -0.1, -0.5, 0.], device=DEV)
+
+    def run(q, k, v, gy, gh, s, gl):
+        q, k, v, s, wl = (t.detach().requires_grad_() for t in (q, k, v, s, w))
+        o, last = sequence.leaky_attention(q, k, v, decay, state=s, return_state=True)
+        y, h = sequence.add_rms_norm(o, wl, q)
+        return (y.detach(), h.detach(), last.detach(), *torch.autograd.grad([y, h, last], [q, k, v, s, wl], [gy, gh, gl]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(*data)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(*data)
+    for new in (*sets, *sets[:2]):
+        for a, b in zip(data, new):
+            a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, run(*new)):
+            assert torch.equal(a, b)
+
+
+# ----------------------------------------------------------------------------------------------------------------------------------------------------------
+# offsets that pass 32 bits: what the same values give in a small tensor
+# ----------------------------------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_far_steps_of_attention(dtype):
+    T, D, step = 36, 64, 1 << 26
+    far = torch.empty(T * step, dtype=dtype, device=DEV)
+    q, k, v, go = (far.as_strided((T, 2, 1, D), (step, step // 2, D, 1), 8 * D * i) for i in range(4))
+    g = gen(17)
+    for t in (q, k, v, go):
+        t.copy_(normal(g, T, 2, 1, D))
+    decay, near = torch.tensor([-0.05], device=DEV), [t.contiguous() for t in (q, k, v, go)]
+
+    def run(q, k, v, go):
+        q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+        o = sequence.leaky_attention(q, k, v, decay)
+        return (o.detach(), *torch.autograd.grad(o, (q, k, v), go))
+
+    for a, b in zip(run(q, k, v, go), run(*near)):
+        assert torch.equal(a, b)
+    for a, b in zip(run(q[::7], k[::7], v[::7], go[::7]), run(*(t[::7] for t in near))):
+        assert torch.equal(a, b)
+
+
+def test_far_states_of_steps():
+    B, H, D = 200, 170, 256
+    q, k, v = (normal(gen(i), B, H, D, dtype=torch.bfloat16).to(DEV) for i in range(3))
+    state, decay = torch.empty(B, H, D, D, device=DEV), torch.full((H,), -0.1, device=DEV)
+    state[-1] = normal(gen(3), H, D, D).to(DEV)
+    last = state[-1:].clone()
+    o = sequence.leaky_attention_step(q, k, v, decay, state)
+    assert torch.equal(o[-1:], sequence.leaky_attention_step(q[-1:], k[-1:], v[-1:], decay, last)) and torch.equal(state[-1:], last)
+
+
+def test_far_rows_of_norm_and_product():
+    g = torch.Generator(device=DEV).manual_seed(18)
+    M, K = 540000, 4096
+    x = torch.empty(M, K, dtype=torch.bfloat16, device=DEV)
+    x[-100:] = torch.randn(100, K, generator=g, device=DEV)
+    x[:-100] = x[-100:].repeat(5399, 1)
+    w = torch.rand(K, generator=g, device=DEV)
+    y, h = sequence.add_rms_norm(x, w, x)
+    ye, he = sequence.add_rms_norm(x[-100:], w, x[-100:])
+    assert torch.equal(y[-100:], ye) and torch.equal(h[-100:], he) and torch.equal(y[:100], ye)
+    del y, h
+    c, s, h = sequence.add_rms_norm_int8(x, w)
+    ce, se, _ = sequence.add_rms_norm_int8(x[-100:], w)
+    assert torch.equal(c[-100:], ce) and torch.equal(s[-100:], se)
+    d = sequence.dequantize_int8(c, s, torch.bfloat16)
+    assert torch.equal(d[-100:], sequence.dequantize_int8(ce, se, torch.bfloat16))
+    del d, x, h
+    wc = torch.randint(-128, 128, (24, K), generator=g, device=DEV, dtype=torch.int32).to(torch.int8)
+    ws = torch.rand(24, generator=g, device=DEV)
+    out, few = sequence.int8_linear(c, s, wc, ws), sequence.int8_linear(ce, se, wc, ws)
+    assert torch.equal(out[-100:], few) and torch.equal(out[:100], few)
+    del c, out
+    c = torch.randint(-128, 128, (70000, 16), generator=g, device=DEV, dtype=torch.int32).to(torch.int8)                # an output beyond 32 bits
+    wc = torch.randint(-128, 128, (32768, 16), generator=g, device=DEV, dtype=torch.int32).to(torch.int8)
+    s, ws = torch.rand(70000, generator=g, device=DEV), torch.rand(32768, generator=g, device=DEV)
+    out = sequence.int8_linear(c, s, wc, ws, out_dtype=torch.bfloat16)
+    assert torch.equal(out[-50:], sequence.int8_linear(c[-50:], s[-50:], wc, ws, out_dtype=torch.bfloat16))
+
+
+def test_one_row_expanded():
+    """Rows that are all the same memory (a stride of 0)."""
+    g = gen(19)
+    x, w = normal(g, 1, 64).to(DEV), torch.ones(64, device=DEV)
+    for a, b in zip(sequence.add_rms_norm(x.expand(70, 64), w, x.expand(70, 64)), sequence.add_rms_norm(x, w, x)):
+        assert torch.equal(a, b.expand(70, 64))
+    c, s, _ = sequence.add_rms_norm_int8(x.expand(70, 64), w)
+    one, s1, _ = sequence.add_rms_norm_int8(x, w)
+    assert torch.equal(c, one.expand(70, 64)) and torch.equal(s, s1.expand(70))
+    wc = torch.randint(-128, 128, (5, 64), generator=g, dtype=torch.int32).to(torch.int8).to(DEV)
+    want = sequence.int8_linear(one, s1, wc, torch.ones(5, device=DEV))
+    assert torch.equal(sequence.int8_linear(one.expand(70, 64), s1.expand(70), wc, torch.ones(5, device=DEV)), want.expand(70, 5))
+    assert torch.equal(sequence.int8_linear(one, s1, wc[:1].expand(5, 64), torch.ones(5, device=DEV)), want[:, :1].expand(1, 5))
 
 
 def test_layer_protocol_on_the_device():

@@ -121,6 +121,12 @@ def test_other_entries_refuse():
     assert L.ss_seq_int8_linear(None, 8, 256, 256, 8, 256, None, 256, 1, 8, 8, 0, None, None) == -22
 
 
+def test_product_entry_refuses_more_than_a_grid_holds():
+    L = _lib()
+    for M, N in ((2 ** 27 + 1, 8), (8, 2 ** 27 + 1), (2 ** 27, 2 ** 27), (2 ** 19, 2 ** 19)):
+        assert L.ss_seq_int8_linear(256, 16, 256, 256, 16, 256, None, 256, M, N, 16, 0, 256, None) == -22
+
+
 @pytest.fixture
 def anywhere(monkeypatch):
     """The reasons of a refusal behind the device check, on CPU tensors (which the library hands back before it launches anything)."""
