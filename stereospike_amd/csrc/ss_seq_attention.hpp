@@ -57,108 +57,53 @@ int ss_seq_leaky_bf16(const LeakyArgs&, float* ws, hipStream_t);
 namespace {
 
 
-// The recurrence itself, one step after the other with the state in registers: HBM-bound on reading and writing the state when T is small (the single-step
-// call).  A workgroup owns 64 columns of one head's state: thread (g, x) holds rows g + 16 r of columns 4 x .. 4 x + 3.
-template <int DT, int ODT, int R, bool V4> __global__ __launch_bounds__(256, 4) void leaky_steps_kernel(const LeakyArgs p)
-{
-    __shared__ float sa[256], sb[256], red[4][64];
-    const int tid = threadIdx.x, x = tid & 15, g = tid >> 4;
-    const int bh = blockIdx.y, b = bh / p.H, h = bh % p.H, j0 = blockIdx.x * 64 + 4 * x;
-    int n = p.T;
-    if (p.lengths) { n = p.lengths[b]; n = n < 0 ? 0 : n > p.T ? p.T : n; }
-    const float lam = expf(p.log_decay[h]);
-    const elem_t<DT>* pa = static_cast<const elem_t<DT>*>(p.a) + b * p.a_b + (h / p.a_group) * p.a_h;
-    const elem_t<DT>* pb = static_cast<const elem_t<DT>*>(p.b) + b * p.b_b + (h / p.b_group) * p.b_h;
-    const elem_t<DT>* pc = static_cast<const elem_t<DT>*>(p.c) + b * p.c_b + (h / p.c_group) * p.c_h;
-    elem_t<ODT>* po = static_cast<elem_t<ODT>*>(p.out) + b * p.o_b + h * p.o_h;
-    const float* s_in = p.s_in ? p.s_in + (long long)bh * p.DA * p.DC : nullptr;
-    float* s_out = p.s_out ? p.s_out + (long long)bh * p.DA * p.DC : nullptr;
-    f32x4 S[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int i = min(g + 16 * r, p.DA - 1);           // (outside: the nearest inside, never used or stored)
-        if (!s_in) S[r] = (f32x4){0.f, 0.f, 0.f, 0.f};
-        else if constexpr (V4) S[r] = *reinterpret_cast<const f32x4*>(s_in + i * p.s_in_row + min(j0, p.DC - 4));
-        else S[r] = (f32x4){s_in[i * p.s_in_row + min(j0, p.DC - 1) * p.s_in_col], s_in[i * p.s_in_row + min(j0 + 1, p.DC - 1) * p.s_in_col],
-                            s_in[i * p.s_in_row + min(j0 + 2, p.DC - 1) * p.s_in_col], s_in[i * p.s_in_row + min(j0 + 3, p.DC - 1) * p.s_in_col]};
-    }
-    for (int i = 0; i < n; ++i) {
-        const long long t = p.reverse ? n - 1 - i : i;
-        __syncthreads();
-        sa[tid] = tid < p.DA ? widen<DT>(pa[t * p.a_t + tid]) * p.o_scale : 0.f;
-        sb[tid] = tid < p.DA ? widen<DT>(pb[t * p.b_t + tid]) * p.b_scale : 0.f;
-        __syncthreads();
-        f32x4 c = {0.f, 0.f, 0.f, 0.f}, o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) if (j0 + e < p.DC) c[e] = widen<DT>(pc[t * p.c_t + j0 + e]);
-        const bool leaks = i > 0 || !p.reverse;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int row = g + 16 * r;                    // rows behind DA: sa, sb are zero there
-            f32x4 s = S[r];
-            if (leaks) s = s * lam;
-            s += sb[row] * c;
-            o += sa[row] * s;
-            S[r] = s;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            o[e] += __shfl_xor(o[e], 16);
-            o[e] += __shfl_xor(o[e], 32);
-        }
-        if ((tid & 48) == 0) *reinterpret_cast<f32x4*>(&red[tid >> 6][4 * x]) = o;
-        __syncthreads();
-        if (tid < 64 && blockIdx.x * 64 + tid < p.DC)
-            po[t * p.o_t + blockIdx.x * 64 + tid] = narrow<ODT>(red[0][tid] + red[1][tid] + red[2][tid] + red[3][tid]);
-    }
-    if (tid < 64 && blockIdx.x * 64 + tid < p.DC)
-        for (int t = n; t < p.T; ++t) po[t * p.o_t + blockIdx.x * 64 + tid] = 0;
-    if (s_out) {
-        const float last = p.reverse && n > 0 ? lam : 1.f;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int i = g + 16 * r;
-            if (i < p.DA) {
-                if constexpr (V4) { if (j0 < p.DC) *reinterpret_cast<f32x4*>(s_out + i * p.s_out_row + j0) = S[r] * last; }
-                else
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) if (j0 + e < p.DC) s_out[i * p.s_out_row + (j0 + e) * p.s_out_col] = S[r][e] * last;
-            }
-        }
-    }
-}
-
-// One step, forward: the state is read, updated and written once (HBM-bound: 8 bytes for each of its values); all R rows of a thread are in flight at once.
-template <int DT, int ODT, int R> __global__ __launch_bounds__(256) void leaky_step_kernel(const LeakyArgs p)
+// One step, S = lambda S + b c^T and out = a^T S (in reverse the leak comes after: s_out = lambda S).  HBM-bound: the state is read, updated and written once,
+// 8 bytes for each of its values.  A workgroup has 64 columns of one head's state, thread (g, x) rows g + 16 r of columns 4 x .. 4 x + 3, all R of them in
+// flight at once.  (512 streams of 16 heads of 128 x 128, bf16: 1.08 GB in 208 us, a large copy's rate; one stream of 8 heads of 64 x 64: 4.0 us,
+// little over an empty launch.)  V4: the state's rows take 16-byte accesses.
+template <int DT, int ODT, int R, bool V4> __global__ __launch_bounds__(256) void leaky_step_kernel(const LeakyArgs p)
 {
     __shared__ float sa[256], sb[256], red[4][64];
     const int tid = threadIdx.x, x = tid & 15, g = tid >> 4;
     const int bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H, j0 = blockIdx.x * 64 + 4 * x;
-    const float* s_in = p.s_in + (long long)bh * p.DA * p.DC + j0;
-    float* s_out = p.s_out + (long long)bh * p.DA * p.DC + j0;
-    const bool live = j0 < p.DC;
+    const bool valid = !p.lengths || p.lengths[b] > 0;     // no step: the state as it is, an output of zeros
     f32x4 S[R];
     // (rows and columns outside are read at the nearest inside: a branch per load would end the loads' flight together)
-    const float* from = live ? s_in : s_in - j0;
+    if (p.s_in) {
+        const float* s_in = p.s_in + (long long)bh * p.DA * p.DC;
 #pragma unroll
-    for (int r = 0; r < R; ++r) S[r] = *reinterpret_cast<const f32x4*>(from + (long long)min(g + 16 * r, p.DA - 1) * p.s_in_row);
-    const float lam = expf(p.log_decay[h]);
+        for (int r = 0; r < R; ++r) {
+            const float* row = s_in + min(g + 16 * r, p.DA - 1) * p.s_in_row;
+            if constexpr (V4) S[r] = *reinterpret_cast<const f32x4*>(row + min(j0, p.DC - 4));
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e) S[r][e] = row[min(j0 + e, p.DC - 1) * p.s_in_col];
+        }
+    } else
+#pragma unroll
+        for (int r = 0; r < R; ++r) S[r] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    const float lam = expf(p.log_decay[h]), before = p.reverse || !valid ? 1.f : lam, after = p.reverse && valid ? lam : 1.f;
     if (tid < p.DA) {
-        sa[tid] = widen<DT>(static_cast<const elem_t<DT>*>(p.a)[b * p.a_b + (h / p.a_group) * p.a_h + tid]) * p.o_scale;
-        sb[tid] = widen<DT>(static_cast<const elem_t<DT>*>(p.b)[b * p.b_b + (h / p.b_group) * p.b_h + tid]) * p.b_scale;
+        sa[tid] = valid ? widen<DT>(static_cast<const elem_t<DT>*>(p.a)[b * p.a_b + (h / p.a_group) * p.a_h + tid]) * p.o_scale : 0.f;
+        sb[tid] = valid ? widen<DT>(static_cast<const elem_t<DT>*>(p.b)[b * p.b_b + (h / p.b_group) * p.b_h + tid]) * p.b_scale : 0.f;
     }
     f32x4 c = {0.f, 0.f, 0.f, 0.f}, o = {0.f, 0.f, 0.f, 0.f};
-    if (live)
+    if (valid)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) c[e] = widen<DT>(static_cast<const elem_t<DT>*>(p.c)[b * p.c_b + (h / p.c_group) * p.c_h + j0 + e]);
+        for (int e = 0; e < 4; ++e)
+            if (j0 + e < p.DC) c[e] = widen<DT>(static_cast<const elem_t<DT>*>(p.c)[b * p.c_b + (h / p.c_group) * p.c_h + j0 + e]);
     __syncthreads();
+    float* s_out = p.s_out ? p.s_out + (long long)bh * p.DA * p.DC : nullptr;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const int row = g + 16 * r;
-        if (live && row < p.DA) {
-            const f32x4 s = S[r] * lam + sb[row] * c;
+        if (j0 < p.DC && row < p.DA) {
+            const f32x4 s = S[r] * before + sb[row] * c;
             o += sa[row] * s;
-            *reinterpret_cast<f32x4*>(s_out + (long long)row * p.s_out_row) = s;
+            if constexpr (V4) { if (s_out) *reinterpret_cast<f32x4*>(s_out + row * p.s_out_row + j0) = s * after; }
+            else if (s_out)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) if (j0 + e < p.DC) s_out[row * p.s_out_row + (j0 + e) * p.s_out_col] = s[e] * after;
         }
     }
 #pragma unroll
@@ -169,19 +114,18 @@ template <int DT, int ODT, int R> __global__ __launch_bounds__(256) void leaky_s
     if ((tid & 48) == 0) *reinterpret_cast<f32x4*>(&red[tid >> 6][4 * x]) = o;
     __syncthreads();
     if (tid < 64 && blockIdx.x * 64 + tid < p.DC)
-        static_cast<elem_t<ODT>*>(p.out)[b * p.o_b + h * p.o_h + blockIdx.x * 64 + tid] = narrow<ODT>(red[0][tid] + red[1][tid] + red[2][tid] + red[3][tid]);
+        static_cast<elem_t<ODT>*>(p.out)[b * p.o_b + h * p.o_h + blockIdx.x * 64 + tid] =
+            valid ? narrow<ODT>(red[0][tid] + red[1][tid] + red[2][tid] + red[3][tid]) : elem_t<ODT>(0);
 }
 
-template <int DT, int ODT> int steps(const LeakyArgs& p, hipStream_t s)
+template <int DT, int ODT> int step(const LeakyArgs& p, hipStream_t s)
 {
     const bool v4 = p.DC % 4 == 0 && (!p.s_in || (p.s_in_col == 1 && p.s_in_row % 4 == 0 && aligned(p.s_in, 16))) &&
                     (!p.s_out || (p.s_out_col == 1 && p.s_out_row % 4 == 0 && aligned(p.s_out, 16)));
     const dim3 grid((unsigned)((p.DC + 63) / 64), (unsigned)(p.B * p.H));
-    const bool one = p.T == 1 && !p.reverse && v4 && p.s_in && p.s_out && !p.lengths;
     auto go = [&](auto R) {
-        if (one) leaky_step_kernel<DT, ODT, R.value><<<grid, 256, 0, s>>>(p);
-        else if (v4) leaky_steps_kernel<DT, ODT, R.value, true><<<grid, 256, 0, s>>>(p);
-        else leaky_steps_kernel<DT, ODT, R.value, false><<<grid, 256, 0, s>>>(p);
+        if (v4) leaky_step_kernel<DT, ODT, R.value, true><<<grid, 256, 0, s>>>(p);
+        else leaky_step_kernel<DT, ODT, R.value, false><<<grid, 256, 0, s>>>(p);
         return launched();
     };
     if (p.DA <= 64) return go(std::integral_constant<int, 4>());
@@ -197,8 +141,9 @@ template <int DT, int ODT> int steps(const LeakyArgs& p, hipStream_t s)
 //         + lambda^i a_i W                                 (3)
 //   W    <- lambda^CH W + sum_j lambda^(CH-j) b_j c_j^T    (4)
 //
-// A workgroup of WV (4 or 8) wavefronts owns 16 WV columns of one head's state for one SEGMENT of the steps; a wavefront owns 16 of them, with all DA rows
-// of W in its registers.
+// A workgroup owns a block of columns of one head's state for one SEGMENT of the steps, a wavefront 16 or 32 of them with all DA rows of W in its registers.
+// Several segments: a first pass computes what each adds to the state (STATE: (4) alone, of b and c), a scan or the second pass joins them, the second pass
+// computes the outputs.  That reads b and c twice, which costs less than the steps one after the other: a head's time axis is cut until the card is filled.
 // Products are taken so that accumulators ARE the next product's operand: a 16 x 16 accumulator gives lane l rows 4 (l / 16) .. + 3 of column l % 16; two
 // of them, one above the other, are the 8 contraction values of a 16x16x32 operand in the order {4g .. 4g+3, 16+4g .. 16+4g+3} (four 16x16x4 operands in
 // fp32).  a and b are staged in LDS in that order, so W never leaves the registers; P is shared between the wavefronts through LDS in operand order.
@@ -262,7 +207,9 @@ __device__ __forceinline__ unsigned round_pk(float lo, float hi)
 }
 
 // The tile form on fp32 operands: the 16x16x4 fp32 matrix instructions, a workgroup of WV (4 or 8) wavefronts with 16 columns each, two workgroups on a CU.
-// Bound by those instructions (157 TFLOP/s), so the 16-row tiles behind DA and the wavefronts behind DC are left out.
+// Bound by those instructions (157 TFLOP/s) and, where streams are ragged, by the longest one's chunks in a row (5 us each with 128 columns, 3.5 of them the
+// instructions' own); the 16-row tiles behind DA and the wavefronts behind DC are left out (training, 48 heads of 80 and 96, 777 steps: 218 -> 196 us).  Blocks of
+// 64 columns with twice the workgroups took 203.
 template <int DA, int WV, bool STATE>
 __global__ __launch_bounds__(64 * WV, DA == 64 || (DA == 128 && WV == 8) ? 4 : 2) void leaky_chunk_kernel(const LeakyMaps maps)
 {
@@ -505,6 +452,9 @@ __global__ __launch_bounds__(64 * WV, DA == 64 || (DA == 128 && WV == 8) ? 4 : 2
 // The tile form on 16-bit operands: chunks of 32 steps, a workgroup of four wavefronts owns 64 NT columns, a wavefront 16 NT of them (W: DA x 16 NT in its
 // registers).  a, b, c of the next chunk are on their way to registers while this one is computed, then go to the other of two LDS buffers: one barrier for
 // the buffers and one for P per chunk, two workgroups on a CU.
+// Bound by the vector instructions beside the products (of 625 in a wavefront's chunk 71 are products; the split of lambda^(CH-j) c and the conversions of W lead),
+// the output pass near memory too: 64 heads of 128 x 128, 4096 steps, bf16: 30 us for the states (134 MB), 10 for the scan, 77 for the outputs (300 MB).
+// Chunks of 64 steps in eight wavefronts took 209 us for the whole, this form 118.
 // Rows are unpadded; the 16-byte granule q of row r lies in slot q ^ f(r), f chosen so that the three ways they are read (a granule of 16 rows, half granules
 // of 16 rows, and the transposing 4 x 16 read) meet no bank twice.
 // ---------------------------------------------------------------------------------------------------------------------------------------------------------
@@ -924,7 +874,7 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
     }
 }
 
-// ws[s] (what segment s adds to the state) -> the state that enters segment s + 1
+// ws[s] (what segment s adds to the state) -> the state that enters segment s + 1, in fp32.  HBM-bound (64 heads of 128 x 128, 7 states: 59 MB in 10 us).
 __global__ __launch_bounds__(256) void leaky_scan_kernel(float* __restrict__ ws, const float* __restrict__ log_decay, int H, int ncb, int per, int nstate, int seg)
 {
     const unsigned parts = per / 1024, head = blockIdx.x / parts, bh = head / ncb;
@@ -944,8 +894,6 @@ __global__ __launch_bounds__(256) void leaky_scan_kernel(float* __restrict__ ws,
         at += (long long)U * per;
     }
 }
-
-constexpr int kStepsMax = 8;                 // calls of fewer steps walk the recurrence
 
 template <int DT> struct LeakyShape {
     static constexpr int CH = 32;
@@ -982,7 +930,7 @@ template <int DT> struct LeakyShape {
     }
     static long long state_floats(int T, int B, int H, int DA, int DC)
     {
-        if (T < kStepsMax) return 0;
+        if (T == 1) return 0;
         const LeakyPlan r = plan(T, B, H, DA, DC);
         return (long long)B * H * (r.nseg - 1) * (r.ncb * r.dcb) * pad(DA);
     }
@@ -1030,7 +978,9 @@ template <int DT> struct LeakyShape {
     }
     static int run(const LeakyArgs& p, float* ws, hipStream_t s)
     {
-        if (p.T < kStepsMax) return p.out_f32 ? steps<DT, SS_SEQ_F32>(p, s) : steps<DT, DT>(p, s);
+        // one step has its own kernel; from two on a tile (8 heads of 64 x 64, bf16: a kernel that walks the steps 4.8 us for 2, 6.4 for 4, 9.3 for 7, the tile form
+        // 6.5 for any; 128 heads of 128 x 128: 54, 70 and 95 against 14)
+        if (p.T == 1) return p.out_f32 ? step<DT, SS_SEQ_F32>(p, s) : step<DT, DT>(p, s);
         const LeakyPlan r = plan(p.T, p.B, p.H, p.DA, p.DC);
         if (int rc = states(p, r, ws, s)) return rc;
         LeakyMaps one{{map_of(p, r, ws, false)}, 0};
@@ -1047,7 +997,7 @@ template <int DT> struct LeakyShape {
     {
         const int group = d.H / d.Hk;
         float *each_k = d.ws, *each_v = each_k + heads_floats(d, d.Dk), *rstate = each_v + heads_floats(d, d.Dv);      // gradients by query head
-        const bool tiles = d.T >= kStepsMax;
+        const bool tiles = d.T > 1;
         const LeakyPlan fwd = plan(d.T, d.B, d.H, d.Dk, d.Dv);
         if (bwd_floats(d) && (!d.ws || !aligned(d.ws, 16))) return SS_SEQ_EINVAL;
         if (tiles && fwd.nseg > 1 && d.g_q && (!d.states || !aligned(d.states, 16))) return SS_SEQ_EINVAL;
@@ -1070,7 +1020,7 @@ template <int DT> struct LeakyShape {
         LeakyArgs pk = map(d.Dv, d.Dk, 1, d.scale, 1.f, d.v, d.g, d.q, group == 1 ? d.g_k : each_k, group > 1 || DT == SS_SEQ_F32);
         pk.s_in = d.g_last; pk.s_in_row = 1; pk.s_in_col = d.Dv;
         if (!tiles) {
-            auto go = [&](const LeakyArgs& p) { return p.out_f32 ? steps<DT, SS_SEQ_F32>(p, s) : steps<DT, DT>(p, s); };
+            auto go = [&](const LeakyArgs& p) { return p.out_f32 ? step<DT, SS_SEQ_F32>(p, s) : step<DT, DT>(p, s); };
             if (d.g_q) if (int rc = go(pq)) return rc;
             if (d.g_v) if (int rc = go(pv)) return rc;
             if (d.g_k) if (int rc = go(pk)) return rc;

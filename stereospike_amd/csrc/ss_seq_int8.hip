@@ -31,7 +31,7 @@ __device__ __forceinline__ float scaled(int acc, float as, float ws, float bias)
 // 16 (l / 16), so one load of a wavefront is 64 consecutive bytes of 16 rows, and the product gives lane l rows 4 (l / 16) .. + 3 of X against row l % 16 of Y.
 // The four wavefronts of a workgroup take every fourth 64 k of the same 16 rows of X (256 consecutive bytes of a row at a time) and add up in LDS.
 // SWAP: X is a (few channels), else X is w (few tokens).
-// 1 x 8192 x 4096 (33.6 MB): see the table of the sequence operators for its time.
+// (1 x 8192 x 4096, 33.6 MB: 8.2 us, 4.1 TB/s: 128 KB of each workgroup's rows are one burst and its latency.)
 // ---------------------------------------------------------------------------------------------------------------------------------------------------------
 template <int DT, int MT, bool SWAP> __global__ __launch_bounds__(256) void mm_rows_kernel(const MmArgs p)
 {
@@ -104,7 +104,8 @@ template <int DT, int MT, bool SWAP> __global__ __launch_bounds__(256) void mm_r
 // tile: WM x WN wavefronts, each 32 TI channels x 32 TJ tokens in v_mfma_i32_32x32x32_i8 (lane l: row l % 32, 16 k from 16 (l / 32); taken as w a^T, so a
 // lane ends with four consecutive channels of one token).  128 k per step: rows of 128 bytes travel global -> LDS without registers into the other of two
 // buffers while this step is computed; granule q of row r lies in slot q ^ (r / 2 % 8), which 16 rows of one granule read without a bank conflict.  The result
-// goes through LDS once more, so that stores are whole 128-byte lines.
+// goes through LDS once more, so that stores are whole 128-byte lines.  (8192 x 8192 x 4096, spread codes: 550 GOP in 277 us, 1985 TOP/s; the library's product of
+// 8192 cubed reaches 2110.  29920 x 512 x 4608: 141 GOP in 72 us.)  Bound by the matrix cores with LDS reads beside them: 8 fragments feed 8 products.
 // ---------------------------------------------------------------------------------------------------------------------------------------------------------
 struct TileGrid {
     int tm, tn;                             // tiles
@@ -279,16 +280,29 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mm_tile_kernel(const MmArgs p
     }
 }
 
-// the parts' sums, scaled
-template <int DT> __global__ __launch_bounds__(256) void mm_join_kernel(const MmArgs p, const int* __restrict__ part, int parts)
+// the parts' sums, scaled; V consecutive outputs of a thread, 8 parts in flight
+template <int DT, int V> __global__ __launch_bounds__(256) void mm_join_kernel(const MmArgs p, const int* __restrict__ part, int parts)
 {
+    struct alignas(4 * V) Sums { int v[V]; };
     const long long mn = p.M * p.N;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < mn; i += (long long)gridDim.x * 256) {
-        int s = part[i];
-        for (int k = 1; k < parts; ++k) s += part[k * mn + i];
+    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * V; i < mn; i += (long long)gridDim.x * 256 * V) {
+        Sums s = *reinterpret_cast<const Sums*>(part + i);
+        for (int k = 1; k < parts; k += 8) {
+            Sums x[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) x[u] = *reinterpret_cast<const Sums*>(part + min(k + u, parts - 1) * mn + i);
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (k + u < parts)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) s.v[e] += x[u].v[e];
+        }
         const long long m = i / p.N;
         const int n = (int)(i - m * p.N);
-        static_cast<elem_t<DT>*>(p.out)[i] = narrow<DT>(scaled(s, p.as[m], p.wsc[n], p.bias ? p.bias[n] : 0.f));
+        Pack<DT, V> o;
+#pragma unroll
+        for (int e = 0; e < V; ++e) o.v[e] = narrow<DT>(scaled(s.v[e], p.as[m], p.wsc[n + e], p.bias ? p.bias[n + e] : 0.f));
+        *reinterpret_cast<Pack<DT, V>*>(static_cast<elem_t<DT>*>(p.out) + i) = o;
     }
 }
 
@@ -318,20 +332,25 @@ struct MmPlan {
 MmPlan choose(long long M, int N, int K, bool a_ok, bool w_ok)
 {
     MmPlan r{};
-    // few rows on one side: the other side's bytes are all that matters.  From 65 rows on the streamed form would read the small operand more often than
-    // the large one is worth, and the tile form's reuse wins.
-    if (M <= 64 && M <= N) { r.form = 0; return r; }
+    // few rows on one side: the other side's bytes are all that matters.  (N = K = 4096: 33 rows streamed 11.3 us, tiles 11.8; 48 rows 12.7 and 12.6; 64 rows 14.5
+    // and 13.5; N = 512, K = 4608: 64 rows 14.6 and 10.5.  Few channels are streamed up to 64: 4096 rows, 64 channels 13.7 us, tiles 14.3.)
+    if (M <= 32 && M <= N) { r.form = 0; return r; }
     if (N <= 64) { r.form = 1; return r; }
     const long long t256 = ((M + 255) / 256) * ((N + 255) / 256), t128 = ((M + 127) / 128) * ((N + 127) / 128);
     const int all = (K + 127) / 128;
-    // 256 x 256 reads each operand half as often as 128 x 128, but needs a tile for most CUs: from 192 tiles on (three quarters of 256)
-    r.form = t256 >= 192 ? 3 : 2;
+    // 256 x 256 reads each operand half as often as 128 x 128, but needs a tile for most CUs.  (K = 4096: 48 tiles 58 us, those of 128 27; 80 tiles 59 and 35; 176
+    // tiles 60 to 62 and 62; 208 tiles 61 and 73; 256 tiles 73 and 83.)
+    r.form = t256 >= 176 ? 3 : 2;
     r.parts = 1;
-    if (r.form == 2 && t128 < 256) {        // two workgroups of the 128 form fit a CU: parts until there are some 512, of 4 steps at least
-        long long parts = 512 / t128;
-        if (parts > all / 4) parts = all / 4;
-        if (parts < 1) parts = 1;
-        r.parts = (int)parts;
+    if (r.form == 2 && t128 < 256) {
+        // Parts of k: the count with the least estimated time in us, 0.75 for a step of 128 k and 2 around them, 4 for the joining launch and the partials' way out
+        // and in at 4 TB/s; two workgroups fit a CU.  (512 x 512 x 4608: whole 24.6 us, 6 parts 13.0; 256 x 256 x 16384: 74 and 14.8 in 32 parts; 1536 x 1536 x 1024:
+        // whole 10.6, two parts 20.7.)
+        double least = 0.;
+        for (int n = 1; n <= 512 / t128 && n <= all; ++n) {
+            const double t = ((all + n - 1) / n) * 0.75 + 2. + (n > 1 ? 4. + (double)n * M * N * 8e-6 / 4. : 0.);
+            if (n == 1 || t < least) { r.parts = n; least = t; }
+        }
     }
     r.steps = (all + r.parts - 1) / r.parts;
     r.parts = (all + r.steps - 1) / r.steps;
@@ -354,8 +373,11 @@ template <int DT, int WM, int WN, int TI, int TJ> int tiles(const MmArgs& p, con
     mm_tile_kernel<DT, WM, WN, TI, TJ><<<dim3((unsigned)(tg.tm * tg.tn), (unsigned)r.parts), Sh::THREADS, 0, s>>>(p, tg);
     if (int rc = launched()) return rc;
     if (tg.part) {
-        const long long want = (p.M * p.N + 255) / 256;
-        mm_join_kernel<DT><<<(unsigned)(want < 4096 ? want : 4096), 256, 0, s>>>(p, tg.part, r.parts);
+        const bool four = p.N % 4 == 0 && aligned(p.out, 16);
+        const long long want = (p.M * p.N / (four ? 4 : 1) + 255) / 256;
+        const unsigned grid = (unsigned)(want < 4096 ? want : 4096);
+        if (four) mm_join_kernel<DT, 4><<<grid, 256, 0, s>>>(p, tg.part, r.parts);
+        else mm_join_kernel<DT, 1><<<grid, 256, 0, s>>>(p, tg.part, r.parts);
         return launched();
     }
     return SS_SEQ_OK;
