@@ -249,7 +249,7 @@ __global__ __launch_bounds__(64 * WV, DA == 64 || (DA == 128 && WV == 8) ? 4 : 2
     if (seg == 0) {
         if (p.s_in) {
             const float* s_in = p.s_in + (long long)bh * p.DA * p.DC;
-            const float first = p.reverse || n == 0 ? 1.f : exp2f(gl);
+            const float first = exp2f(gl * (float)((p.reverse || n == 0 ? 0 : 1) + (STATE ? plan.seg : 0)));
 #pragma unroll
             for (int kt = 0; kt < KA; ++kt)
 #pragma unroll
@@ -372,14 +372,18 @@ __global__ __launch_bounds__(64 * WV, DA == 64 || (DA == 128 && WV == 8) ? 4 : 2
         }
         if (!on) continue;
         // (2) and (4) share the wavefront's columns of c
-        const float keep = exp2f(gl * (float)e);
+        // (the state pass weighs by the distance to the segment's end, so W only accumulates)
+        const float tail = STATE ? exp2f(gl * (float)(stop - CH - i0)) : 1.f;
+        if constexpr (!STATE) {
+            const float keep = exp2f(gl * (float)e);
 #pragma unroll
-        for (int kt = 0; kt < KA; ++kt) W[kt] *= keep;
+            for (int kt = 0; kt < KA; ++kt) W[kt] *= keep;
+        }
         bool wild = false;
         float fc[2][4];
 #pragma unroll
         for (int jt = 0; jt < 2; ++jt) {
-            const f32x4 w = *reinterpret_cast<const f32x4*>(rw + 16 * jt + 4 * g);
+            const f32x4 w = *reinterpret_cast<const f32x4*>(rw + 16 * jt + 4 * g) * tail;
             float fin[4];                                                // without what is not finite: 0 * NaN would reach steps before it
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -453,7 +457,7 @@ __global__ __launch_bounds__(64 * WV, DA == 64 || (DA == 128 && WV == 8) ? 4 : 2
 // registers).  a, b, c of the next chunk are on their way to registers while this one is computed, then go to the other of two LDS buffers: one barrier for
 // the buffers and one for P per chunk, two workgroups on a CU.
 // Bound by the vector instructions beside the products (of 625 in a wavefront's chunk 71 are products; the split of lambda^(CH-j) c and the conversions of W lead),
-// the output pass near memory too: 64 heads of 128 x 128, 4096 steps, bf16: 30 us for the states (134 MB), 10 for the scan, 77 for the outputs (300 MB).
+// the output pass near memory too: 64 heads of 128 x 128, 4096 steps, bf16: 34 us for the states (134 MB), 10 for the scan, 77 for the outputs (300 MB).
 // Chunks of 64 steps in eight wavefronts took 209 us for the whole, this form 118.
 // Rows are unpadded; the 16-byte granule q of row r lies in slot q ^ f(r), f chosen so that the three ways they are read (a granule of 16 rows, half granules
 // of 16 rows, and the transposing 4 x 16 read) meet no bank twice.
@@ -524,7 +528,7 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
         if (seg == 0) {
             if (p.s_in) {
                 const float* s_in = p.s_in + (long long)bh * p.DA * p.DC;
-                const float first = p.reverse || n == 0 ? 1.f : exp2f(gl);
+                const float first = exp2f(gl * (float)((p.reverse || n == 0 ? 0 : 1) + (STATE ? plan.seg : 0)));
 #pragma unroll
                 for (int kt = 0; kt < KA; ++kt)
 #pragma unroll
@@ -740,7 +744,9 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
         float c_down[NT];
         bool wild = false;
         {
-            const f32x4 w0 = *reinterpret_cast<const f32x4*>(rw + 4 * g), w1 = *reinterpret_cast<const f32x4*>(rw + 16 + 4 * g);
+            // (the state pass weighs by the distance to the segment's end, so W only accumulates)
+            const float tail = STATE ? exp2f(gl * (float)(stop - CH - i0)) : 1.f;
+            const f32x4 w0 = *reinterpret_cast<const f32x4*>(rw + 4 * g) * tail, w1 = *reinterpret_cast<const f32x4*>(rw + 16 + 4 * g) * tail;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const char* q = lc + (oc ^ (32 * nt));
@@ -817,7 +823,7 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
                         }
                 }
         if constexpr (!STATE) store(i0, acc);
-        const float keep = e == CH ? keep_all : exp2f(gl * (float)e);
+        const float keep = STATE ? 1.f : e == CH ? keep_all : exp2f(gl * (float)e);
 #pragma unroll
         for (int kt = 0; kt < KA; ++kt) {
             const char* q = lb + (o4 ^ (32 * kt));
@@ -830,10 +836,10 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) d[nt] = mfma16<DT>(fb, t0[nt], d[nt]);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) W[kt][nt] = W[kt][nt] * keep + d[nt] * c_down[nt];
+                for (int nt = 0; nt < NT; ++nt) W[kt][nt] = (STATE ? W[kt][nt] : W[kt][nt] * keep) + d[nt] * c_down[nt];
             } else {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) W[kt][nt] = mfma16<DT>(fb, t2[nt], W[kt][nt] * keep);
+                for (int nt = 0; nt < NT; ++nt) W[kt][nt] = mfma16<DT>(fb, t2[nt], STATE ? W[kt][nt] : W[kt][nt] * keep);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) W[kt][nt] = mfma16<DT>(fb, t1[nt], W[kt][nt]);
 #pragma unroll

@@ -95,6 +95,8 @@ def leaky_attention(q_seq: torch.Tensor, k_seq: torch.Tensor, v_seq: torch.Tenso
     lambda (1 - 1 / tau of a leaky integrator; -inf forgets at once).  scale: Dk ** -0.5 by default.
     state: fp32 [B, H, Dk, Dv], S before the first step (None: zero).  lengths: int32 [B] on the device, the valid steps of each stream (clamped to 0 .. T);
     rows behind them are not read, their outputs and gradients are zero.
+    A NaN or an infinity reaches its own step's output and, through the state, its head's later steps (a value's: in its column), never an earlier step, another
+    stream or another head; the state's entries that held it are infinite or NaN from there on.
     Returns o_seq [T, B, H, Dv]; with return_state also the state after the last valid step (fp32).  States, sums and decays are fp32.  Gradients: q, k, v and
     state, from both results."""
     out, last = _call('leaky_attention', lambda: _refuse_attention(q_seq, k_seq, v_seq, log_decay, state, lengths, 2), q_seq, k_seq, v_seq, log_decay, scale, state, lengths)
