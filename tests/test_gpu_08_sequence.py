@@ -168,6 +168,14 @@ def test_leaky_attention_around_a_tile(T, dtype):
     leaky_check(T, 7, 2, 1, 65, 129, dtype, state=True, ragged=True, grads=True)
 
 
+@pytest.mark.parametrize('shape', [(1, 7, 4, 2, 33, 65), (1, 2, 3, 1, 128, 64), (1, 1, 2, 2, 200, 7), (2, 7, 4, 2, 16, 16), (3, 1, 6, 2, 80, 96)])
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_leaky_attention_of_few_steps(shape, dtype):
+    """One step with shared heads, lengths of 0 and 1 and rows of any alignment, and its neighbours."""
+    leaky_check(*shape, dtype, state=True, ragged=True, grads=True)
+    leaky_check(*shape, dtype, state=False, ragged=False, grads=True, seed=2)
+
+
 @pytest.mark.parametrize('T', [1, 3, 40, 700])
 @pytest.mark.parametrize('dtype', DTYPES)
 def test_a_decay_that_is_not_a_number_stays_in_its_head(T, dtype):
