@@ -3,14 +3,29 @@
 
 namespace {
 
-template <int DT> __global__ __launch_bounds__(256) void group_sum_kernel(const float* __restrict__ x, elem_t<DT>* __restrict__ out, long long n, int group, int D)
+// the gradient of a shared head: the sum over its `group` query heads in their order, fp32; V consecutive values of a thread, the heads' loads in flight together.
+// HBM-bound (4662 rows of 8 heads of 96, fp32: 14.3 MB read, 7.2 written in 5 us)
+template <int DT, int V> __global__ __launch_bounds__(256) void group_sum_kernel(const float* __restrict__ x, elem_t<DT>* __restrict__ out, long long n, int group, int D)
 {
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-        const long long r = i / D;
+    typedef Pack<SS_SEQ_F32, V> F;
+    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * V; i < n; i += (long long)gridDim.x * 256 * V) {
+        const long long r = n <= 0x7FFFFFFF ? (long long)((unsigned)i / (unsigned)D) : i / D;
         const float* q = x + r * group * D + (i - r * D);
-        float s = q[0];
-        for (int k = 1; k < group; ++k) s += q[(long long)k * D];
-        out[i] = narrow<DT>(s);
+        F s = *reinterpret_cast<const F*>(q);
+        for (int k = 1; k < group; k += 4) {
+            F v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const F*>(q + (long long)min(k + u, group - 1) * D);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (k + u < group)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) s.v[e] += v[u].v[e];
+        }
+        Pack<DT, V> o;
+#pragma unroll
+        for (int e = 0; e < V; ++e) o.v[e] = narrow<DT>(s.v[e]);
+        *reinterpret_cast<Pack<DT, V>*>(out + i) = o;
     }
 }
 
@@ -90,11 +105,18 @@ int ss_seq_group_sum(const float* x, void* out, long long rows, int group, int D
 {
     if (!x || !out || rows < 1 || group < 1 || D < 1) return SS_SEQ_EINVAL;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const long long n = rows * D, want = (n + 255) / 256;
+    const long long n = rows * D;
+    const bool four = D % 4 == 0 && aligned(x, 16) && aligned(out, 16);
+    const long long want = (n / (four ? 4 : 1) + 255) / 256;
     const unsigned grid = (unsigned)(want < 8192 ? want : 8192);
-    if (dtype == SS_SEQ_F32) group_sum_kernel<SS_SEQ_F32><<<grid, 256, 0, s>>>(x, static_cast<float*>(out), n, group, D);
-    else if (dtype == SS_SEQ_F16) group_sum_kernel<SS_SEQ_F16><<<grid, 256, 0, s>>>(x, static_cast<unsigned short*>(out), n, group, D);
-    else if (dtype == SS_SEQ_BF16) group_sum_kernel<SS_SEQ_BF16><<<grid, 256, 0, s>>>(x, static_cast<unsigned short*>(out), n, group, D);
+    auto go = [&](auto DTC) {
+        constexpr int DT = DTC.value;
+        if (four) group_sum_kernel<DT, 4><<<grid, 256, 0, s>>>(x, static_cast<elem_t<DT>*>(out), n, group, D);
+        else group_sum_kernel<DT, 1><<<grid, 256, 0, s>>>(x, static_cast<elem_t<DT>*>(out), n, group, D);
+    };
+    if (dtype == SS_SEQ_F32) go(std::integral_constant<int, SS_SEQ_F32>());
+    else if (dtype == SS_SEQ_F16) go(std::integral_constant<int, SS_SEQ_F16>());
+    else if (dtype == SS_SEQ_BF16) go(std::integral_constant<int, SS_SEQ_BF16>());
     else return SS_SEQ_EINVAL;
     return launched();
 }
