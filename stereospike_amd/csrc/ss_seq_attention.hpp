@@ -904,11 +904,14 @@ __global__ __launch_bounds__(256) void leaky_scan_kernel(float* __restrict__ ws,
 template <int DT> struct LeakyShape {
     static constexpr int CH = 32;
     static int pad(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
-    static int blocks(int d) { return d <= 128 ? 1 : 2; }
+    // columns of a workgroup's block: 64 where the state of 128 would not leave two workgroups on a CU (16-bit heads over 128 wide; 2048 steps, 32 heads, bf16:
+    // 256 x 256 in blocks of 128 174 us, of 64 119; 192 x 192 167 and 95), else up to 128
+    static int cols(int DA, int DC) { return DC <= 64 || (DT != SS_SEQ_F32 && DA > 128) ? 64 : 128; }
+    static int blocks(int DA, int DC) { return (DC + cols(DA, DC) - 1) / cols(DA, DC); }
     static LeakyPlan plan(int T, int B, int H, int DA, int DC)
     {
         LeakyPlan r;
-        r.ncb = r.sncb = blocks(DC);
+        r.ncb = r.sncb = blocks(DA, DC);
         // Segments: the count with the least estimated time, in chunks.  A round of workgroups (two on a CU; one for fp32, whose matrix instructions one workgroup
         // fills) takes a segment's chunks and two for its state; the state pass half of that; joining costs half a chunk per state in the output pass up to 5
         // segments, else a scan; each further launch two.  (64 heads, 4096 steps, bf16: 4 segments 123 us, 8 108, 16 135; 48 heads, 777 steps, fp32 training:
@@ -930,8 +933,8 @@ template <int DT> struct LeakyShape {
         r.fold = r.nseg <= 5;
         r.trans = 0;
         r.ka = pad(DA) / 16;
-        r.dcb = DC <= 64 ? 64 : 128;
-        r.nt = DT == SS_SEQ_F32 || DC <= 64 ? 1 : 2;
+        r.dcb = cols(DA, DC);
+        r.nt = DT == SS_SEQ_F32 || r.dcb == 64 ? 1 : 2;
         return r;
     }
     static long long state_floats(int T, int B, int H, int DA, int DC)
@@ -967,7 +970,11 @@ template <int DT> struct LeakyShape {
     template <bool STATE> static int pass(LeakyMaps& maps, int count, hipStream_t s)
     {
         const int DA = maps.m[0].p.DA, DC = maps.m[0].p.DC;
-        auto by_dc = [&](auto DAC) { return DC <= 64 ? launch<DAC.value, 4, STATE>(maps, count, s) : launch<DAC.value, 8, STATE>(maps, count, s); };
+        auto by_dc = [&](auto DAC) {
+            if constexpr (DT == SS_SEQ_F32 || DAC.value <= 128)
+                if (cols(DA, DC) == 128) return launch<DAC.value, 8, STATE>(maps, count, s);
+            return launch<DAC.value, 4, STATE>(maps, count, s);
+        };
         return DA <= 64 ? by_dc(std::integral_constant<int, 64>()) : DA <= 128 ? by_dc(std::integral_constant<int, 128>()) : by_dc(std::integral_constant<int, 256>());
     }
     // the states that enter the segments, into ws (nothing where there is one segment)
@@ -1036,7 +1043,7 @@ template <int DT> struct LeakyShape {
             int count = 0;
             auto add = [&](const LeakyArgs& p, float* ws, int trans) {
                 LeakyPlan r = fwd;                         // the forward pass's segments, whatever this map's own sizes
-                r.ncb = blocks(p.DC);
+                r.ncb = blocks(p.DA, p.DC);
                 r.trans = trans;
                 maps.m[count++] = map_of(p, r, ws, false);
             };
