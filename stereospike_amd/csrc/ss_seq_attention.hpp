@@ -966,7 +966,7 @@ template <int DT> struct LeakyShape {
         }
         return launched();
     }
-    // `count` maps of the same padded sizes in one launch
+    // `count` maps of the same padded sizes and column blocks in one launch
     template <bool STATE> static int pass(LeakyMaps& maps, int count, hipStream_t s)
     {
         const int DA = maps.m[0].p.DA, DC = maps.m[0].p.DC;
@@ -1001,7 +1001,7 @@ template <int DT> struct LeakyShape {
     }
 
     // ---- the gradients: three maps.  dq reads the forward pass's states transposed; dk and dv run backwards in time and share the states of (q, g).  dq and
-    // dk are of one shape and run in one launch, with dv where its padded sizes are theirs: the ends of one map's streams fill with the next map's workgroups
+    // dk are of one shape and run in one launch, with dv where its padded sizes and column blocks are theirs: the ends of one map's streams fill with the next map's workgroups
     // (48 heads of 80 and 96, 777 ragged steps, fp32: three launches 196 us a training step, one 158).
     static long long round4(long long n) { return (n + 3) / 4 * 4; }
     static long long heads_floats(const LeakyBwdArgs& d, int D) { return d.H == d.Hk ? 0 : round4((long long)d.T * d.B * d.H * D); }
@@ -1049,7 +1049,7 @@ template <int DT> struct LeakyShape {
             };
             if (d.g_q) add(pq, const_cast<float*>(d.states), 1);
             if (d.g_k) add(pk, rstate, 1);
-            if (d.g_v && pad(d.Dk) != pad(d.Dv) && count) {
+            if (d.g_v && count && !(pad(d.Dk) == pad(d.Dv) && blocks(d.Dk, d.Dv) == blocks(d.Dv, d.Dk))) {
                 if (int rc = pass<false>(maps, count, s)) return rc;
                 count = 0;
             }

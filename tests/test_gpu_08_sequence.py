@@ -176,6 +176,13 @@ def test_leaky_attention_of_few_steps(shape, dtype):
     leaky_check(*shape, dtype, state=False, ragged=False, grads=True, seed=2)
 
 
+@pytest.mark.parametrize('shape', [(70, 2, 2, 1, 160, 256), (70, 2, 2, 2, 256, 160), (40, 1, 2, 1, 130, 193), (600, 1, 2, 2, 96, 65), (600, 2, 2, 1, 192, 129), (70, 1, 2, 2, 32, 96)])
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_leaky_attention_of_unequal_widths(shape, dtype):
+    """Keys and values whose padded widths agree and whose column blocks do not, and the reverse."""
+    leaky_check(*shape, dtype, state=True, ragged=False, grads=True)
+
+
 @pytest.mark.parametrize('T', [1, 3, 40, 700])
 @pytest.mark.parametrize('dtype', DTYPES)
 def test_a_decay_that_is_not_a_number_stays_in_its_head(T, dtype):
