@@ -454,7 +454,7 @@ __global__ __launch_bounds__(64 * WV, DA == 64 || (DA == 128 && WV == 8) ? 4 : 2
 
 // ---------------------------------------------------------------------------------------------------------------------------------------------------------
 // The tile form on 16-bit operands: chunks of 32 steps, a workgroup of four wavefronts owns 64 NT columns, a wavefront 16 NT of them (W: DA x 16 NT in its
-// registers).  a, b, c of the next chunk are on their way to registers while this one is computed, then go to the other of two LDS buffers: one barrier for
+// registers; KA tiles of 16 rows, DA the power of two that its rows in LDS have).  a, b, c of the next chunk are on their way to registers while this one is computed, then go to the other of two LDS buffers: one barrier for
 // the buffers and one for P per chunk, two workgroups on a CU.
 // Bound by the vector instructions beside the products (of 625 in a wavefront's chunk 71 are products; the split of lambda^(CH-j) c and the conversions of W lead),
 // the output pass near memory too: 64 heads of 128 x 128, 4096 steps, bf16: 34 us for the states (134 MB), 10 for the scan, 77 for the outputs (300 MB).
@@ -488,10 +488,10 @@ __device__ __forceinline__ f16x8 half8(const f32x4& x, const f32x4& y, float up)
 // this wavefront's LDS operations are done, then the barrier: unlike __syncthreads() it does not wait for loads on their way to LDS or for stores
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-template <int DT, int DA, int NT, bool STATE, bool VEC>
+template <int DT, int DA, int KA, int NT, bool STATE, bool VEC>
 __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel(const LeakyMaps maps)
 {
-    constexpr int CH = 32, DCB = 64 * NT, KA = DA / 16, SA = DA / 8, SC = DCB / 8;          // SA, SC: granules of a row
+    constexpr int CH = 32, DCB = 64 * NT, SA = DA / 8, SC = DCB / 8;                          // SA, SC: granules of a row
     constexpr int BA = CH * DA, BC = CH * DCB, BUF = (STATE ? 1 : 2) * BA + BC;              // elements of a buffer: [a] b c
     __shared__ __attribute__((aligned(1024))) unsigned short lds[2 * BUF];
     __shared__ __attribute__((aligned(16))) unsigned short sp[STATE ? 8 : 2 * 64 * 8];       // P in operand order, by tile of 16 steps
@@ -666,7 +666,7 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
                 const int it = it1, jt = jt1;
                 f32x4 s = {0.f, 0.f, 0.f, 0.f}, s2 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int k = 0; k < DA / 32; ++k) {
+                for (int k = 0; k < KA / 2; ++k) {
                     const s16x8 xa = *reinterpret_cast<const s16x8*>(la + it * 16 * DA * 2 + (o1 ^ (64 * k)));
                     const s16x8 xb = *reinterpret_cast<const s16x8*>(lb + jt * 16 * DA * 2 + (o1 ^ (64 * k)));
                     if (k & 1) s2 = mfma16<DT>(xb, xa, s2);
@@ -851,7 +851,7 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
 
     if constexpr (STATE) {
         const long long per = (long long)DA * DCB;
-        float* mine = ws + (((long long)bh * plan.ncb + cb) * (plan.nseg - 1) + seg) * per + wv * KA * NT * 256 + lane * 4;
+        float* mine = ws + (((long long)bh * plan.ncb + cb) * (plan.nseg - 1) + seg) * per + wv * (DA / 16) * NT * 256 + lane * 4;
 #pragma unroll
         for (int kt = 0; kt < KA; ++kt)
 #pragma unroll
@@ -904,6 +904,8 @@ __global__ __launch_bounds__(256) void leaky_scan_kernel(float* __restrict__ ws,
 template <int DT> struct LeakyShape {
     static constexpr int CH = 32;
     static int pad(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+    // row tiles of a state in a kernel's registers: three quarters of the padded width where they suffice (16-bit; the fp32 kernel leaves tiles out as it runs)
+    static int row_tiles(int d) { return DT != SS_SEQ_F32 && d > 64 && d <= pad(d) / 4 * 3 ? pad(d) / 64 * 3 : pad(d) / 16; }
     // columns of a workgroup's block: 64 where the state of 128 would not leave two workgroups on a CU (16-bit heads over 128 wide; 2048 steps, 32 heads, bf16:
     // 256 x 256 in blocks of 128 174 us, of 64 119; 192 x 192 167 and 95), else up to 128
     static int cols(int DA, int DC) { return DC <= 64 || (DT != SS_SEQ_F32 && DA > 128) ? 64 : 128; }
@@ -952,7 +954,7 @@ template <int DT> struct LeakyShape {
         const int vec_out = state || (p.DC % 4 == 0 && p.o_t % 4 == 0 && p.o_b % 4 == 0 && p.o_h % 4 == 0 && aligned(p.out, 16) && p.o_t >= 0 && p.o_t < (1 << 24));
         return {p, r, ws, vec, vec_out};
     }
-    template <int DA, int WV, bool STATE> static int launch(LeakyMaps& maps, int count, hipStream_t s)
+    template <int DA, int KA, int WV, bool STATE> static int launch(LeakyMaps& maps, int count, hipStream_t s)
     {
         const LeakyPlan& r = maps.m[0].plan;               // maps of one launch have the same segments and column blocks
         maps.per = (unsigned)(maps.m[0].p.B * maps.m[0].p.H * r.ncb) * (STATE ? r.nseg - 1 : r.nseg);
@@ -961,21 +963,26 @@ template <int DT> struct LeakyShape {
         else {
             bool all = true;
             for (int i = 0; i < count; ++i) all = all && maps.m[i].vec && maps.m[i].vec_out;
-            if (all) leaky_tile_kernel<DT, DA, WV / 4, STATE, true><<<grid, 256, 0, s>>>(maps);
-            else leaky_tile_kernel<DT, DA, WV / 4, STATE, false><<<grid, 256, 0, s>>>(maps);
+            if (all) leaky_tile_kernel<DT, DA, KA, WV / 4, STATE, true><<<grid, 256, 0, s>>>(maps);
+            else leaky_tile_kernel<DT, DA, KA, WV / 4, STATE, false><<<grid, 256, 0, s>>>(maps);
         }
         return launched();
     }
-    // `count` maps of the same padded sizes and column blocks in one launch
+    // `count` maps of the same padded sizes, row tiles and column blocks in one launch
     template <bool STATE> static int pass(LeakyMaps& maps, int count, hipStream_t s)
     {
         const int DA = maps.m[0].p.DA, DC = maps.m[0].p.DC;
-        auto by_dc = [&](auto DAC) {
+        auto by_dc = [&](auto DAC, auto KAC) {
             if constexpr (DT == SS_SEQ_F32 || DAC.value <= 128)
-                if (cols(DA, DC) == 128) return launch<DAC.value, 8, STATE>(maps, count, s);
-            return launch<DAC.value, 4, STATE>(maps, count, s);
+                if (cols(DA, DC) == 128) return launch<DAC.value, KAC.value, 8, STATE>(maps, count, s);
+            return launch<DAC.value, KAC.value, 4, STATE>(maps, count, s);
         };
-        return DA <= 64 ? by_dc(std::integral_constant<int, 64>()) : DA <= 128 ? by_dc(std::integral_constant<int, 128>()) : by_dc(std::integral_constant<int, 256>());
+        auto by_ka = [&](auto DAC) {
+            if constexpr (DT != SS_SEQ_F32 && DAC.value > 64)
+                if (row_tiles(DA) * 16 < DAC.value) return by_dc(DAC, std::integral_constant<int, DAC.value / 16 * 3 / 4>());
+            return by_dc(DAC, std::integral_constant<int, DAC.value / 16>());
+        };
+        return DA <= 64 ? by_ka(std::integral_constant<int, 64>()) : DA <= 128 ? by_ka(std::integral_constant<int, 128>()) : by_ka(std::integral_constant<int, 256>());
     }
     // the states that enter the segments, into ws (nothing where there is one segment)
     static int states(const LeakyArgs& p, const LeakyPlan& r, float* ws, hipStream_t s)
@@ -1001,7 +1008,7 @@ template <int DT> struct LeakyShape {
     }
 
     // ---- the gradients: three maps.  dq reads the forward pass's states transposed; dk and dv run backwards in time and share the states of (q, g).  dq and
-    // dk are of one shape and run in one launch, with dv where its padded sizes and column blocks are theirs: the ends of one map's streams fill with the next map's workgroups
+    // dk are of one shape and run in one launch, with dv where its row tiles and column blocks are theirs: the ends of one map's streams fill with the next map's workgroups
     // (48 heads of 80 and 96, 777 ragged steps, fp32: three launches 196 us a training step, one 158).
     static long long round4(long long n) { return (n + 3) / 4 * 4; }
     static long long heads_floats(const LeakyBwdArgs& d, int D) { return d.H == d.Hk ? 0 : round4((long long)d.T * d.B * d.H * D); }
@@ -1049,7 +1056,7 @@ template <int DT> struct LeakyShape {
             };
             if (d.g_q) add(pq, const_cast<float*>(d.states), 1);
             if (d.g_k) add(pk, rstate, 1);
-            if (d.g_v && count && !(pad(d.Dk) == pad(d.Dv) && blocks(d.Dk, d.Dv) == blocks(d.Dv, d.Dk))) {
+            if (d.g_v && count && !(pad(d.Dk) == pad(d.Dv) && row_tiles(d.Dk) == row_tiles(d.Dv) && blocks(d.Dk, d.Dv) == blocks(d.Dv, d.Dk))) {
                 if (int rc = pass<false>(maps, count, s)) return rc;
                 count = 0;
             }
