@@ -453,9 +453,9 @@ __global__ __launch_bounds__(64 * WV, DA == 64 || (DA == 128 && WV == 8) ? 4 : 2
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------------------------------
-// The tile form on 16-bit operands: chunks of 32 steps, a workgroup of four wavefronts owns 64 NT columns, a wavefront 16 NT of them (W: DA x 16 NT in its
-// registers; KA tiles of 16 rows, DA the power of two that its rows in LDS have).  a, b, c of the next chunk are on their way to registers while this one is computed, then go to the other of two LDS buffers: one barrier for
-// the buffers and one for P per chunk, two workgroups on a CU.
+// The tile form on 16-bit operands: chunks of 32 steps, a workgroup of four wavefronts owns 64 NT columns, a wavefront 16 NT of them (W: KA tiles of 16 rows
+// in its registers; DA is the power of two that rows have in LDS).  a, b, c of the next chunk are on their way to registers while this one is computed, then go to
+// the other of two LDS buffers: one barrier for the buffers and one for P per chunk, two workgroups on a CU.
 // Bound by the vector instructions beside the products (of 625 in a wavefront's chunk 71 are products; the split of lambda^(CH-j) c and the conversions of W lead),
 // the output pass near memory too: 64 heads of 128 x 128, 4096 steps, bf16: 34 us for the states (134 MB), 10 for the scan, 77 for the outputs (300 MB).
 // Chunks of 64 steps in eight wavefronts took 209 us for the whole, this form 118.
@@ -904,7 +904,8 @@ __global__ __launch_bounds__(256) void leaky_scan_kernel(float* __restrict__ ws,
 template <int DT> struct LeakyShape {
     static constexpr int CH = 32;
     static int pad(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
-    // row tiles of a state in a kernel's registers: three quarters of the padded width where they suffice (16-bit; the fp32 kernel leaves tiles out as it runs)
+    // row tiles of a state in a kernel's registers: three quarters of the padded width where they suffice (2048 steps, bf16: 64 heads of 96 x 96 66 -> 61 us, 32 of
+    // 192 x 192 95 -> 81; the fp32 kernel leaves tiles out as it runs)
     static int row_tiles(int d) { return DT != SS_SEQ_F32 && d > 64 && d <= pad(d) / 4 * 3 ? pad(d) / 64 * 3 : pad(d) / 16; }
     // columns of a workgroup's block: 64 where the state of 128 would not leave two workgroups on a CU (16-bit heads over 128 wide; 2048 steps, 32 heads, bf16:
     // 256 x 256 in blocks of 128 174 us, of 64 119; 192 x 192 167 and 95), else up to 128
