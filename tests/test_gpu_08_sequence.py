@@ -734,6 +734,41 @@ def test_captured_gradients_replay():
             assert torch.equal(a, b)
 
 
+def test_captured_gradients_beside_a_living_eager_graph():
+    """A training step captured on aliases of its leaves while an eager graph of the leaves themselves lives: each replay, and the eager backward after it, is right."""
+    g = gen(20)
+    q, k, v = (normal(g, 40, 2, 2, 32).to(DEV).requires_grad_() for _ in range(3))
+    w, decay = (1 + normal(g, 32, std=0.1)).to(DEV).requires_grad_(), torch.tensor([-0.1, -0.01], device=DEV)
+    go = normal(g, 40, 2, 2, 32).to(DEV)
+
+    def run(q, k, v, w):
+        return sequence.add_rms_norm(sequence.leaky_attention(q, k, v, decay), w)[0]
+
+    eager = run(q, k, v, w)
+
+    def step():
+        use = [t.detach().requires_grad_() for t in (q, k, v, w)]
+        return torch.autograd.grad(run(*use), use, go)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    want = torch.autograd.grad(eager, (q, k, v, w), go, retain_graph=True)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    for a, b in zip(torch.autograd.grad(eager, (q, k, v, w), go), want):
+        assert torch.equal(a, b)
+
+
 # ----------------------------------------------------------------------------------------------------------------------------------------------------------
 # offsets that pass 32 bits: what the same values give in a small tensor
 # ----------------------------------------------------------------------------------------------------------------------------------------------------------
