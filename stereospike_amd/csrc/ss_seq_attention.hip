@@ -37,7 +37,8 @@ bool desc_ok(const ss_seq_leaky_desc* d)
     if (d->T < 1 || d->T > (1 << 30) || d->B < 1 || d->H < 1 || (long long)d->B * d->H > 65535 || d->DA < 1 || d->DA > 256 || d->DC < 1 || d->DC > 256) return false;
     if (d->a_group < 1 || d->b_group < 1 || d->c_group < 1 || d->H % d->a_group || d->H % d->b_group || d->H % d->c_group) return false;
     if (!d->a || !d->b || !d->c || !d->out || !d->log_decay) return false;
-    if (d->T > 1 && d->s_in && d->s_in == d->s_out) return false;        // a segment may read the first state after another wrote the last
+    // in place: one step, element for element (a segment may read the first state after another wrote the last)
+    if (d->s_in && d->s_in == d->s_out && (d->T > 1 || d->s_in_row != d->s_out_row || d->s_in_col != d->s_out_col)) return false;
     return true;
 }
 

@@ -121,6 +121,12 @@ def test_other_entries_refuse():
     assert L.ss_seq_int8_linear(None, 8, 256, 256, 8, 256, None, 256, 1, 8, 8, 0, None, None) == -22
 
 
+def test_leaky_entry_refuses_a_state_in_place_of_its_transpose():
+    same = dict(T=1, s_in=512, s_out=512, s_in_row=8, s_in_col=1)
+    for bad in (dict(s_out_row=1, s_out_col=8), dict(s_out_row=16, s_out_col=1)):
+        assert _lib().ss_seq_leaky(ctypes.byref(_desc(**same, **bad)), None) == -22
+
+
 def test_product_entry_refuses_more_than_a_grid_holds():
     L = _lib()
     for M, N in ((2 ** 27 + 1, 8), (8, 2 ** 27 + 1), (2 ** 27, 2 ** 27), (2 ** 19, 2 ** 19)):
