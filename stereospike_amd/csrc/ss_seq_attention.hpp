@@ -149,9 +149,11 @@ template <int DT, int ODT> int step(const LeakyArgs& p, hipStream_t s)
 // fp32).  a and b are staged in LDS in that order, so W never leaves the registers; P is shared between the wavefronts through LDS in operand order.
 // Out comes out transposed: a lane stores four consecutive columns of one step.
 //
-// Rounding (16-bit operands): P and W are rounded to the operands' type for (2) and (3), each term once; (4) splits lambda^(CH-j) c_j into three bf16 or two
-// fp16 terms, so the state keeps fp32 accuracy.  fp16's range is too short for P, W and c's terms: they are scaled by powers of two, taken from the largest value
-// of a tile of P, of a wavefront's columns of W, of a column of c.  fp32 operands run on the fp32 matrix instructions.
+// Rounding (16-bit operands): W is rounded to the operands' type for (3), each term once: half a step of each of DA independent terms, under the output's own
+// rounding.  P has two terms in (2): one value of it serves a whole row of outputs, so its rounding would not average out (few steps, fp16: the error against 64
+// bits was 1.5 times that of outputs rounded once).  (4) splits lambda^(CH-j) c_j into three bf16 or two fp16 terms, so the state keeps fp32 accuracy.
+// fp16's range is too short for P, W and c's terms: they are scaled by powers of two, taken from the largest value of a tile of P, of a wavefront's columns of W,
+// of a column of c.  fp32 operands run on the fp32 matrix instructions.
 // ---------------------------------------------------------------------------------------------------------------------------------------------------------
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef s16x4 __attribute__((address_space(3))) * lds_s16x4;
@@ -472,6 +474,8 @@ template <int DT> __device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, f32x
 }
 // |x|, 0 for what is not finite
 __device__ __forceinline__ float finite(float x) { return fabsf(x) < __builtin_inff() ? fabsf(x) : 0.f; }
+// what is left of x behind its rounded value; 0 where that is not finite
+__device__ __forceinline__ float behind(float x, float rounded) { return fabsf(rounded) < __builtin_inff() ? x - rounded : 0.f; }
 // a power of two that takes `most` into [2^14, 2^15), fp16's upper end, and its inverse; 1 for zero and for what is not finite
 __device__ __forceinline__ void fp16_scale(float most, float& up, float& down)
 {
@@ -492,9 +496,10 @@ template <int DT, int DA, int KA, int NT, bool STATE, bool VEC>
 __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel(const LeakyMaps maps)
 {
     constexpr int CH = 32, DCB = 64 * NT, SA = DA / 8, SC = DCB / 8;                          // SA, SC: granules of a row
+    constexpr int PL = 2 * 64 * 8;
     constexpr int BA = CH * DA, BC = CH * DCB, BUF = (STATE ? 1 : 2) * BA + BC;              // elements of a buffer: [a] b c
     __shared__ __attribute__((aligned(1024))) unsigned short lds[2 * BUF];
-    __shared__ __attribute__((aligned(16))) unsigned short sp[STATE ? 8 : 2 * 64 * 8];       // P in operand order, by tile of 16 steps
+    __shared__ __attribute__((aligned(16))) unsigned short sp[STATE ? 8 : 2 * PL];           // P's two terms in operand order, by tile of 16 steps
     __shared__ __attribute__((aligned(16))) float rw[CH];                                    // lambda^(e - j) b_scale of the chunk's steps
     __shared__ float p_down[4];                                                              // fp16: what undoes the scale of P's three tiles
     constexpr bool H = DT == SS_SEQ_F16;
@@ -629,7 +634,7 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
             }
     };
 
-    if constexpr (!STATE) { if (tid < 128) *reinterpret_cast<f32x4*>(sp + tid * 8) = (f32x4){0.f, 0.f, 0.f, 0.f}; }      // the half of P above the diagonal stays zero
+    if constexpr (!STATE) *reinterpret_cast<f32x4*>(sp + tid * 8) = (f32x4){0.f, 0.f, 0.f, 0.f};         // the half of P above the diagonal stays zero
     if (tid < CH) rw[tid] = exp2f(gl * (float)(CH - tid)) * p.b_scale;
     // lambda^i o_scale of this lane's steps; lambda^(i - j) and both scales for this lane's entries of the wavefront's tile of P (0: above the diagonal)
     const int it1 = (wv + 1) >> 1, jt1 = wv >> 1;
@@ -680,11 +685,22 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
                 if constexpr (H) {
                     float up, down;
                     fp16_scale(wave_max(fmaxf(fmaxf(finite(s[0]), finite(s[1])), fmaxf(finite(s[2]), finite(s[3])))), up, down);
-                    *reinterpret_cast<f16x4*>(sp + (wv * 64 + lane) * 4) = (f16x4){(_Float16)(s[0] * up), (_Float16)(s[1] * up), (_Float16)(s[2] * up), (_Float16)(s[3] * up)};
+                    f16x4 x, z;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        x[r] = (_Float16)(s[r] * up);
+                        z[r] = (_Float16)behind(s[r] * up, (float)x[r]);
+                    }
+                    *reinterpret_cast<f16x4*>(sp + (wv * 64 + lane) * 4) = x;
+                    *reinterpret_cast<f16x4*>(sp + PL + (wv * 64 + lane) * 4) = z;
                     if (lane == 0) p_down[wv] = down;
                 } else {
                     typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+                    f32x4 z;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) z[r] = behind(s[r], (float)(__bf16)s[r]);
                     *reinterpret_cast<u32x2*>(sp + (it * 64 + lane) * 8 + jt * 4) = (u32x2){round_pk(s[0], s[1]), round_pk(s[2], s[3])};
+                    *reinterpret_cast<u32x2*>(sp + PL + (it * 64 + lane) * 8 + jt * 4) = (u32x2){round_pk(z[0], z[1]), round_pk(z[2], z[3])};
                 }
             }
             // (3)
@@ -767,11 +783,17 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
                 if constexpr (!STATE && H) {               // a product of 16 steps for each tile of P, its scale undone as it is added
                     const f16x4 *fp = reinterpret_cast<const f16x4*>(sp) + lane, cl = __builtin_bit_cast(f16x4, (s16x4)__builtin_shufflevector(fin, fin, 0, 1, 2, 3)), ch = __builtin_bit_cast(f16x4, (s16x4)__builtin_shufflevector(fin, fin, 4, 5, 6, 7));
                     const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-                    acc[0][nt] += __builtin_amdgcn_mfma_f32_16x16x16f16(cl, fp[0], z, 0, 0, 0) * p_down[0];
-                    acc[1][nt] += __builtin_amdgcn_mfma_f32_16x16x16f16(cl, fp[64], z, 0, 0, 0) * p_down[1] + __builtin_amdgcn_mfma_f32_16x16x16f16(ch, fp[128], z, 0, 0, 0) * p_down[2];
+                    auto both_terms = [&](const f16x4& c, int t) {
+                        return __builtin_amdgcn_mfma_f32_16x16x16f16(c, fp[64 * t], __builtin_amdgcn_mfma_f32_16x16x16f16(c, fp[PL / 4 + 64 * t], z, 0, 0, 0), 0, 0, 0);
+                    };
+                    acc[0][nt] += both_terms(cl, 0) * p_down[0];
+                    acc[1][nt] += both_terms(cl, 1) * p_down[1] + both_terms(ch, 2) * p_down[2];
                 } else if constexpr (!STATE) {
 #pragma unroll
-                    for (int it = 0; it < 2; ++it) acc[it][nt] = mfma16<DT>(fin, *reinterpret_cast<const s16x8*>(sp + (it * 64 + lane) * 8), acc[it][nt]);
+                    for (int it = 0; it < 2; ++it) {
+                        acc[it][nt] = mfma16<DT>(fin, *reinterpret_cast<const s16x8*>(sp + PL + (it * 64 + lane) * 8), acc[it][nt]);
+                        acc[it][nt] = mfma16<DT>(fin, *reinterpret_cast<const s16x8*>(sp + (it * 64 + lane) * 8), acc[it][nt]);
+                    }
                 }
                 float v[8];
 #pragma unroll
@@ -812,7 +834,8 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
                 for (int it = 0; it < 2; ++it) {
                     if (j > 16 * it + l16) continue;
                     const int jl = 16 * (j >> 2 & 3) + l16;              // the lane that holds P_ij
-                    const float pij = H ? widen<DT>(sp[((it + (j >> 4)) * 64 + jl) * 4 + (j & 3)]) * p_down[it + (j >> 4)] : widen<DT>(sp[(it * 64 + jl) * 8 + (j >> 4) * 4 + (j & 3)]);
+                    const unsigned short* at = sp + (H ? ((it + (j >> 4)) * 64 + jl) * 4 : (it * 64 + jl) * 8 + (j >> 4) * 4) + (j & 3);
+                    const float pij = (widen<DT>(at[0]) + widen<DT>(at[PL])) * (H ? p_down[it + (j >> 4)] : 1.f);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

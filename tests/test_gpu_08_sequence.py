@@ -176,6 +176,18 @@ def test_leaky_attention_of_few_steps(shape, dtype):
     leaky_check(*shape, dtype, state=False, ragged=False, grads=True, seed=2)
 
 
+@pytest.mark.parametrize('T', [2, 9, 32])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_short_sequences_round_their_outputs_once(T, dtype):
+    """Within one tile and without a state only the token-by-token weights lie between operands and outputs, and those have two terms of the operands' type: what is
+    left of them is half a step of a half step, beside the fp32 roundings and the output's own."""
+    for Dk, Dv in ((8, 24), (64, 64), (200, 31)):
+        q, k, v, decay, _, _ = leaky_case(T, 3, 2, 1, Dk, Dv, dtype, False, False, seed=21)
+        o = sequence.leaky_attention(q.to(DEV), k.to(DEV), v.to(DEV), decay.to(DEV))
+        want, size = leaky_ref(q, k, v, decay, Dk ** -0.5)[0], leaky_ref(q.abs(), k.abs(), v.abs(), decay, Dk ** -0.5)[0]
+        within(o, want, size * ((2 * T + Dk + 80) * U + HALF[dtype] ** 2) + want.abs() * HALF[dtype] * 1.02 + TINY[dtype], f'{Dk} x {Dv}')
+
+
 @pytest.mark.parametrize('shape', [(70, 2, 2, 1, 160, 256), (70, 2, 2, 2, 256, 160), (40, 1, 2, 1, 130, 193), (600, 1, 2, 2, 96, 65), (600, 2, 2, 1, 192, 129), (70, 1, 2, 2, 32, 96)])
 @pytest.mark.parametrize('dtype', DTYPES)
 def test_leaky_attention_of_unequal_widths(shape, dtype):
