@@ -458,7 +458,7 @@ __global__ __launch_bounds__(64 * WV, DA == 64 || (DA == 128 && WV == 8) ? 4 : 2
 // The tile form on 16-bit operands: chunks of 32 steps, a workgroup of four wavefronts owns 64 NT columns, a wavefront 16 NT of them (W: KA tiles of 16 rows
 // in its registers; DA is the power of two that rows have in LDS).  a, b, c of the next chunk are on their way to registers while this one is computed, then go to
 // the other of two LDS buffers: one barrier for the buffers and one for P per chunk, two workgroups on a CU.
-// Bound by the vector instructions beside the products (of 625 in a wavefront's chunk 71 are products; the split of lambda^(CH-j) c and the conversions of W lead),
+// Bound by the vector instructions beside the products (of some 630 in a wavefront's chunk 75 are products; the split of lambda^(CH-j) c and the conversions of W lead),
 // the output pass near memory too: 64 heads of 128 x 128, 4096 steps, bf16: 34 us for the states (134 MB), 10 for the scan, 77 for the outputs (300 MB).
 // Chunks of 64 steps in eight wavefronts took 209 us for the whole, this form 118.
 // Rows are unpadded; the 16-byte granule q of row r lies in slot q ^ f(r), f chosen so that the three ways they are read (a granule of 16 rows, half granules
