@@ -149,9 +149,9 @@ template <int DT, int ODT> int step(const LeakyArgs& p, hipStream_t s)
 // fp32).  a and b are staged in LDS in that order, so W never leaves the registers; P is shared between the wavefronts through LDS in operand order.
 // Out comes out transposed: a lane stores four consecutive columns of one step.
 //
-// Rounding (16-bit operands): W is rounded to the operands' type for (3), each term once: half a step of each of DA independent terms, under the output's own
-// rounding.  P has two terms in (2): one value of it serves a whole row of outputs, so its rounding would not average out (few steps, fp16: the error against 64
-// bits was 1.5 times that of outputs rounded once).  (4) splits lambda^(CH-j) c_j into three bf16 or two fp16 terms, so the state keeps fp32 accuracy.
+// Rounding (16-bit operands): W has two terms of the operands' type in (3) and P two in (2), the rounded value and what that leaves, so the output's own rounding is
+// the only one that shows (with one term of W the error against 64 bits was 1.35 - 1.4 times that of outputs rounded once; the second costs 7 - 9 %: T = 4096,
+// 64 heads of 128 x 128, bf16: 135 -> 145 us).  (4) splits lambda^(CH-j) c_j into three bf16 or two fp16 terms (24 and 23 bits), so the state keeps fp32 accuracy.
 // fp16's range is too short for P, W and c's terms: they are scaled by powers of two, taken from the largest value of a tile of P, of a wavefront's columns of W,
 // of a column of c.  fp32 operands run on the fp32 matrix instructions.
 // ---------------------------------------------------------------------------------------------------------------------------------------------------------
@@ -484,10 +484,33 @@ __device__ __forceinline__ void fp16_scale(float most, float& up, float& down)
     up = __uint_as_float((unsigned)(268 - e) << 23);       // 2^(14 - (e - 127))
     down = __uint_as_float((unsigned)(e - 14) << 23);
 }
-__device__ __forceinline__ f16x8 half8(const f32x4& x, const f32x4& y, float up)
+// eight fp32 values, times `up` for fp16, as two terms of the operands' type: the rounded value and what that leaves.  CAREFUL: for any value; else for finite ones
+template <int DT, bool CAREFUL> __device__ __forceinline__ void two_terms(const f32x4& x, const f32x4& y, float up, s16x8& first, s16x8& second)
 {
-    return (f16x8){(_Float16)(x[0] * up), (_Float16)(x[1] * up), (_Float16)(x[2] * up), (_Float16)(x[3] * up),
-                   (_Float16)(y[0] * up), (_Float16)(y[1] * up), (_Float16)(y[2] * up), (_Float16)(y[3] * up)};
+    if constexpr (DT == SS_SEQ_F16) {
+        f16x8 p, q;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float v = (i < 4 ? x[i & 3] : y[i & 3]) * up;
+            p[i] = (_Float16)v;
+            q[i] = (_Float16)(CAREFUL ? behind(v, (float)p[i]) : v - (float)p[i]);
+        }
+        first = __builtin_bit_cast(s16x8, p);
+        second = __builtin_bit_cast(s16x8, q);
+    } else {
+        unsigned p[4];
+        float z[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float a = i < 2 ? x[2 * i] : y[2 * i - 4], b = i < 2 ? x[2 * i + 1] : y[2 * i - 3];
+            p[i] = round_pk(a, b);
+            const float pa = __uint_as_float(p[i] << 16), pb = __uint_as_float(p[i] & 0xFFFF0000u);
+            z[2 * i] = CAREFUL ? behind(a, pa) : a - pa;
+            z[2 * i + 1] = CAREFUL ? behind(b, pb) : b - pb;
+        }
+        first = __builtin_bit_cast(s16x8, mk8(p[0], p[1], p[2], p[3]));
+        second = __builtin_bit_cast(s16x8, mk8(round_pk(z[0], z[1]), round_pk(z[2], z[3]), round_pk(z[4], z[5]), round_pk(z[6], z[7])));
+    }
 }
 // this wavefront's LDS operations are done, then the barrier: unlike __syncthreads() it does not wait for loads on their way to LDS or for stores
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -704,11 +727,8 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
                 }
             }
             // (3)
-#pragma unroll
-            for (int it = 0; it < 2; ++it)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) acc[it][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
             float up = 1.f, down = 1.f;
+            bool odd = false;                                            // this wavefront's W holds an infinity
             if constexpr (H) {
                 float most = 0.f;
 #pragma unroll
@@ -719,6 +739,7 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
                         for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(W[kt][nt][r]));
                 most = wave_max(most);
                 if (most == __builtin_inff()) {                          // rare: the others' scale without what is infinite
+                    odd = true;
                     most = 0.f;
 #pragma unroll
                     for (int kt = 0; kt < KA; ++kt)
@@ -730,23 +751,48 @@ __global__ __launch_bounds__(256, DA * NT <= 256 ? 2 : 1) void leaky_tile_kernel
                 }
                 fp16_scale(most, up, down);
             }
+            // CAREFUL: the second term is 0 behind what is not finite (infinity - infinity would make a NaN of it)
+            auto read = [&](auto CAREFUL) {
 #pragma unroll
-            for (int k = 0; k < KA / 2; ++k) {
-                s16x8 xa[2];
+                for (int it = 0; it < 2; ++it)
 #pragma unroll
-                for (int it = 0; it < 2; ++it) {
-                    const char* q = la + it * 16 * DA * 2 + (o3 ^ (64 * k));
-                    const char* q2 = la + it * 16 * DA * 2 + (o3 ^ (64 * k + 32));
-                    xa[it] = __builtin_shufflevector(*reinterpret_cast<const s16x4*>(q), *reinterpret_cast<const s16x4*>(q2), 0, 1, 2, 3, 4, 5, 6, 7);
+                    for (int nt = 0; nt < NT; ++nt) acc[it][nt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < KA / 2; ++k) {
+                    s16x8 xa[2];
+#pragma unroll
+                    for (int it = 0; it < 2; ++it) {
+                        const char* q = la + it * 16 * DA * 2 + (o3 ^ (64 * k));
+                        const char* q2 = la + it * 16 * DA * 2 + (o3 ^ (64 * k + 32));
+                        xa[it] = __builtin_shufflevector(*reinterpret_cast<const s16x4*>(q), *reinterpret_cast<const s16x4*>(q2), 0, 1, 2, 3, 4, 5, 6, 7);
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const f32x4 x = W[2 * k][nt], z = W[2 * k + 1][nt];
+                        s16x8 f0, f1;
+                        two_terms<DT, CAREFUL.value>(x, z, up, f0, f1);
+#pragma unroll
+                        for (int it = 0; it < 2; ++it) acc[it][nt] = mfma16<DT>(f0, xa[it], mfma16<DT>(f1, xa[it], acc[it][nt]));
+                    }
+                    // the conversions of all of W at once do not fit the registers (32 heads of 256 x 256, bf16: 180 us with the spills, 127 without)
+                    if constexpr (KA * NT >= 12) if (k % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                 }
+            };
+            if constexpr (H) {
+                if (odd) read(std::true_type());
+                else read(std::false_type());
+            } else {
+                read(std::false_type());
+                f32x4 sum = acc[0][0] + acc[1][0];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const f32x4 x = W[2 * k][nt], z = W[2 * k + 1][nt];
-                    s16x8 fw;
-                    if constexpr (H) fw = __builtin_bit_cast(s16x8, half8(x, z, up));
-                    else fw = __builtin_bit_cast(s16x8, mk8(round_pk(x[0], x[1]), round_pk(x[2], x[3]), round_pk(z[0], z[1]), round_pk(z[2], z[3])));
+                for (int nt = 1; nt < NT; ++nt) sum += acc[0][nt] + acc[1][nt];
+                sum[0] += sum[1] + sum[2] + sum[3];
+                if (__any(!(sum[0] == sum[0]))) {                        // rare: again, with care
 #pragma unroll
-                    for (int it = 0; it < 2; ++it) acc[it][nt] = mfma16<DT>(fw, xa[it], acc[it][nt]);
+                    for (int kt = 0; kt < KA; ++kt)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) asm("" : "+v"(W[kt][nt]));       // (or the first terms of all of W are kept for this branch, and spill)
+                    read(std::true_type());
                 }
             }
 #pragma unroll

@@ -188,6 +188,28 @@ def test_short_sequences_round_their_outputs_once(T, dtype):
         within(o, want, size * ((2 * T + Dk + 80) * U + HALF[dtype] ** 2) + want.abs() * HALF[dtype] * 1.02 + TINY[dtype], f'{Dk} x {Dv}')
 
 
+@pytest.mark.parametrize('shape', [(40, 2, 2, 1, 64, 64), (70, 3, 4, 2, 24, 40), (300, 1, 2, 2, 128, 128), (90, 1, 2, 1, 192, 80), (130, 2, 2, 2, 200, 72)])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_sequences_of_many_tiles_round_their_outputs_once(shape, dtype):
+    """Where the state carries the result, and in the gradients: it meets the query in two terms of the operands' type, so what is left of its rounding is half a step
+    of a half step (and, for fp16, 2^-39 of the largest value of a state, scaled to fp16's upper end, at the lower end of that type's range), beside the fp32 roundings
+    and the output's own."""
+    T, B, H, Hk, Dk, Dv = shape
+    q, k, v, decay, s, _ = leaky_case(*shape, dtype, True, False, seed=22)
+    use = [t.to(DEV).requires_grad_() for t in (q, k, v, s)]
+    o = sequence.leaky_attention(*use[:3], decay.to(DEV), state=use[3])
+    go = normal(gen(23), *o.shape, dtype=dtype)
+    got = (o, *torch.autograd.grad(o, use[:3], go.to(DEV)))
+
+    def exact(f):
+        leaf = [f(t).double().requires_grad_() for t in (q, k, v)]
+        o = leaky_ref(*leaf, decay, Dk ** -0.5, f(s))[0]
+        return (o.detach(), *torch.autograd.grad(o, leaf, f(go).double()))
+
+    for name, a, b, m in zip(('o', 'gradient of q', 'gradient of k', 'gradient of v'), got, exact(lambda t: t), exact(torch.abs)):
+        within(a, b, m * ((2 * T + Dk + Dv + 80) * U + HALF[dtype] ** 2) + b.abs() * HALF[dtype] * 1.02 + TINY[dtype], name)
+
+
 @pytest.mark.parametrize('shape', [(70, 2, 2, 1, 160, 256), (70, 2, 2, 2, 256, 160), (40, 1, 2, 1, 130, 193), (600, 1, 2, 2, 96, 65), (600, 2, 2, 1, 192, 129), (70, 1, 2, 2, 32, 96)])
 @pytest.mark.parametrize('dtype', DTYPES)
 def test_leaky_attention_of_unequal_widths(shape, dtype):
