@@ -75,6 +75,10 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_fwd_kernel(const No
             const float t = p.w[min(j, p.C - 1)];
             w[v * VEC + e] = j < p.C ? t : 0.f;
         }
+    bool wild = false;                                     // a weight that is not finite: h * w is not either, whatever h (0 * infinity is a NaN)
+    if constexpr (INT8)
+#pragma unroll
+        for (int i = 0; i < NE; ++i) wild = wild || !(fabsf(w[i]) <= 3.402823466e38f);
     const bool add = p.r != nullptr;
     P px[NV], pr[NV];
     auto load = [&](long long row) {                       // behind the row's end: its last access, counted as zeros below
@@ -142,6 +146,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_fwd_kernel(const No
             if (most == top)
 #pragma unroll
                 for (int i = 0; i < NE; ++i) top64 = fmax(top64, fabs((double)h[i] * (double)w[i]));
+            if (wild) top64 = __builtin_inf();             // (the maxima pass over NaN)
             top64 = row_reduce<TPR, true>(top64, redd);
             broken = broken || !(top64 < 3.4e38);
             const float c = 127.f / top;

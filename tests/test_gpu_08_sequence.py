@@ -486,6 +486,20 @@ def test_norm_int8_ties_zeros_and_what_is_not_finite():
         assert not codes[3:].any() and scales[3] == 0 and scales[4:].isnan().all() and scales[:3].isfinite().all()
 
 
+@pytest.mark.parametrize('C', [5, 64, 1000, 1500, 5000])
+def test_norm_int8_of_weights_that_are_not_finite(C):
+    """h * weight that is not a number, from either side, shows in every row: codes 0, scale NaN, as where h holds one."""
+    x, w, _ = norm_case(6, C, torch.float32, False, seed=C)
+    x[3, C - 2] = 0.
+    for at, bad in ((C - 1, math.nan), (C // 2, math.nan), (C - 2, math.inf), (0, -math.inf)):
+        wb = w.clone()
+        wb[at] = bad
+        for dtype in DTYPES:
+            codes, scales, _ = sequence.add_rms_norm_int8(x.to(dtype).to(DEV), wb.to(DEV))
+            assert not codes.any() and scales.isnan().all(), (at, bad, dtype)
+            assert sequence.dequantize_int8(codes, scales).isnan().all()
+
+
 # ----------------------------------------------------------------------------------------------------------------------------------------------------------
 # 8-bit integer product
 # ----------------------------------------------------------------------------------------------------------------------------------------------------------
