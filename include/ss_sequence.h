@@ -111,7 +111,7 @@ int ss_seq_rms_norm_bwd(const void* g_y, const void* g_sum, const void* h, const
 /*
  * The same norm handed on in 8 bits: u = h * weight, top = max |u| of the row, codes = rint(127 u / top) (ties to even, exact: values next to a border are
  * decided in fp64), scales[row] = top * rstd / 127, so codes * scale is the norm.  A row of zeros has scale 0; a row in
- * which h or the weight holds a NaN or an infinity has codes 0 and scale NaN.
+ * which h or the weight holds a NaN or an infinity has codes 0 and scale NaN (finite values may have products beyond fp32).
  */
 int ss_seq_rms_norm_int8(const void* x, long long x_stride, const void* residual, long long r_stride, const float* weight, signed char* codes, float* scales,
                          void* sum, long long rows, int C, float eps, int dtype, void* stream);

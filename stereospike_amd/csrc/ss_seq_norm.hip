@@ -148,9 +148,9 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_fwd_kernel(const No
                 for (int i = 0; i < NE; ++i) top64 = fmax(top64, fabs((double)h[i] * (double)w[i]));
             if (wild) top64 = __builtin_inf();             // (the maxima pass over NaN)
             top64 = row_reduce<TPR, true>(top64, redd);
-            broken = broken || !(top64 < 3.4e38);
+            broken = broken || !(top64 <= 1.7976931348623157e308);
             const float c = 127.f / top;
-            const bool plain = top > 1e-30f && !broken;    // 127 / top in range
+            const bool plain = top > 1e-30f && top <= 3.402823466e38f && !broken;        // 127 / top in range
             if (lane == 0) p.scales[row] = broken ? __uint_as_float(0x7FC00000u) : top64 == 0. ? 0.f : (float)(top64 * (double)rstd / 127.0);
             int code[NE];
             bool close = !plain;

@@ -500,6 +500,21 @@ def test_norm_int8_of_weights_that_are_not_finite(C):
             assert sequence.dequantize_int8(codes, scales).isnan().all()
 
 
+@pytest.mark.parametrize('C', [64, 1500])
+@pytest.mark.parametrize('size', [1e25, 1e36])
+def test_norm_int8_of_products_beyond_fp32(C, size):
+    """Finite values whose products with the weight pass fp32's largest number: the norm is within it, so codes and scale are."""
+    x, w, _ = norm_case(4, C, torch.float32, False, seed=C)
+    x, w = x * size, w * 1e15
+    codes, scales, _ = sequence.add_rms_norm_int8(x.to(DEV), w.to(DEV))
+    d = x.double()
+    u = d * w.double()
+    top = u.abs().amax(-1, keepdim=True)
+    assert top.max() > 3.5e38 and torch.equal(codes.cpu().double(), torch.round(u * 127. / top))
+    want = (top * (d.square().mean(-1, keepdim=True) + 1e-6).rsqrt() / 127.)[:, 0]
+    within(scales, want, want * NORM_ROOM, 'scales')
+
+
 # ----------------------------------------------------------------------------------------------------------------------------------------------------------
 # 8-bit integer product
 # ----------------------------------------------------------------------------------------------------------------------------------------------------------
