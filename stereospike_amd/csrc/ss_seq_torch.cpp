@@ -5,6 +5,8 @@
 // stereospike_amd/sequence.py turns that into the error that names the operand.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -44,6 +46,13 @@ bool records(std::initializer_list<Tensor> ts)
 {
     if (!at::GradMode::is_enabled()) return false;
     for (const Tensor& t : ts) if (t.defined() && t.requires_grad()) return true;
+    return false;
+}
+// A recording that would hold the outputs' allocation without the launch (torch.jit.trace, a proxy tracer), or a forward-mode tangent, which the outputs would not have.
+bool recorded(std::initializer_list<Tensor> ts)
+{
+    if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value()) return true;
+    for (const Tensor& t : ts) if (t.defined() && t._fw_grad(0).defined()) return true;
     return false;
 }
 // gradients that raise when they are differentiated again (only under create_graph)
@@ -156,7 +165,7 @@ std::optional<std::tuple<Tensor, Tensor>> leaky_attention(const Tensor& q0, cons
 {
     const Tensor& st = given(state0);
     if (!attention_ok(q0, k0, v0, log_decay0, st, given(lengths0), 4)) return std::nullopt;
-    if (at::GradMode::is_enabled() && log_decay0.requires_grad()) return std::nullopt;
+    if ((at::GradMode::is_enabled() && log_decay0.requires_grad()) || recorded({q0, k0, v0, log_decay0, st})) return std::nullopt;
     const c10::DeviceGuard guard(q0.device());
     const double scale = scale0.has_value() ? *scale0 : 1. / std::sqrt((double)q0.size(3));
     const int64_t T = q0.size(0), B = q0.size(1), H = q0.size(2), Dk = q0.size(3), Dv = v0.size(3);
@@ -175,7 +184,7 @@ std::optional<std::tuple<Tensor, Tensor>> leaky_attention(const Tensor& q0, cons
 
 std::optional<Tensor> leaky_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& state, std::optional<double> scale)
 {
-    if (!attention_ok(q, k, v, log_decay, state, Tensor(), 3) || !state.is_contiguous()) return std::nullopt;
+    if (!attention_ok(q, k, v, log_decay, state, Tensor(), 3) || !state.is_contiguous() || recorded({q, k, v, log_decay, state})) return std::nullopt;
     const c10::DeviceGuard guard(q.device());
     const at::NoGradGuard plain;
     const Tensor out = at::empty({q.size(0), q.size(1), v.size(2)}, q.options());
@@ -253,7 +262,7 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
 std::optional<std::tuple<Tensor, Tensor>> add_rms_norm(const Tensor& x, const Tensor& weight, const Maybe& residual0, double eps)
 {
     const Tensor& residual = given(residual0);
-    if (!norm_ok(x, weight, residual, eps)) return std::nullopt;
+    if (!norm_ok(x, weight, residual, eps) || recorded({x, weight, residual})) return std::nullopt;
     const c10::DeviceGuard guard(x.device());
     if (records({x, residual, weight})) {
         const variable_list r = AddRmsNorm::apply(x, weight.contiguous(), residual.defined() ? Maybe(residual) : Maybe(), eps);
@@ -267,7 +276,7 @@ std::optional<std::tuple<Tensor, Tensor>> add_rms_norm(const Tensor& x, const Te
 std::optional<std::tuple<Tensor, Tensor, Tensor>> add_rms_norm_int8(const Tensor& x, const Tensor& weight, const Maybe& residual0, double eps)
 {
     const Tensor& residual = given(residual0);
-    if (!norm_ok(x, weight, residual, eps)) return std::nullopt;
+    if (!norm_ok(x, weight, residual, eps) || recorded({x, weight, residual})) return std::nullopt;
     const c10::DeviceGuard guard(x.device());
     const at::NoGradGuard plain;
     const Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kChar)), scales = at::empty(x.sizes().slice(0, x.dim() - 1), weight.options()),
@@ -283,7 +292,7 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> add_rms_norm_int8(const Tensor
 std::optional<Tensor> dequantize_int8(const Tensor& codes, const Tensor& scales, at::ScalarType dtype)
 {
     if (!codes.is_cuda() || codes.scalar_type() != at::kChar || codes.dim() < 1 || codes.size(-1) < 1 || code_of(dtype) < 0) return std::nullopt;
-    if (!is(scales, codes, at::kFloat, codes.sizes().slice(0, codes.dim() - 1))) return std::nullopt;
+    if (!is(scales, codes, at::kFloat, codes.sizes().slice(0, codes.dim() - 1)) || recorded({scales})) return std::nullopt;
     const c10::DeviceGuard guard(codes.device());
     const at::NoGradGuard plain;
     const Tensor out = at::empty(codes.sizes(), codes.options().dtype(dtype)), c = codes.contiguous(), s = scales.contiguous();
@@ -304,7 +313,7 @@ std::optional<Tensor> int8_linear(const Tensor& codes, const Tensor& scales, con
     if (!is(weight, codes, at::kChar, {N, K}) || codes.size(-1) != K || N < 1 || N > kMaxSide || K < 1 || K > kMaxK || codes.numel() / K > kMaxSide) return std::nullopt;
     if (!is(scales, codes, at::kFloat, codes.sizes().slice(0, codes.dim() - 1)) || !is(weight_scale, codes, at::kFloat, {N})) return std::nullopt;
     if (bias.defined() && !is(bias, codes, at::kFloat, {N})) return std::nullopt;
-    if (records({scales, weight_scale, bias})) return std::nullopt;
+    if (records({scales, weight_scale, bias}) || recorded({scales, weight_scale, bias})) return std::nullopt;
     const c10::DeviceGuard guard(codes.device());
     const at::NoGradGuard plain;
     auto shape = codes.sizes().vec();

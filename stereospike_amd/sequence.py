@@ -10,7 +10,8 @@
 They stand beside the fused neuron layers of `fused.py`: a leaky integrator whose state is a matrix and is read by a query, the gain / skip-add epilogue of a
 layer without spikes, and the product of small-integer activations (spike counts are 8-bit codes of scale 1) with a weight.  Like those they need the HIP
 library and HIP tensors, launch on torch's current stream of the tensors' device, allocate their workspaces from torch's caching allocator and may be recorded
-into a HIP graph; there is no eager fallback.  A backward pass that is itself captured needs leaves whose gradients no live eager graph reaches
+into a HIP graph; there is no eager fallback, and tracers (torch.jit.trace, torch.fx) and
+forward-mode derivatives are refused.  A backward pass that is itself captured needs leaves whose gradients no live eager graph reaches
 (engine.GraphedTrainer shows how).  Gradients are first derivatives: differentiating them again raises.
 
 Calls go straight to the library (csrc/ss_seq_torch.cpp), which checks, allocates and launches; it hands a call with unfit operands back, and the functions
@@ -19,6 +20,8 @@ here then raise the SSNeuronError that names the operand.
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _seqlib
 from ._lib import SSNeuronError, _require_hip
@@ -37,6 +40,14 @@ def _operand(t, name, dev, dtype, shape):
         raise SSNeuronError(f'{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}')
 
 
+def _refuse_recording(name, args):
+    """Raises where a tracer records or an operand has a forward-mode tangent: the trace would hold no launch, the outputs no tangent."""
+    if torch.jit.is_tracing() or get_proxy_mode() is not None:
+        raise SSNeuronError(f'{name} cannot be traced: its kernels are launched outside of torch\'s operators (a HIP graph records them)')
+    if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in args):
+        raise SSNeuronError(f'{name} has no forward-mode derivative')
+
+
 def _call(name, refuse, *args):
     """The library's answer, or the error that `refuse` raises for operands it does not take."""
     try:
@@ -44,6 +55,7 @@ def _call(name, refuse, *args):
     except TypeError:
         r = None                                           # something that is no tensor
     if r is None:
+        _refuse_recording(name, args)
         refuse()
         raise SSNeuronError(f'{name}: operands refused')
     return r

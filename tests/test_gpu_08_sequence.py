@@ -686,6 +686,25 @@ def test_refusals_on_the_device():
         sequence.int8_linear(q.to(torch.int8), torch.ones(3, device=DEV), torch.zeros(5, 8, dtype=torch.int8, device=DEV), torch.ones(5, device=DEV))
 
 
+def test_tracers_and_forward_mode_are_refused_on_the_device():
+    q, g = torch.randn(3, 2, 2, 8, device=DEV), torch.zeros(2, device=DEV)
+    x, c, one = torch.randn(3, 8, device=DEV), torch.zeros(3, 8, dtype=torch.int8, device=DEV), torch.ones(3, device=DEV)
+    w, sw, ones = torch.zeros(5, 8, dtype=torch.int8, device=DEV), torch.ones(5, device=DEV), torch.ones(8, device=DEV)
+    s = torch.zeros(2, 2, 8, 8, device=DEV)
+    for call, t in ((lambda t: sequence.leaky_attention(q, t, q, g), q), (lambda t: sequence.leaky_attention(q, q, q, t), g), (lambda t: sequence.leaky_attention(q, q, q, g, state=t), s),
+                    (lambda t: sequence.leaky_attention_step(t, q[0], q[0], g, s.clone()), q[0]), (lambda t: sequence.add_rms_norm(t, ones)[0], x),
+                    (lambda t: sequence.add_rms_norm(x, ones, t)[1], x), (lambda t: sequence.add_rms_norm_int8(x, ones, t)[2], x),
+                    (lambda t: sequence.dequantize_int8(c, t), one), (lambda t: sequence.int8_linear(c, one, w, sw, t), sw)):
+        with torch.autograd.forward_ad.dual_level():
+            with pytest.raises(sequence.SSNeuronError, match='no forward-mode'):
+                call(torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)))
+        with pytest.raises(sequence.SSNeuronError, match='cannot be traced'):
+            torch.jit.trace(call, (t,))
+        with pytest.raises(sequence.SSNeuronError, match='cannot be traced'):
+            torch.fx.experimental.proxy_tensor.make_fx(call)(t)
+        call(t)                                            # and nothing of it stays behind
+
+
 def test_gradients_are_not_differentiated_again():
     q = torch.randn(4, 1, 1, 8, device=DEV, requires_grad=True)
     o = sequence.leaky_attention(q, q, q, torch.zeros(1, device=DEV))

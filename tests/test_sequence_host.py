@@ -217,3 +217,31 @@ def test_layers_keep_the_state_protocol():
     assert set(q.state_dict()) == {'weight', 'weight_scale', 'bias'} and q.weight.dtype == torch.int8
     assert layer.Int8Linear(torch.nn.Linear(6, 3, bias=False)).bias is None
     assert list(layer.AddRMSNorm(7).state_dict()) == ['weight']
+
+
+def _every_call():
+    """(name, call of one floating operand, that operand) for each entry point."""
+    q, g, s = torch.randn(3, 2, 2, 8), torch.zeros(2), torch.zeros(2, 2, 8, 8)
+    x, c, one = torch.randn(3, 8), torch.zeros(3, 8, dtype=torch.int8), torch.ones(3)
+    w, sw = torch.zeros(5, 8, dtype=torch.int8), torch.ones(5)
+    return [('leaky_attention', lambda t: sequence.leaky_attention(t, q, q, g), q), ('leaky_attention', lambda t: sequence.leaky_attention(q, q, t, g), q),
+            ('leaky_attention', lambda t: sequence.leaky_attention(q, q, q, t), g), ('leaky_attention', lambda t: sequence.leaky_attention(q, q, q, g, state=t), s),
+            ('leaky_attention_step', lambda t: sequence.leaky_attention_step(q[0], t, q[0], g, s), q[0]),
+            ('leaky_attention_step', lambda t: sequence.leaky_attention_step(q[0], q[0], q[0], g, t), s),
+            ('add_rms_norm', lambda t: sequence.add_rms_norm(t, torch.ones(8))[0], x), ('add_rms_norm', lambda t: sequence.add_rms_norm(x, t, x)[0], torch.ones(8)),
+            ('add_rms_norm', lambda t: sequence.add_rms_norm(x, torch.ones(8), t)[0], x), ('add_rms_norm_int8', lambda t: sequence.add_rms_norm_int8(x, torch.ones(8), t), x),
+            ('dequantize_int8', lambda t: sequence.dequantize_int8(c, t), one), ('int8_linear', lambda t: sequence.int8_linear(c, t, w, sw), one),
+            ('int8_linear', lambda t: sequence.int8_linear(c, one, w, sw, t), sw)]
+
+
+@pytest.mark.parametrize('i', range(len(_every_call())))
+def test_tracers_and_forward_mode_are_refused(anywhere, i):
+    """A trace would hold the outputs' allocation without the launch, and an output would have no tangent."""
+    name, call, t = _every_call()[i]
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(SSNeuronError, match=f'{name} has no forward-mode'):
+            call(torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)))
+    with pytest.raises(SSNeuronError, match=f'{name} cannot be traced'):
+        torch.jit.trace(call, (t,))
+    with pytest.raises(SSNeuronError, match=f'{name} cannot be traced'):
+        torch.fx.experimental.proxy_tensor.make_fx(call)(t)
