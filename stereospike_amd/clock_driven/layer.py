@@ -72,6 +72,8 @@ class LeakyAttention(nn.Module):
             return self.forward_sequence(q[None], k[None], v[None])[0]
         if self._state(q, v) is None:
             self.s = torch.zeros((*q.shape, v.shape[-1]), dtype=torch.float32, device=q.device)
+        elif self.s.requires_grad:                         # a training pass left it: its graph keeps its own tensor, the steps from here on are no part of it
+            self.s = self.s.detach().clone()
         return sequence.leaky_attention_step(q, k, v, self.log_decay, self.s, self.scale)
 
     def extra_repr(self):

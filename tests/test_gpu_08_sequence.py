@@ -944,3 +944,27 @@ def test_layer_protocol_on_the_device():
     functional.detach_net(att)
     with pytest.raises(sequence.SSNeuronError, match='reset_net'):
         att(q[0, :1], k[0, :1], v[0, :1])
+
+
+def test_steps_without_gradients_after_a_training_pass():
+    """Steps under no_grad leave the training graph's own state alone, and what is trained after them does not reach behind them."""
+    att = layer.LeakyAttention(2, tau=[2., 50.]).to(DEV)
+    q, k, v, _, _, _ = (t.to(DEV) if t is not None else None for t in leaky_case(6, 2, 2, 2, 16, 16, torch.float32, False, False))
+    first = [t[:3].clone().requires_grad_() for t in (q, k, v)]
+    o = att.forward_sequence(*first)
+    trained = att.s
+    before = trained.detach().clone()
+    with torch.no_grad():
+        att(q[3], k[3], v[3])
+        att(q[4], k[4], v[4])
+    assert not att.s.requires_grad and torch.equal(trained, before)
+    start = att.s.clone()
+    last = [t[5:].clone().requires_grad_() for t in (q, k, v)]
+    o2 = att.forward_sequence(*last)
+    assert torch.equal(o2, sequence.leaky_attention(*(t.detach() for t in last), att.log_decay, state=start))
+    assert all(g is None for g in torch.autograd.grad(o2.sum(), first, retain_graph=True, allow_unused=True))
+    got = torch.autograd.grad((o.sum(), trained.sum()), first)                   # the pass before is differentiated as if nothing had come after it
+    use = [t.detach().requires_grad_() for t in first]
+    want = torch.autograd.grad([t.sum() for t in sequence.leaky_attention(*use, att.log_decay, return_state=True)], use)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
