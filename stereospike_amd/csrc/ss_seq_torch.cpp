@@ -184,7 +184,8 @@ std::optional<std::tuple<Tensor, Tensor>> leaky_attention(const Tensor& q0, cons
 
 std::optional<Tensor> leaky_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& state, std::optional<double> scale)
 {
-    if (!attention_ok(q, k, v, log_decay, state, Tensor(), 3) || !state.is_contiguous() || recorded({q, k, v, log_decay, state})) return std::nullopt;
+    if (!state.defined() || !attention_ok(q, k, v, log_decay, state, Tensor(), 3) || !state.is_contiguous() || recorded({q, k, v, log_decay, state})) return std::nullopt;
+    if (state.requires_grad() || records({q, k, v, log_decay})) return std::nullopt;
     const c10::DeviceGuard guard(q.device());
     const at::NoGradGuard plain;
     const Tensor out = at::empty({q.size(0), q.size(1), v.size(2)}, q.options());

@@ -92,8 +92,14 @@ def _refuse_attention(q, k, v, log_decay, state, lengths, lead):
         _operand(state, 'state', dev, torch.float32, (B, H, Dk, Dv))
     if lengths is not None:
         _operand(lengths, 'lengths', dev, torch.int32, (B,))
-    if lead == 1 and not state.is_contiguous():
-        raise SSNeuronError('state: tensor must be contiguous (it is updated in place)')
+    if lead == 1:
+        _operand(state, 'state', dev, torch.float32, (B, H, Dk, Dv))
+        if not state.is_contiguous():
+            raise SSNeuronError('state: tensor must be contiguous (it is updated in place)')
+        if state.requires_grad:
+            raise SSNeuronError('state: it is updated in place, outside of any graph, and requires a gradient — pass state.detach().clone()')
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay)):
+            raise SSNeuronError('leaky_attention_step has no gradient: call it under torch.no_grad(), or leaky_attention with T = 1')
 
 
 def leaky_attention(q_seq: torch.Tensor, k_seq: torch.Tensor, v_seq: torch.Tensor, log_decay: torch.Tensor, scale: Optional[float] = None,
@@ -118,7 +124,7 @@ def leaky_attention(q_seq: torch.Tensor, k_seq: torch.Tensor, v_seq: torch.Tenso
 def leaky_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor,
                          scale: Optional[float] = None) -> torch.Tensor:
     """One time step of `leaky_attention`: q [B, H, Dk], k [B, Hk, Dk], v [B, Hk, Dv]; `state` (fp32 [B, H, Dk, Dv], contiguous) is updated IN PLACE.
-    Returns o [B, H, Dv].  No gradients (use leaky_attention with T = 1)."""
+    Returns o [B, H, Dv].  No gradients: a state that requires one, or q, k, v that do while gradients are enabled, are refused (use leaky_attention with T = 1)."""
     return _call('leaky_attention_step', lambda: _refuse_attention(q, k, v, log_decay, state, None, 1), q, k, v, log_decay, state, scale)
 
 

@@ -968,3 +968,18 @@ def test_steps_without_gradients_after_a_training_pass():
     want = torch.autograd.grad([t.sum() for t in sequence.leaky_attention(*use, att.log_decay, return_state=True)], use)
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_a_step_under_autograd_is_refused_on_the_device():
+    q, k, v, decay, s, _ = (t.to(DEV) if t is not None else None for t in leaky_case(1, 2, 2, 2, 16, 16, torch.float32, True, False))
+    before = s.clone()
+    with pytest.raises(sequence.SSNeuronError, match='step has no gradient'):
+        sequence.leaky_attention_step(q[0], k[0].clone().requires_grad_(), v[0], decay, s)
+    with torch.no_grad(), pytest.raises(sequence.SSNeuronError, match='state: it is updated in place'):
+        sequence.leaky_attention_step(q[0], k[0], v[0], decay, s.clone().requires_grad_())
+    with pytest.raises(sequence.SSNeuronError, match='state is on'):
+        sequence.leaky_attention_step(q[0], k[0], v[0], decay, None)
+    assert torch.equal(s, before)
+    with torch.no_grad():                                  # without gradients enabled the operands may require one
+        o = sequence.leaky_attention_step(q[0].clone().requires_grad_(), k[0], v[0], decay, s)
+    assert not o.requires_grad and torch.equal(o, sequence.leaky_attention_step(q[0], k[0], v[0], decay, before))

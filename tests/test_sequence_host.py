@@ -166,6 +166,24 @@ def test_attention_refusals(anywhere):
         sequence.leaky_attention_step(q, k, v, g, s)
 
 
+def test_a_step_under_autograd_is_refused(anywhere):
+    """It has no gradient: operands that require one while gradients are enabled, or a state (updated in place) that does, would lose it without a word."""
+    q, k, v = (t[0] for t in _qkv())
+    g, s = torch.zeros(4), torch.zeros(2, 4, 8, 6)
+    for i in range(3):
+        use = [q, k, v]
+        use[i] = use[i].clone().requires_grad_()
+        with pytest.raises(SSNeuronError, match='step has no gradient'):
+            sequence.leaky_attention_step(*use, g, s)
+    with pytest.raises(SSNeuronError, match='step has no gradient'):
+        sequence.leaky_attention_step(q, k, v, g.clone().requires_grad_(), s)
+    for state in (s.clone().requires_grad_(), s.clone().requires_grad_() * 2):
+        with pytest.raises(SSNeuronError, match='state: it is updated in place'):
+            sequence.leaky_attention_step(q, k, v, g, state)
+        with torch.no_grad(), pytest.raises(SSNeuronError, match='state: it is updated in place'):
+            sequence.leaky_attention_step(q, k, v, g, state)
+
+
 def test_norm_and_product_refusals(anywhere):
     x, w = torch.zeros(3, 8), torch.ones(8)
     for args, kw, what in (((x.double(), w), {}, 'x: expected'), ((x, w[:4]), {}, 'weight'), ((x, w.half()), {}, 'weight'), ((x, w), dict(residual=x.half()), 'residual'),
