@@ -274,11 +274,9 @@ std::optional<std::tuple<Tensor, Tensor>> add_rms_norm(const Tensor& x, const Te
     return std::make_tuple(y, residual.defined() ? sum : x);
 }
 
-std::optional<std::tuple<Tensor, Tensor, Tensor>> add_rms_norm_int8(const Tensor& x, const Tensor& weight, const Maybe& residual0, double eps)
+// codes, scales and, with a residual, the sum
+variable_list norm_int8_run(const Tensor& x, const Tensor& weight, const Tensor& residual, double eps)
 {
-    const Tensor& residual = given(residual0);
-    if (!norm_ok(x, weight, residual, eps) || recorded({x, weight, residual})) return std::nullopt;
-    const c10::DeviceGuard guard(x.device());
     const at::NoGradGuard plain;
     const Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kChar)), scales = at::empty(x.sizes().slice(0, x.dim() - 1), weight.options()),
                  sum = residual.defined() ? at::empty(x.sizes(), x.options()) : Tensor();
@@ -287,7 +285,31 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> add_rms_norm_int8(const Tensor
         check(ss_seq_rms_norm_int8(xr.data_ptr(), xr.stride(0), ptr<void>(rr), rr.defined() ? rr.stride(0) : 0, ptr<float>(weight.contiguous()),
                                    static_cast<signed char*>(codes.data_ptr()), ptr<float>(scales), ptr<void>(sum), xr.size(0), (int)xr.size(1), (float)eps,
                                    code_of(x.scalar_type()), stream_of(x)), "ss_seq_rms_norm_int8");
-    return std::make_tuple(codes, scales, residual.defined() ? sum : x);
+    return {codes, scales, sum};
+}
+
+// codes and scales have no gradient; the sum has an addition's
+struct AddRmsNormInt8 : torch::autograd::Function<AddRmsNormInt8> {
+    static variable_list forward(AutogradContext* ctx, Tensor x, Tensor residual, Tensor weight, double eps)
+    {
+        ctx->set_materialize_grads(false);
+        const variable_list r = norm_int8_run(x, weight, residual, eps);
+        ctx->mark_non_differentiable({r[0], r[1]});
+        return r;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        return {ctx->needs_input_grad(0) ? grads[2] : Tensor(), ctx->needs_input_grad(1) ? grads[2] : Tensor(), Tensor(), Tensor()};
+    }
+};
+
+std::optional<std::tuple<Tensor, Tensor, Tensor>> add_rms_norm_int8(const Tensor& x, const Tensor& weight, const Maybe& residual0, double eps)
+{
+    const Tensor& residual = given(residual0);
+    if (!norm_ok(x, weight, residual, eps) || recorded({x, weight, residual})) return std::nullopt;
+    const c10::DeviceGuard guard(x.device());
+    const variable_list r = residual.defined() && records({x, residual}) ? AddRmsNormInt8::apply(x, residual, weight.detach(), eps) : norm_int8_run(x, weight, residual, eps);
+    return std::make_tuple(r[0], r[1], residual.defined() ? r[2] : x);
 }
 
 std::optional<Tensor> dequantize_int8(const Tensor& codes, const Tensor& scales, at::ScalarType dtype)

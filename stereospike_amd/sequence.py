@@ -154,7 +154,7 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
 def add_rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
     """`add_rms_norm` handed on in 8 bits: returns (codes int8 [..., C], scales fp32 [...], h) with codes * scales the norm; the largest value of a row has the
     code +-127, ties go to the even code.  A row of zeros has scale 0; a row with a NaN or an infinity, its own or
-    the weight's, has codes 0 and scale NaN.  No gradients."""
+    the weight's, has codes 0 and scale NaN.  Codes and scales have no gradient (nor has the weight); h has that of the addition."""
     return _call('add_rms_norm_int8', lambda: _refuse_norm(x, weight, residual, eps), x, weight, residual, eps)
 
 

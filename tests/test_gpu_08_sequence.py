@@ -469,6 +469,28 @@ def test_norm_int8(C, dtype, residual):
         within(back, values, values.abs() * (HALF[dtype] + U) * 1.01 + TINY[dtype], 'values')
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_norm_int8_keeps_the_sum_in_the_graph(dtype):
+    """h is handed on to the next layer's residual: its gradient reaches x and residual as an addition's does, with a residual as without."""
+    x, w, r = (t.to(DEV) for t in norm_case(5, 72, dtype, True, seed=2))
+    g = normal(gen(3), 5, 72, dtype=dtype).to(DEV)
+    plain = sequence.add_rms_norm_int8(x, w, r)
+    for need in ((True, True), (True, False), (False, True)):
+        a, b, wl = x.clone().requires_grad_(need[0]), r.clone().requires_grad_(need[1]), w.clone().requires_grad_()
+        codes, scales, h = sequence.add_rms_norm_int8(a, wl, b)
+        for got, want in zip((codes, scales, h), plain):
+            assert torch.equal(got, want)
+        assert h.requires_grad and not scales.requires_grad
+        for got in torch.autograd.grad(h, [t for t in (a, b) if t.requires_grad], g, retain_graph=True):
+            assert torch.equal(got, g)
+        h.sum().backward()
+        assert wl.grad is None
+    a = x.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(sequence.add_rms_norm_int8(a, w)[2], a, g)[0], g)
+    assert torch.equal(torch.autograd.grad(sequence.add_rms_norm_int8(a, w, a)[2], a, g)[0], g + g)
+    assert not sequence.add_rms_norm_int8(x, w.clone().requires_grad_(), r)[2].requires_grad
+
+
 def test_norm_int8_ties_zeros_and_what_is_not_finite():
     x = torch.zeros(6, 64)
     x[0, 0], x[0, 1:8] = 127., torch.tensor([0.5, 1.5, 2.5, -0.5, -1.5, -2.5, 126.5])         # a code's step is 1: ties, to even
