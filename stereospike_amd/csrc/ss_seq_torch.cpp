@@ -315,7 +315,7 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> add_rms_norm_int8(const Tensor
 std::optional<Tensor> dequantize_int8(const Tensor& codes, const Tensor& scales, at::ScalarType dtype)
 {
     if (!codes.is_cuda() || codes.scalar_type() != at::kChar || codes.dim() < 1 || codes.size(-1) < 1 || code_of(dtype) < 0) return std::nullopt;
-    if (!is(scales, codes, at::kFloat, codes.sizes().slice(0, codes.dim() - 1)) || recorded({scales})) return std::nullopt;
+    if (!is(scales, codes, at::kFloat, codes.sizes().slice(0, codes.dim() - 1)) || records({scales}) || recorded({scales})) return std::nullopt;
     const c10::DeviceGuard guard(codes.device());
     const at::NoGradGuard plain;
     const Tensor out = at::empty(codes.sizes(), codes.options().dtype(dtype)), c = codes.contiguous(), s = scales.contiguous();

@@ -159,7 +159,7 @@ def add_rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[
 
 
 def dequantize_int8(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
-    """The values that 8-bit codes [..., C] with a scale per row [...] stand for."""
+    """The values that 8-bit codes [..., C] with a scale per row [...] stand for, codes * scales rounded once to dtype.  No gradients."""
     def refuse():
         _require_hip(codes, 'codes')
         if codes.dim() < 1 or codes.shape[-1] < 1:
@@ -168,6 +168,8 @@ def dequantize_int8(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtyp
         _operand(scales, 'scales', codes.device, torch.float32, codes.shape[:-1])
         if dtype not in _FLOATS:
             raise SSNeuronError(f'dtype: expected float32, float16 or bfloat16, got {dtype}')
+        if torch.is_grad_enabled() and scales.requires_grad:
+            raise SSNeuronError('dequantize_int8 has no gradient: call it under torch.no_grad() or detach scales')
     return _call('dequantize_int8', refuse, codes, scales, dtype)
 
 

@@ -727,6 +727,14 @@ def test_tracers_and_forward_mode_are_refused_on_the_device():
         call(t)                                            # and nothing of it stays behind
 
 
+def test_values_of_codes_under_autograd_are_refused_on_the_device():
+    c, s = torch.ones(3, 8, dtype=torch.int8, device=DEV), torch.ones(3, device=DEV, requires_grad=True)
+    with pytest.raises(sequence.SSNeuronError, match='dequantize_int8 has no gradient'):
+        sequence.dequantize_int8(c, s)
+    with torch.no_grad():
+        assert torch.equal(sequence.dequantize_int8(c, s), c.float())
+
+
 def test_gradients_are_not_differentiated_again():
     q = torch.randn(4, 1, 1, 8, device=DEV, requires_grad=True)
     o = sequence.leaky_attention(q, q, q, torch.zeros(1, device=DEV))

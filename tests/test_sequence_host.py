@@ -206,6 +206,11 @@ def test_norm_and_product_refusals(anywhere):
         sequence.dequantize_int8(a, torch.ones(3), torch.float64)
 
 
+def test_values_of_codes_under_autograd_are_refused(anywhere):
+    with pytest.raises(SSNeuronError, match='dequantize_int8 has no gradient'):
+        sequence.dequantize_int8(torch.zeros(3, 8, dtype=torch.int8), torch.ones(3, requires_grad=True))
+
+
 def test_quantize_channels():
     torch.manual_seed(0)
     w = torch.randn(5, 40)
