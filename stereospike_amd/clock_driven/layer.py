@@ -58,19 +58,20 @@ class LeakyAttention(nn.Module):
 
     def forward_sequence(self, q_seq, k_seq, v_seq, lengths: Optional[torch.Tensor] = None):
         """lengths: int32 [B], the valid steps of each stream; the state of a stream stops at its last valid step."""
-        out, self.s = sequence.leaky_attention(q_seq, k_seq, v_seq, self.log_decay, self.scale, self._state(q_seq[0] if q_seq.dim() == 4 else q_seq, v_seq), lengths, True)
+        out, self.s = sequence.leaky_attention(q_seq, k_seq, v_seq, self.log_decay, self.scale, self._state(q_seq.shape[-3:], v_seq), lengths, True)
         return out
 
-    def _state(self, q, v):
-        if self.s is not None and tuple(self.s.shape) != (*q.shape, v.shape[-1]):
-            raise SSNeuronError(f'state shape {tuple(self.s.shape)} does not fit queries {tuple(q.shape)} and values of {v.shape[-1]}; '
+    def _state(self, shape, v):
+        """The state, if it fits queries of this shape [B, heads, Dk]."""
+        if self.s is not None and tuple(self.s.shape) != (*shape, v.shape[-1]):
+            raise SSNeuronError(f'state shape {tuple(self.s.shape)} does not fit queries {tuple(shape)} and values of {v.shape[-1]}; '
                                 f'call functional.reset_net(net) when the batch shape changes')
         return self.s
 
     def forward(self, q, k, v):
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, self.s)):
             return self.forward_sequence(q[None], k[None], v[None])[0]
-        if self._state(q, v) is None:
+        if self._state(q.shape, v) is None:
             self.s = torch.zeros((*q.shape, v.shape[-1]), dtype=torch.float32, device=q.device)
         elif self.s.requires_grad:                         # a training pass left it: its graph keeps its own tensor, the steps from here on are no part of it
             self.s = self.s.detach().clone()

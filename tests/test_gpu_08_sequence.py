@@ -1013,3 +1013,18 @@ def test_a_step_under_autograd_is_refused_on_the_device():
     with torch.no_grad():                                  # without gradients enabled the operands may require one
         o = sequence.leaky_attention_step(q[0].clone().requires_grad_(), k[0], v[0], decay, s)
     assert not o.requires_grad and torch.equal(o, sequence.leaky_attention_step(q[0], k[0], v[0], decay, before))
+
+
+def test_layer_of_no_steps():
+    """A sequence of no steps leaves the state as it is and gives no outputs, as the function does."""
+    att = layer.LeakyAttention(2).to(DEV)
+    q, k, v, _, _, _ = (t.to(DEV) if t is not None else None for t in leaky_case(3, 2, 2, 1, 16, 24, torch.bfloat16, False, False))
+    assert att.forward_sequence(q[:0], k[:0], v[:0]).shape == (0, 2, 2, 24) and not att.s.any() and att.s.shape == (2, 2, 16, 24)
+    att.forward_sequence(q, k, v)
+    s = att.s.clone()
+    assert att.forward_sequence(q[:0], k[:0], v[:0]).shape == (0, 2, 2, 24) and torch.equal(att.s, s)
+    with pytest.raises(sequence.SSNeuronError, match='reset_net'):
+        att.forward_sequence(q[:0, :1], k[:0, :1], v[:0, :1])
+    for bad in (q[0], q[None]):
+        with pytest.raises(sequence.SSNeuronError):
+            att.forward_sequence(bad, k, v)
