@@ -110,12 +110,23 @@ Tensor attention_run(const Tensor& q, const Tensor& k, const Tensor& v, const Te
     return ws;
 }
 
+// no step, or no stream: outputs that are empty or zeros, the state as it is, and nothing to launch
+variable_list attention_none(const Tensor& q, const Tensor& v, const Tensor& log_decay, const Tensor& state)
+{
+    return {at::zeros({q.size(0), q.size(1), q.size(2), v.size(3)}, q.options()),
+            state.defined() ? state.clone() : at::zeros({q.size(1), q.size(2), q.size(3), v.size(3)}, log_decay.options())};
+}
+
 struct LeakyAttention : torch::autograd::Function<LeakyAttention> {
     // (an operand that is not there has no edge: the state's, if it is there, is the fifth)
     static variable_list forward(AutogradContext* ctx, Tensor q, Tensor k, Tensor v, Tensor log_decay, Maybe state0, Maybe lengths0, double scale)
     {
         const Tensor &state = given(state0), &lengths = given(lengths0);
         ctx->set_materialize_grads(false);
+        if (q.numel() == 0) {
+            ctx->save_for_backward({q, k, v, state});
+            return attention_none(q, v, log_decay, state);
+        }
         const Tensor out = at::empty({q.size(0), q.size(1), q.size(2), v.size(3)}, q.options()),
                      last = at::empty({q.size(1), q.size(2), q.size(3), v.size(3)}, log_decay.options());
         const Tensor states = attention_run(q, k, v, out, log_decay, scale, lengths, state, last);
@@ -126,6 +137,10 @@ struct LeakyAttention : torch::autograd::Function<LeakyAttention> {
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
         const variable_list s = ctx->get_saved_variables();
+        if (s[0].numel() == 0) {
+            const Tensor g_s = !s[3].defined() || !ctx->needs_input_grad(4) ? Tensor() : grads[1].defined() ? grads[1] : at::zeros_like(s[3]);
+            return {at::zeros_like(s[0]), at::zeros_like(s[1]), at::zeros_like(s[2]), Tensor(), g_s, Tensor(), Tensor()};
+        }
         const Tensor &q = s[0], &k = s[1], &v = s[2], &state = s[3], &log_decay = s[4], &lengths = s[5], &states = s[6];
         const c10::DeviceGuard guard(q.device());
         const bool need_q = ctx->needs_input_grad(0), need_k = ctx->needs_input_grad(1), need_v = ctx->needs_input_grad(2), need_s = state.defined() && ctx->needs_input_grad(4);
@@ -169,12 +184,14 @@ std::optional<std::tuple<Tensor, Tensor>> leaky_attention(const Tensor& q0, cons
     const c10::DeviceGuard guard(q0.device());
     const double scale = scale0.has_value() ? *scale0 : 1. / std::sqrt((double)q0.size(3));
     const int64_t T = q0.size(0), B = q0.size(1), H = q0.size(2), Dk = q0.size(3), Dv = v0.size(3);
-    if (T == 0 || B == 0)                                  // no step: nothing to launch
-        return std::make_tuple(at::zeros({T, B, H, Dv}, q0.options()), st.defined() ? st.clone() : at::zeros({B, H, Dk, Dv}, log_decay0.options()));
     const Tensor q = last_contiguous(q0), k = last_contiguous(k0), v = last_contiguous(v0), log_decay = log_decay0.contiguous(),
                  state = st.defined() ? st.contiguous() : Tensor(), lengths = lengths0.has_value() ? lengths0->contiguous() : Tensor();
     if (records({q, k, v, state})) {
         const variable_list r = LeakyAttention::apply(q, k, v, log_decay, st.defined() ? Maybe(state) : Maybe(), lengths.defined() ? Maybe(lengths) : Maybe(), scale);
+        return std::make_tuple(r[0], r[1]);
+    }
+    if (T == 0 || B == 0) {
+        const variable_list r = attention_none(q, v, log_decay, state);
         return std::make_tuple(r[0], r[1]);
     }
     const Tensor out = at::empty({T, B, H, Dv}, q.options()), last = at::empty({B, H, Dk, Dv}, log_decay.options());

@@ -693,6 +693,22 @@ def test_nothing_to_do():
     assert sequence.dequantize_int8(c, torch.ones(0, device=DEV)).shape == (0, 8)
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_gradients_of_nothing_to_do(dtype):
+    """No step or no stream under autograd: gradients of the operands' shapes, the state's is the last state's."""
+    q, k, v, decay, s, _ = (t.to(DEV) if t is not None else None for t in leaky_case(3, 2, 4, 2, 8, 6, dtype, True, False))
+    for cut in ((slice(0, 0), slice(None)), (slice(None), slice(0, 0)), (slice(0, 0), slice(0, 0))):
+        use = [t[cut].clone().requires_grad_() for t in (q, k, v)]
+        state = s[cut[1]].clone().requires_grad_()
+        o, last = sequence.leaky_attention(*use, decay, state=state, return_state=True)
+        assert torch.equal(last, state) and o.shape == (*use[0].shape[:3], 6) and o.dtype == dtype
+        g = torch.randn_like(last)
+        got = torch.autograd.grad([o, last], [*use, state], [torch.ones_like(o), g], retain_graph=True)
+        assert [t.shape for t in got[:3]] == [t.shape for t in use] and torch.equal(got[3], g)
+        assert not torch.autograd.grad(o.sum(), state, retain_graph=True)[0].any()
+        assert torch.autograd.grad(sequence.leaky_attention(*use, decay).sum(), use[1])[0].shape == use[1].shape
+
+
 def test_refusals_on_the_device():
     """The library hands unfit operands back before it launches; the error names the operand."""
     q, g = torch.zeros(3, 2, 4, 8, device=DEV), torch.zeros(4, device=DEV)
