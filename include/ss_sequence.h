@@ -121,7 +121,7 @@ int ss_seq_dequant_int8(const signed char* codes, const float* scales, void* out
 /*
  * 8-bit integer product:  out[m][n] = (sum_k a[m][k] * w[n][k]) * a_scale[m] * w_scale[n] + bias[n]
  * a [M][K] (row stride lda), w [N][K] (row stride ldw), sums exact in 32-bit integers (K < 131072), out [M][N] contiguous in out_dtype; bias may be NULL.
- * Any row strides and alignment; rows that are not aligned to 16 bytes are copied into the workspace first.  M, N <= 2^27.
+ * Any row strides and alignment; rows that are not aligned to 16 bytes are copied into the workspace first.  M, N <= 2^27, less than 2^24 tiles of 128 x 128 outputs.
  */
 long long ss_seq_int8_linear_ws_ints(const signed char* a, long long lda, const signed char* w, long long ldw, long long M, int N, int K);      /* of ws */
 int ss_seq_int8_linear(const signed char* a, long long lda, const float* a_scale, const signed char* w, long long ldw, const float* w_scale,

@@ -18,7 +18,7 @@ MAX_HEAD_DIM = 256
 MAX_NORM_WIDTH = 16384
 MAX_INT8_K = 131071
 MAX_STATES = 65535
-MAX_STEPS, MAX_SIDE = 1 << 30, 1 << 27
+MAX_STEPS, MAX_SIDE, MAX_TILES = 1 << 30, 1 << 27, 1 << 24
 
 _ops = None
 

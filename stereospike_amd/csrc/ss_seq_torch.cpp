@@ -23,7 +23,7 @@ typedef std::optional<Tensor> Maybe;
 
 namespace {
 
-constexpr int64_t kMaxHead = 256, kMaxWidth = 16384, kMaxK = 131071, kMaxStates = 65535, kMaxSteps = 1 << 30, kMaxSide = 1 << 27;
+constexpr int64_t kMaxHead = 256, kMaxWidth = 16384, kMaxK = 131071, kMaxStates = 65535, kMaxSteps = 1 << 30, kMaxSide = 1 << 27, kMaxTiles = 1 << 24;
 
 struct SeqError : std::runtime_error { using std::runtime_error::runtime_error; };
 
@@ -351,6 +351,7 @@ std::optional<Tensor> int8_linear(const Tensor& codes, const Tensor& scales, con
     if (!codes.is_cuda() || codes.scalar_type() != at::kChar || codes.dim() < 1 || weight.dim() != 2 || code_of(out_dtype) < 0) return std::nullopt;
     const int64_t N = weight.size(0), K = weight.size(1);
     if (!is(weight, codes, at::kChar, {N, K}) || codes.size(-1) != K || N < 1 || N > kMaxSide || K < 1 || K > kMaxK || codes.numel() / K > kMaxSide) return std::nullopt;
+    if ((codes.numel() / K + 127) / 128 * ((N + 127) / 128) >= kMaxTiles) return std::nullopt;
     if (!is(scales, codes, at::kFloat, codes.sizes().slice(0, codes.dim() - 1)) || !is(weight_scale, codes, at::kFloat, {N})) return std::nullopt;
     if (bias.defined() && !is(bias, codes, at::kFloat, {N})) return std::nullopt;
     if (records({scales, weight_scale, bias}) || recorded({scales, weight_scale, bias})) return std::nullopt;

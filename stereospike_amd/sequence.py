@@ -192,7 +192,8 @@ def int8_linear(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor,
                 out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """out[..., n] = (sum_k codes[..., k] * weight[n, k]) * scales[...] * weight_scale[n] + bias[n], the sum exact in 32-bit integers.
 
-    codes int8 [..., K] (spike counts are codes of scale 1), scales fp32 [...], weight int8 [N, K], weight_scale fp32 [N], bias fp32 [N]; K < 131072, at most 2^27 rows and channels.  Scaled in
+    codes int8 [..., K] (spike counts are codes of scale 1), scales fp32 [...], weight int8 [N, K], weight_scale fp32 [N], bias fp32 [N]; K < 131072, at most 2^27 rows and channels, less than 2^24
+    tiles of 128 x 128 outputs.  Scaled in
     fp32, rounded once to out_dtype (float32 / float16 / bfloat16).  No gradients."""
     def refuse():
         _require_hip(codes, 'codes')
@@ -210,6 +211,8 @@ def int8_linear(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor,
             raise SSNeuronError(f'weight: [N, K] = [{N}, {K}]; N >= 1 and 1 <= K <= {_seqlib.MAX_INT8_K} (sums stay within 32 bits) are implemented')
         if max(N, codes.numel() // K) > _seqlib.MAX_SIDE:
             raise SSNeuronError(f'{codes.numel() // K} rows, {N} channels: at most {_seqlib.MAX_SIDE} of each')
+        if -(-(codes.numel() // K) // 128) * -(-N // 128) >= _seqlib.MAX_TILES:
+            raise SSNeuronError(f'{codes.numel() // K} rows by {N} channels: less than {_seqlib.MAX_TILES} tiles of 128 x 128 outputs in one call')
         if out_dtype not in _FLOATS:
             raise SSNeuronError(f'out_dtype: expected float32, float16 or bfloat16, got {out_dtype}')
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (scales, weight_scale, bias)):

@@ -724,6 +724,12 @@ def test_refusals_on_the_device():
         sequence.int8_linear(q.to(torch.int8), torch.ones(3, device=DEV), torch.zeros(5, 8, dtype=torch.int8, device=DEV), torch.ones(5, device=DEV))
 
 
+def test_a_product_of_too_many_outputs_is_refused_by_name_on_the_device():
+    a, s = torch.zeros(1, 16, dtype=torch.int8, device=DEV).expand(2 ** 19, 16), torch.ones(1, device=DEV).expand(2 ** 19)
+    with pytest.raises(sequence.SSNeuronError, match='524288 rows by 524288 channels'):
+        sequence.int8_linear(a, s, a, s)
+
+
 def test_tracers_and_forward_mode_are_refused_on_the_device():
     q, g = torch.randn(3, 2, 2, 8, device=DEV), torch.zeros(2, device=DEV)
     x, c, one = torch.randn(3, 8, device=DEV), torch.zeros(3, 8, dtype=torch.int8, device=DEV), torch.ones(3, device=DEV)

@@ -133,6 +133,27 @@ def test_product_entry_refuses_more_than_a_grid_holds():
         assert L.ss_seq_int8_linear(256, 16, 256, 256, 16, 256, None, 256, M, N, 16, 0, 256, None) == -22
 
 
+def test_limits_agree():
+    """The three places that know a limit: the Python checks, the library's, and the C entries' own."""
+    src = open(os.path.join(ROOT, 'stereospike_amd', 'csrc', 'ss_seq_torch.cpp')).read()
+    mine = {n: int(v) << int(by or 0) for n, v, by in re.findall(r'\b(kMax\w+) = (\d+)(?: << (\d+))?', src)}
+    assert mine == dict(kMaxHead=_seqlib.MAX_HEAD_DIM, kMaxWidth=_seqlib.MAX_NORM_WIDTH, kMaxK=_seqlib.MAX_INT8_K, kMaxStates=_seqlib.MAX_STATES,
+                        kMaxSteps=_seqlib.MAX_STEPS, kMaxSide=_seqlib.MAX_SIDE, kMaxTiles=_seqlib.MAX_TILES)
+    L, null = _lib(), None
+    L.ss_seq_leaky_ws_floats.argtypes, L.ss_seq_leaky_ws_floats.restype = [p], i64
+    # inside every limit a workspace is asked for, behind one nothing is (and the entry refuses)
+    inside = dict(T=65536, B=1, H=1, DA=_seqlib.MAX_HEAD_DIM, DC=_seqlib.MAX_HEAD_DIM)
+    assert L.ss_seq_leaky_ws_floats(ctypes.byref(_desc(**inside))) > 0
+    for behind in (dict(DA=_seqlib.MAX_HEAD_DIM + 1), dict(DC=_seqlib.MAX_HEAD_DIM + 1), dict(T=_seqlib.MAX_STEPS + 1), dict(B=_seqlib.MAX_STATES + 1)):
+        assert L.ss_seq_leaky_ws_floats(ctypes.byref(_desc(**{**inside, **behind}))) == 0
+        assert L.ss_seq_leaky(ctypes.byref(_desc(**{**inside, **behind})), null) == -22
+    L.ss_seq_rms_norm_ws_floats.argtypes, L.ss_seq_rms_norm_ws_floats.restype = [i64, i32, i32], i64
+    assert L.ss_seq_rms_norm_ws_floats(2, _seqlib.MAX_NORM_WIDTH, 0) > 0 and L.ss_seq_rms_norm_ws_floats(2, _seqlib.MAX_NORM_WIDTH + 1, 0) == 0
+    for M, N, K, rc in ((0, _seqlib.MAX_SIDE, 16, 0), (_seqlib.MAX_SIDE + 1, 1, 16, -22), (1, _seqlib.MAX_SIDE + 1, 16, -22), (0, 8, _seqlib.MAX_INT8_K, 0), (0, 8, _seqlib.MAX_INT8_K + 1, -22),
+                        (128 * 4096, 128 * (_seqlib.MAX_TILES // 4096), 16, -22)):
+        assert L.ss_seq_int8_linear(256, K, 256, 256, K, 256, null, 256, M, N, K, 0, null, null) == rc, (M, N, K)
+
+
 @pytest.fixture
 def anywhere(monkeypatch):
     """The reasons of a refusal behind the device check, on CPU tensors (which the library hands back before it launches anything)."""
@@ -164,6 +185,12 @@ def test_attention_refusals(anywhere):
         sequence.leaky_attention_step(q[0], k[0], v[0], g, torch.zeros(2, 4, 6, 8).transpose(2, 3))
     with pytest.raises(SSNeuronError, match='3 axes'):
         sequence.leaky_attention_step(q, k, v, g, s)
+
+
+def test_a_product_of_too_many_outputs_is_refused_by_name(anywhere):
+    a, s = torch.zeros(1, 16, dtype=torch.int8).expand(2 ** 19, 16), torch.ones(1).expand(2 ** 19)
+    with pytest.raises(SSNeuronError, match='524288 rows by 524288 channels'):
+        sequence.int8_linear(a, s, a, s)
 
 
 def test_a_step_under_autograd_is_refused(anywhere):
