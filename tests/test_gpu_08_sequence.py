@@ -122,6 +122,35 @@ def test_leaky_attention_state_and_lengths(shape, dtype):
     leaky_check(*shape, dtype, state=True, ragged=False, grads=True, seed=3)
 
 
+def segments_of(dtype, T, B, H, Dk, Dv):
+    """(segments, the lengths that they may have) of the forward pass, from the size of its workspace: a padded state for each but the last."""
+    import ctypes
+    from test_sequence_host import _desc, _lib
+    code, size = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype], _lib().ss_seq_leaky_ws_floats
+    size.argtypes, size.restype = [ctypes.c_void_p], ctypes.c_longlong
+    pad = 64 if Dk <= 64 else 128 if Dk <= 128 else 256
+    cols = 64 if Dv <= 64 or (code and Dk > 128) else 128
+    n, left = divmod(size(ctypes.byref(_desc(dtype=code, out_dtype=code, T=T, B=B, H=H, DA=Dk, DC=Dv))), B * H * -(-Dv // cols) * cols * pad)
+    chunks = -(-T // 32)
+    assert left == 0
+    return n + 1, [32 * c for c in range(1, chunks + 1) if -(-chunks // c) == n + 1]
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('shape,few', [((400, 42, 2, 1, 24, 40), True), ((1100, 12, 2, 1, 24, 40), False), ((700, 12, 1, 1, 72, 136), False), ((600, 12, 1, 1, 136, 72), False)])
+def test_leaky_attention_of_ragged_streams_in_segments(shape, few, dtype, monkeypatch):
+    """Streams that end on a segment's border, one step before and one behind it, and in no segment at all; few segments (joined by the output pass) and many (by a
+    scan), with a state, shared heads and all gradients."""
+    T, B, H, Hk, Dk, Dv = shape
+    n, seg = segments_of(dtype, T, B, H, Dk, Dv)
+    assert 2 <= n <= 5 if few else n > 5 and len(seg) == 1, (n, seg)
+    borders = [32 * c for c in range(1, -(-T // 32))] if few else [seg[0], n // 2 * seg[0], (n - 1) * seg[0]]
+    lengths = torch.tensor([T, 0, 1, *(b + d for b in borders for d in (-1, 0, 1)), *[T] * B][:B], dtype=torch.int32)
+    case = leaky_case
+    monkeypatch.setitem(globals(), 'leaky_case', lambda *args: (*case(*args)[:5], lengths))
+    leaky_check(*shape, dtype, state=True, ragged=True, grads=True)
+
+
 @pytest.mark.parametrize('dtype', DTYPES)
 def test_leaky_attention_long(dtype):
     leaky_check(5000, 1, 2, 2, 16, 24, dtype, state=True, ragged=False, grads=False)
@@ -576,6 +605,22 @@ def test_int8_linear_larger(shape):
     y = (a.to(DEV).double() @ w.to(DEV).double().t()) * sa.to(DEV).double()[:, None] * sw.to(DEV).double()
     want = y + b.to(DEV).double()
     within(got, want, y.abs() * 3.1 * U + want.abs() * 2 * U + 1e-30, str(shape))
+
+
+@pytest.mark.parametrize('shape', [(3500, 3333, 400), (3500, 3333, 387), (3400, 3584, 640), (3329, 3329, 128), (3400, 3590, 1000)])
+@pytest.mark.parametrize('out', DTYPES)
+def test_int8_linear_in_tiles_of_256(shape, out):
+    """At least 176 tiles of 256 x 256: several k steps and a partial one, rows copied to alignment, element stores, each type, with a bias and without."""
+    M, N, K = shape
+    assert -(-M // 256) * -(-N // 256) >= 176
+    a, sa, w, sw, b = (t.to(DEV) for t in product_case(M, N, K, True, seed=K))
+    y = (a.double() @ w.double().t()) * sa.double()[:, None] * (sw.double() / 512)
+    for bias in (None, b / 512):
+        got = sequence.int8_linear(a, sa, w, sw / 512, bias, out)
+        want = y if bias is None else y + bias.double()
+        if out == torch.float16:
+            assert want.abs().max() < 65504
+        within(got, want, y.abs() * 3.1 * U + want.abs() * (HALF[out] * 1.01 + U) + TINY[out], f'{shape}, bias {bias is not None}')
 
 
 def test_int8_linear_extreme_sums_and_strides():
