@@ -96,7 +96,7 @@ int ss_seq_group_sum(const float* x, void* out, long long rows, int group, int D
  * Add + root-mean-square norm:   h = round(x + residual)  (residual NULL: h = x, sum not written),
  *                                y = h * rstd * weight,   rstd = 1 / sqrt(mean(h^2) + eps)
  * x, residual: rows of C with their own row strides; y, sum: [rows][C] contiguous; weight fp32 [C]; rstd fp32 [rows] (NULL: not wanted).
- * Sums in fp32 (in fp64 where fp32 leaves its range).
+ * Sums in fp32 (in fp64 where fp32 leaves its range); rstd is fp32, so sqrt(mean(h^2) + eps) has to be at least 3e-39.
  */
 int ss_seq_rms_norm_fwd(const void* x, long long x_stride, const void* residual, long long r_stride, const float* weight, void* y, void* sum, float* rstd,
                         long long rows, int C, float eps, int dtype, void* stream);

@@ -59,7 +59,7 @@ namespace {
 
 // One step, S = lambda S + b c^T and out = a^T S (in reverse the leak comes after: s_out = lambda S).  HBM-bound: the state is read, updated and written once,
 // 8 bytes for each of its values.  A workgroup has 64 columns of one head's state, thread (g, x) rows g + 16 r of columns 4 x .. 4 x + 3, all R of them in
-// flight at once.  (512 streams of 16 heads of 128 x 128, bf16: 1.08 GB in 208 us, a large copy's rate; one stream of 8 heads of 64 x 64: 4.0 us,
+// flight at once.  (512 streams of 16 heads of 128 x 128, bf16: 1.08 GB in 213 us, a large copy's rate; one stream of 8 heads of 64 x 64: 4.2 us,
 // little over an empty launch.)  V4: the state's rows take 16-byte accesses.
 template <int DT, int ODT, int R, bool V4> __global__ __launch_bounds__(256) void leaky_step_kernel(const LeakyArgs p)
 {
@@ -150,8 +150,8 @@ template <int DT, int ODT> int step(const LeakyArgs& p, hipStream_t s)
 // Out comes out transposed: a lane stores four consecutive columns of one step.
 //
 // Rounding (16-bit operands): W has two terms of the operands' type in (3) and P two in (2), the rounded value and what that leaves, so the output's own rounding is
-// the only one that shows (with one term of W the error against 64 bits was 1.35 - 1.4 times that of outputs rounded once; the second costs 7 - 9 %: T = 4096,
-// 64 heads of 128 x 128, bf16: 135 -> 145 us).  (4) splits lambda^(CH-j) c_j into three bf16 or two fp16 terms (24 and 23 bits), so the state keeps fp32 accuracy.
+// the only one that shows (with one term of W the error against 64 bits was 1.35 - 1.4 times that of outputs rounded once; the second costs 2 - 9 %: T = 4096,
+// 64 heads of 128 x 128, bf16: 122 -> 132 us).  (4) splits lambda^(CH-j) c_j into three bf16 or two fp16 terms (24 and 23 bits), so the state keeps fp32 accuracy.
 // fp16's range is too short for P, W and c's terms: they are scaled by powers of two, taken from the largest value of a tile of P, of a wavefront's columns of W,
 // of a column of c.  fp32 operands run on the fp32 matrix instructions.
 // ---------------------------------------------------------------------------------------------------------------------------------------------------------
@@ -458,9 +458,9 @@ __global__ __launch_bounds__(64 * WV, DA == 64 || (DA == 128 && WV == 8) ? 4 : 2
 // The tile form on 16-bit operands: chunks of 32 steps, a workgroup of four wavefronts owns 64 NT columns, a wavefront 16 NT of them (W: KA tiles of 16 rows
 // in its registers; DA is the power of two that rows have in LDS).  a, b, c of the next chunk are on their way to registers while this one is computed, then go to
 // the other of two LDS buffers: one barrier for the buffers and one for P per chunk, two workgroups on a CU.
-// Bound by the vector instructions beside the products (of some 630 in a wavefront's chunk 75 are products; the split of lambda^(CH-j) c and the conversions of W lead),
-// the output pass near memory too: 64 heads of 128 x 128, 4096 steps, bf16: 34 us for the states (134 MB), 10 for the scan, 77 for the outputs (300 MB).
-// Chunks of 64 steps in eight wavefronts took 209 us for the whole, this form 118.
+// Bound by the vector instructions beside the products (of 784 in a wavefront's chunk 91 are products; the split of lambda^(CH-j) c and the terms of W lead): they issue
+// 59 % of the output pass's time, the matrix cores are busy 28 % of it.  64 heads of 128 x 128, 4096 steps, bf16: 38 us for the states (134 MB), 10 for the scan, 89 for the
+// outputs (300 MB).  Chunks of 64 steps in eight wavefronts took 209 us for the whole where this form took 118 (both with one term of W).
 // Rows are unpadded; the 16-byte granule q of row r lies in slot q ^ f(r), f chosen so that the three ways they are read (a granule of 16 rows, half granules
 // of 16 rows, and the transposing 4 x 16 read) meet no bank twice.
 // ---------------------------------------------------------------------------------------------------------------------------------------------------------
@@ -973,11 +973,11 @@ __global__ __launch_bounds__(256) void leaky_scan_kernel(float* __restrict__ ws,
 template <int DT> struct LeakyShape {
     static constexpr int CH = 32;
     static int pad(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
-    // row tiles of a state in a kernel's registers: three quarters of the padded width where they suffice (2048 steps, bf16: 64 heads of 96 x 96 66 -> 61 us, 32 of
-    // 192 x 192 95 -> 81; the fp32 kernel leaves tiles out as it runs)
+    // row tiles of a state in a kernel's registers: three quarters of the padded width where they suffice (2048 steps, bf16: 64 heads of 96 x 96 76 -> 68 us, 32 of
+    // 192 x 192 101 -> 88; the fp32 kernel leaves tiles out as it runs)
     static int row_tiles(int d) { return DT != SS_SEQ_F32 && d > 64 && d <= pad(d) / 4 * 3 ? pad(d) / 64 * 3 : pad(d) / 16; }
     // columns of a workgroup's block: 64 where the state of 128 would not leave two workgroups on a CU (16-bit heads over 128 wide; 2048 steps, 32 heads, bf16:
-    // 256 x 256 in blocks of 128 174 us, of 64 119; 192 x 192 167 and 95), else up to 128
+    // 256 x 256 in blocks of 128 174 us, of 64 119; 192 x 192 167 and 95, with one term of W), else up to 128
     static int cols(int DA, int DC) { return DC <= 64 || (DT != SS_SEQ_F32 && DA > 128) ? 64 : 128; }
     static int blocks(int DA, int DC) { return (DC + cols(DA, DC) - 1) / cols(DA, DC); }
     static LeakyPlan plan(int T, int B, int H, int DA, int DC)
@@ -986,8 +986,8 @@ template <int DT> struct LeakyShape {
         r.ncb = r.sncb = blocks(DA, DC);
         // Segments: the count with the least estimated time, in chunks.  A round of workgroups (two on a CU; one for fp32, whose matrix instructions one workgroup
         // fills) takes a segment's chunks and two for its state; the state pass half of that; joining costs half a chunk per state in the output pass up to 5
-        // segments, else a scan; each further launch two.  (64 heads, 4096 steps, bf16: 4 segments 123 us, 8 108, 16 135; 48 heads, 777 steps, fp32 training:
-        // 4 segments 262 us, 5 215, 7 268.)
+        // segments, else a scan; each further launch two.  (64 heads, 4096 steps, bf16: 4 segments 152 us, 8 132, 16 169; 48 heads, 777 steps, fp32 training:
+        // 4 segments 179 us, 5 147, 7 165.)
         const int chunks = (T + CH - 1) / CH;
         const double base = (double)B * H * r.ncb, slots = DT == SS_SEQ_F32 ? 256. : 512.;
         int best = 1;
@@ -1069,7 +1069,7 @@ template <int DT> struct LeakyShape {
     static int run(const LeakyArgs& p, float* ws, hipStream_t s)
     {
         // one step has its own kernel; from two on a tile (8 heads of 64 x 64, bf16: a kernel that walks the steps 4.8 us for 2, 6.4 for 4, 9.3 for 7, the tile form
-        // 6.5 for any; 128 heads of 128 x 128: 54, 70 and 95 against 14)
+        // 7 for any; 128 heads of 128 x 128: 54, 70 and 95 against 15)
         if (p.T == 1) return p.out_f32 ? step<DT, SS_SEQ_F32>(p, s) : step<DT, DT>(p, s);
         const LeakyPlan r = plan(p.T, p.B, p.H, p.DA, p.DC);
         if (int rc = states(p, r, ws, s)) return rc;

@@ -1,8 +1,6 @@
 // ss_seq_common.hpp — shared device helpers of the ss_seq_*.hip units (sequence operators).
 #pragma once
 #include <hip/hip_runtime.h>
-#include <hip/hip_fp16.h>
-#include <hip/hip_bf16.h>
 #include <stdint.h>
 #include <math.h>
 #include <type_traits>
@@ -12,7 +10,6 @@
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));

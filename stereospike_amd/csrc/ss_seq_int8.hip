@@ -5,7 +5,7 @@
 // The sum is exact in 32 bits for K < 131072 (128 * 128 * 131071 < 2^31), so no order of summation and no split over k changes a result.
 //
 // Three forms, by a rule on the sizes alone (choose()):
-//   rows   one operand has at most 64 rows: the other is streamed once from memory, straight into matrix operands (bound by reading it).
+//   rows   at most 32 tokens, or at most 64 channels: the other operand is streamed once from memory, straight into matrix operands (bound by reading it).
 //   tile   256 x 256 or 128 x 128 outputs per workgroup, both operands through LDS (bound by the matrix cores and LDS reads).
 //   split  the tile form over parts of k into 32-bit partials, joined by a second pass, where there are too few tiles to fill the card.
 // Rows that are not aligned to 16 bytes are copied into aligned, zero-padded rows first (tile form) or read unaligned (rows form).
@@ -31,7 +31,8 @@ __device__ __forceinline__ float scaled(int acc, float as, float ws, float bias)
 // 16 (l / 16), so one load of a wavefront is 64 consecutive bytes of 16 rows, and the product gives lane l rows 4 (l / 16) .. + 3 of X against row l % 16 of Y.
 // The four wavefronts of a workgroup take every fourth 64 k of the same 16 rows of X (256 consecutive bytes of a row at a time) and add up in LDS.
 // SWAP: X is a (few channels), else X is w (few tokens).
-// (1 x 8192 x 4096, 33.6 MB: 8.2 us, 4.1 TB/s: 128 KB of each workgroup's rows are one burst and its latency.)
+// (1 x 8192 x 4096, 33.6 MB: 12 us with another weight every call, 2.8 TB/s, 9 with the same one, which the L2 caches hold in part: 64 KB of a workgroup's rows are two
+// bursts and their latency.)
 // ---------------------------------------------------------------------------------------------------------------------------------------------------------
 template <int DT, int MT, bool SWAP> __global__ __launch_bounds__(256) void mm_rows_kernel(const MmArgs p)
 {

@@ -56,7 +56,7 @@ template <int TPR, int NE> __device__ __forceinline__ float rstd_of(float s, con
 }
 
 // HBM-bound; the next row's loads are under way while a row is reduced and written.  (bf16, 16384 x 4096 with a residual: 537 MB in 103 us, 5.2 TB/s; in 8 bits 470 MB
-// in 115 us, 4.1 TB/s: the codes' roundings and the exact decision next to a border show.)
+// in 111 us, 4.2 TB/s: the codes' roundings and the exact decision next to a border show.)
 template <int DT, int VEC, int TPR, int NV, bool INT8>
 __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_fwd_kernel(const NormArgs p)
 {
@@ -187,7 +187,7 @@ struct NormBwdArgs {
 };
 
 // g_h = rstd (w g_y - n mean(w g_y n)) + g_sum in one pass over h, g_y, g_sum; a block keeps its rows' part of the weight's gradient in registers and leaves one row
-// of partials, so no atomics.  HBM-bound (29920 x 512, bf16, both gradients: 123 MB in 26 us, 4.7 TB/s).
+// of partials, so no atomics.  HBM-bound (29920 x 512, bf16, both gradients: 123 MB in 28 us, 4.4 TB/s).
 template <int DT, int VEC, int TPR, int NV>
 __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_bwd_kernel(const NormBwdArgs p)
 {

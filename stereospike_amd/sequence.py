@@ -13,6 +13,8 @@ library and HIP tensors, launch on torch's current stream of the tensors' device
 into a HIP graph; there is no eager fallback, and tracers (torch.jit.trace, torch.fx) and
 forward-mode derivatives are refused.  A backward pass that is itself captured needs leaves whose gradients no live eager graph reaches
 (engine.GraphedTrainer shows how).  Gradients are first derivatives: differentiating them again raises.
+Nothing is cast: torch.autocast does not reach these functions (cast a 16-bit x and its residual to one type), and log_decay, norm weights and scales stay fp32
+(net.half() and the like turn the layers' into a type that is refused; convert the activations instead).
 
 Calls go straight to the library (csrc/ss_seq_torch.cpp), which checks, allocates and launches; it hands a call with unfit operands back, and the functions
 here then raise the SSNeuronError that names the operand.
@@ -87,7 +89,7 @@ def _refuse_attention(q, k, v, log_decay, state, lengths, lead):
         raise SSNeuronError(f'{q.shape[0]} steps: at most {_seqlib.MAX_STEPS} in one call')
     _operand(log_decay, 'log_decay', dev, torch.float32, (H,))
     if lead == 2 and log_decay.requires_grad and torch.is_grad_enabled():
-        raise SSNeuronError('log_decay: the decay of a head is a constant of the layer (as tau of a LIFNode); it has no gradient — pass log_decay.detach()')
+        raise SSNeuronError('log_decay: the decay of a head is a constant here (as tau of a LIFNode, unlike a ParametricLIFNode\'s); it has no gradient — pass log_decay.detach()')
     if state is not None:
         _operand(state, 'state', dev, torch.float32, (B, H, Dk, Dv))
     if lengths is not None:
@@ -110,13 +112,13 @@ def leaky_attention(q_seq: torch.Tensor, k_seq: torch.Tensor, v_seq: torch.Tenso
 
     q_seq [T, B, H, Dk], k_seq [T, B, Hk, Dk], v_seq [T, B, Hk, Dv] in one of float32 / float16 / bfloat16 with any strides (a last axis that is not
     contiguous is copied); H is a multiple of Hk and query head h reads key / value head h // (H // Hk).  Dk, Dv <= 256.  log_decay fp32 [H], <= 0: the log of
-    lambda (1 - 1 / tau of a leaky integrator; -inf forgets at once).  scale: Dk ** -0.5 by default.
+    lambda (1 - 1 / tau of a leaky integrator; -inf forgets at once); it has no gradient.  scale: Dk ** -0.5 by default.
     state: fp32 [B, H, Dk, Dv], S before the first step (None: zero).  lengths: int32 [B] on the device, the valid steps of each stream (clamped to 0 .. T);
     rows behind them are not read, their outputs and gradients are zero.
     A NaN or an infinity reaches its own step's output and, through the state, its head's later steps (a value's: in its column), never an earlier step, another
     stream or another head; the state's entries that held it are infinite or NaN from there on.
-    Returns o_seq [T, B, H, Dv]; with return_state also the state after the last valid step (fp32).  States, sums and decays are fp32.  Gradients: q, k, v and
-    state, from both results."""
+    Returns o_seq [T, B, H, Dv]; with return_state also the state after the last valid step (fp32).  States, sums and decays are fp32, outputs and gradients are
+    rounded once.  Gradients: q, k, v and state, from both results."""
     out, last = _call('leaky_attention', lambda: _refuse_attention(q_seq, k_seq, v_seq, log_decay, state, lengths, 2), q_seq, k_seq, v_seq, log_decay, scale, state, lengths)
     return (out, last) if return_state else out
 
