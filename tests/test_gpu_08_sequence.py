@@ -6,6 +6,7 @@ import math
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from stereospike_amd import sequence
 from stereospike_amd.clock_driven import functional, layer
@@ -1095,3 +1096,28 @@ def test_layer_of_no_steps():
     for bad in (q[0], q[None]):
         with pytest.raises(sequence.SSNeuronError):
             att.forward_sequence(bad, k, v)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_gradients_under_checkpointing_and_saved_tensor_hooks(dtype):
+    """What the backward pass needs is saved as tensors are: recomputed (checkpoint) or kept on the host meanwhile, the gradients are bit for bit those without."""
+    g = gen(24)
+    q, k, v = (normal(g, 300, 2, h, 64, dtype=dtype).to(DEV).transpose(0, 1).contiguous().transpose(0, 1).requires_grad_() for h in (4, 2, 2))
+    s, w = normal(g, 2, 4, 64, 64).to(DEV).requires_grad_(), (1 + normal(g, 64, std=0.1)).to(DEV).requires_grad_()
+    decay, n = torch.tensor([-0.1, -0.01, -0.5, 0.], device=DEV), torch.tensor([300, 120], dtype=torch.int32, device=DEV)
+    leaves = (q, k, v, s, w)
+
+    def run(q, k, v, s, w):
+        o, last = sequence.leaky_attention(q, k, v, decay, state=s, lengths=n, return_state=True)
+        y, h = sequence.add_rms_norm(o, w, q)
+        return y, sequence.add_rms_norm_int8(y, w, h)[2], last
+
+    def grads(outs):
+        return torch.autograd.grad(sum(t.float().square().sum() for t in outs), leaves)
+
+    want = grads(run(*leaves))
+    with torch.autograd.graph.save_on_cpu():
+        kept = run(*leaves)
+    for got in (grads(torch.utils.checkpoint.checkpoint(run, *leaves, use_reentrant=False)), grads(kept)):
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
