@@ -459,7 +459,7 @@ __global__ __launch_bounds__(64 * WV, DA == 64 || (DA == 128 && WV == 8) ? 4 : 2
 // in its registers; DA is the power of two that rows have in LDS).  a, b, c of the next chunk are on their way to registers while this one is computed, then go to
 // the other of two LDS buffers: one barrier for the buffers and one for P per chunk, two workgroups on a CU.
 // Bound by the vector instructions beside the products (of 784 in a wavefront's chunk 91 are products; the split of lambda^(CH-j) c and the terms of W lead): they issue
-// 59 % of the output pass's time, the matrix cores are busy 28 % of it.  64 heads of 128 x 128, 4096 steps, bf16: 38 us for the states (134 MB), 10 for the scan, 89 for the
+// 59 % of the output pass's time, the matrix cores are busy 28 % of it.  64 heads of 128 x 128, 4096 steps, bf16: 38 us for the states (134 MB), 10 for the scan, 87 for the
 // outputs (300 MB).  Chunks of 64 steps in eight wavefronts took 209 us for the whole where this form took 118 (both with one term of W).
 // Rows are unpadded; the 16-byte granule q of row r lies in slot q ^ f(r), f chosen so that the three ways they are read (a granule of 16 rows, half granules
 // of 16 rows, and the transposing 4 x 16 read) meet no bank twice.
